@@ -451,6 +451,59 @@ VS_API vs_status vs_gather_stats(vs_ctx* ctx, uint32_t n, float* refine_norm, fl
 VS_API vs_status vs_noise_means(vs_ctx* ctx, uint32_t n, float* transforms, const float* opacities,
                                 const float* visible, float scale, float limit, uint32_t seed);
 
+/* ---- row operators of a learned head over splats ---------------------------
+ * Dropout, layer norm and the two joined, forward and backward, on rows x cols
+ * values of one element type, for the residual blocks of a network that reads
+ * per-splat features (no counterpart in the reference).  Sums and statistics
+ * are f32; each output is rounded to its type once.
+ *
+ * Inputs named with a stride hold row r at r * stride elements (a stride of 0
+ * stands for cols); everything else is contiguous.  Buffers need the alignment
+ * of their element; whole 16-byte vectors are used where base and rows allow.
+ * An output may be the same buffer as an input of the same call that is
+ * contiguous and of its shape; buffers that overlap otherwise are not allowed.
+ * rows may be 0 (the weight gradients are then zeros).
+ *
+ * Dropout's mask is a function of (seed, offset, index), index = row * cols +
+ * col, and is never stored: with t = round(65536 p) (at most 65535 unless p is
+ * 1), the value is kept when its 16-bit number is at least t and multiplied by
+ * 65536 / (65536 - t); dropped values give 0 whatever they hold.  The number is
+ * half-word index % 8 (low half first) of the four words of Philox 4x32 with
+ * ten rounds for the counter (index / 8, offset), low words first, and the key
+ * seed.  Calls that must not share a mask take different offsets. */
+typedef enum vs_dtype { VS_F32 = 0, VS_F16 = 1, VS_BF16 = 2 } vs_dtype;
+
+/* y = dropout(x); with the gradient of y as x it gives the gradient of x. */
+VS_API vs_status vs_dropout(vs_ctx* ctx, uint64_t count, int32_t dtype, const void* x, double p, uint64_t seed,
+                            uint64_t offset, void* y);
+/* y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps), mean and var
+ * over each row.  weight and bias ([cols], f32 or the rows' type) may be NULL
+ * (ones, zeros), mean and rstd ([rows] f32, what the backward reads) too. */
+VS_API vs_status vs_layer_norm(vs_ctx* ctx, uint64_t rows, uint32_t cols, int32_t dtype, int32_t weight_dtype,
+                               const void* x, uint64_t x_stride, const void* weight, const void* bias, float eps,
+                               void* y, float* mean, float* rstd);
+/* dx, dweight, dbias of vs_layer_norm; dweight and dbias ([cols], of
+ * weight_dtype) may be NULL.  Their sums over the rows are taken in a fixed
+ * order: equal inputs give equal bits. */
+VS_API vs_status vs_layer_norm_backward(vs_ctx* ctx, uint64_t rows, uint32_t cols, int32_t dtype,
+                                        int32_t weight_dtype, const void* dy, uint64_t dy_stride, const void* x,
+                                        uint64_t x_stride, const void* weight, const float* mean, const float* rstd,
+                                        void* dx, void* dweight, void* dbias);
+/* z = residual + dropout(x), rounded to the rows' type, and y, mean, rstd of
+ * the layer norm of z. */
+VS_API vs_status vs_dropout_add_norm(vs_ctx* ctx, uint64_t rows, uint32_t cols, int32_t dtype, int32_t weight_dtype,
+                                     const void* x, uint64_t x_stride, const void* residual, uint64_t residual_stride,
+                                     const void* weight, const void* bias, double p, uint64_t seed, uint64_t offset,
+                                     float eps, void* y, void* z, float* mean, float* rstd);
+/* Its gradient: dresidual = dz + the layer norm's gradient (dz, the gradient
+ * that reaches z past the norm, may be NULL), dx = dropout(dresidual). */
+VS_API vs_status vs_dropout_add_norm_backward(vs_ctx* ctx, uint64_t rows, uint32_t cols, int32_t dtype,
+                                              int32_t weight_dtype, const void* dy, uint64_t dy_stride,
+                                              const void* dz, uint64_t dz_stride, const void* z, uint64_t z_stride,
+                                              const void* weight, const float* mean, const float* rstd, double p,
+                                              uint64_t seed, uint64_t offset, void* dx, void* dresidual,
+                                              void* dweight, void* dbias);
+
 /* ---- building blocks exposed for tests ------------------------------------ */
 /* Stable LSD radix sort of (key, value) u32 pairs on bits [0, key_bits). */
 VS_API vs_status vs_radix_sort_pairs(vs_ctx* ctx, uint32_t* keys, uint32_t* values, uint32_t count,

@@ -66,6 +66,8 @@ class PeerSet(ctypes.Structure):
                 ("cams", c_vp * PEER_MAX), ("view_masks", c_vp * PEER_MAX)]
 
 
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2  # vs_dtype
+
 COMPACT_ROW = 16  # VS_COMPACT_ROW: floats per splat of vs_vjp_compact
 
 
@@ -163,6 +165,20 @@ _SIGS = {
     "vs_gather_stats": ([c_vp, ctypes.c_uint32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp], ctypes.c_int),
     "vs_noise_means": ([c_vp, ctypes.c_uint32, c_vp, c_vp, c_vp, ctypes.c_float, ctypes.c_float, ctypes.c_uint32],
                        ctypes.c_int),
+    "vs_dropout": ([c_vp, ctypes.c_uint64, ctypes.c_int32, c_vp, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64,
+                    c_vp], ctypes.c_int),
+    "vs_layer_norm": ([c_vp, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int32, ctypes.c_int32, c_vp, ctypes.c_uint64,
+                       c_vp, c_vp, ctypes.c_float, c_vp, c_vp, c_vp], ctypes.c_int),
+    "vs_layer_norm_backward": ([c_vp, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int32, ctypes.c_int32, c_vp,
+                                ctypes.c_uint64, c_vp, ctypes.c_uint64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp],
+                               ctypes.c_int),
+    "vs_dropout_add_norm": ([c_vp, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int32, ctypes.c_int32, c_vp,
+                             ctypes.c_uint64, c_vp, ctypes.c_uint64, c_vp, c_vp, ctypes.c_double, ctypes.c_uint64,
+                             ctypes.c_uint64, ctypes.c_float, c_vp, c_vp, c_vp, c_vp], ctypes.c_int),
+    "vs_dropout_add_norm_backward": ([c_vp, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int32, ctypes.c_int32, c_vp,
+                                      ctypes.c_uint64, c_vp, ctypes.c_uint64, c_vp, ctypes.c_uint64, c_vp, c_vp, c_vp,
+                                      ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, c_vp, c_vp, c_vp, c_vp],
+                                     ctypes.c_int),
     "vs_radix_sort_pairs": ([c_vp, c_vp, c_vp, ctypes.c_uint32, ctypes.c_uint32], ctypes.c_int),
     "vs_radix_sort_pairs_static": ([c_vp, c_vp, c_vp, ctypes.c_uint32, ctypes.c_uint32], ctypes.c_int),
     "vs_scan_inclusive": ([c_vp, c_vp, ctypes.c_uint32, c_vp], ctypes.c_int),

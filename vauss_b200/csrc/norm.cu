@@ -1,0 +1,321 @@
+// Layer norm over rows and its gradient, alone or joined with the dropout and
+// the residual sum before it (z = residual + dropout(x), y = layer norm of z).
+//
+//   forward   m = mean z, v = mean (z - m)^2, q = 1 / sqrt(v + eps),
+//             y = (z - m) q w + b
+//   backward  h = (z - m) q, g = dy w,
+//             t = q (g - mean g - h mean(g h)) (+ dz),
+//             dresidual = t, dx = dropout(t), dw = sum_rows dy h, db = sum_rows dy
+#include "rows.cuh"
+
+namespace {
+
+using namespace vs;
+
+// Rows of `cols` values that start `stride` values apart.
+template <typename T> struct Mat {
+  T* p;
+  uint64_t stride;
+  VSD T* row(uint64_t r) const { return p + r * stride; }
+};
+
+struct Shape {
+  uint64_t rows;
+  uint32_t cols;
+};
+
+// One CTA per row, three passes over it: any width, stride and alignment.  The
+// mean is a quotient, not a product with 1 / cols, so that a constant row whose
+// sum is exact has a variance of exactly zero.
+template <typename T, bool kJoin>
+__global__ void __launch_bounds__(256) norm_fwd_rows_kernel(Shape s, Mat<const T> x, Mat<const T> residual, Weights wt,
+                                                            float eps, const Dropout d, T* y, T* z, float* mean,
+                                                            float* rstd) {
+  __shared__ float scratch[33];
+  const float cols = (float)s.cols;
+  for (uint64_t r = blockIdx.x; r < s.rows; r += gridDim.x) {
+    const T* in = x.row(r);
+    T* out = y + r * s.cols;
+    T* zr = kJoin ? z + r * s.cols : nullptr;
+    float sum = 0.0f;
+    for (uint64_t c = threadIdx.x; c < s.cols; c += blockDim.x) {
+      if (kJoin) {
+        float v = to_f32(in[c]);
+        if (d.threshold) v = dropped(v, keep_at(d, r * s.cols + c), d.scale);
+        const T zc = from_f32<T>(to_f32(residual.row(r)[c]) + v);
+        zr[c] = zc;
+        sum += to_f32(zc);
+      } else {
+        sum += to_f32(in[c]);
+      }
+    }
+    const T* src = kJoin ? zr : in;
+    const float m = block_sum(sum, scratch) / cols;
+    float sq = 0.0f;
+    for (uint64_t c = threadIdx.x; c < s.cols; c += blockDim.x) {
+      const float e = to_f32(src[c]) - m;
+      sq = fmaf(e, e, sq);
+    }
+    const float q = rsqrtf(block_sum(sq, scratch) / cols + eps);
+    for (uint64_t c = threadIdx.x; c < s.cols; c += blockDim.x) {
+      const float w = wt.weight ? load_as(wt.weight, wt.dtype, c) : 1.0f;
+      const float b = wt.bias ? load_as(wt.bias, wt.dtype, c) : 0.0f;
+      out[c] = from_f32<T>(fmaf((to_f32(src[c]) - m) * q, w, b));
+    }
+    if (threadIdx.x == 0) {
+      if (mean) mean[r] = m;
+      if (rstd) rstd[r] = q;
+    }
+  }
+}
+
+template <typename T, bool kJoin>
+__global__ void __launch_bounds__(256) norm_bwd_rows_kernel(Shape s, Mat<const T> dy, Mat<const T> dz, Mat<const T> z,
+                                                            Weights wt, const float* mean, const float* rstd,
+                                                            const Dropout d, T* dx, T* dresidual) {
+  __shared__ float scratch[33];
+  const float cols = (float)s.cols;
+  for (uint64_t r = blockIdx.x; r < s.rows; r += gridDim.x) {
+    const float m = mean[r], q = rstd[r];
+    const T *gy = dy.row(r), *zr = z.row(r);
+    float sg = 0.0f, sgh = 0.0f;
+    for (uint64_t c = threadIdx.x; c < s.cols; c += blockDim.x) {
+      const float g = to_f32(gy[c]) * (wt.weight ? load_as(wt.weight, wt.dtype, c) : 1.0f);
+      sg += g;
+      sgh = fmaf(g, (to_f32(zr[c]) - m) * q, sgh);
+    }
+    sg = block_sum(sg, scratch) / cols;
+    sgh = block_sum(sgh, scratch) / cols;
+    for (uint64_t c = threadIdx.x; c < s.cols; c += blockDim.x) {
+      const float g = to_f32(gy[c]) * (wt.weight ? load_as(wt.weight, wt.dtype, c) : 1.0f);
+      float t = q * (g - sg - (to_f32(zr[c]) - m) * q * sgh);
+      if (kJoin) {
+        if (dz.p) t += to_f32(dz.row(r)[c]);
+        float v = t;
+        if (d.threshold) v = dropped(t, keep_at(d, r * s.cols + c), d.scale);
+        dresidual[r * s.cols + c] = from_f32<T>(t);
+        dx[r * s.cols + c] = from_f32<T>(v);
+      } else {
+        dx[r * s.cols + c] = from_f32<T>(t);
+      }
+    }
+  }
+}
+
+// Column sums of a strip of rows: partial[strip][0] = sum dy h, [1] = sum dy.
+// 32 columns x 8 rows of threads; each thread's rows are summed in order, then
+// the eight in order, so the result does not depend on timing.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_cols_kernel(Shape s, Mat<const T> dy, Mat<const T> z, const float* mean,
+                                                        const float* rstd, uint64_t strip, float* partial) {
+  __shared__ float sw[8][32], sb[8][32];
+  const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x;
+  const uint64_t r0 = blockIdx.y * strip;
+  const uint64_t r1 = r0 + strip < s.rows ? r0 + strip : s.rows;
+  float w = 0.0f, b = 0.0f;
+  if (c < s.cols) {
+    for (uint64_t r = r0 + threadIdx.y; r < r1; r += 8) {
+      const float g = to_f32(dy.row(r)[c]);
+      w = fmaf(g, (to_f32(z.row(r)[c]) - mean[r]) * rstd[r], w);
+      b += g;
+    }
+  }
+  sw[threadIdx.y][threadIdx.x] = w;
+  sb[threadIdx.y][threadIdx.x] = b;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < s.cols) {
+    for (int k = 1; k < 8; ++k) {
+      w += sw[k][threadIdx.x];
+      b += sb[k][threadIdx.x];
+    }
+    float* out = partial + (uint64_t)blockIdx.y * 2 * s.cols;
+    out[c] = w;
+    out[s.cols + c] = b;
+  }
+}
+
+// dw and db from the strips' partial sums, 32 columns x 32 strips of threads.
+__global__ void __launch_bounds__(1024) norm_join_kernel(uint32_t cols, uint32_t strips, const float* partial,
+                                                         int32_t dtype, void* dweight, void* dbias) {
+  __shared__ float sw[32][33], sb[32][33];
+  const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x;
+  float w = 0.0f, b = 0.0f;
+  if (c < cols) {
+    for (uint32_t k = threadIdx.y; k < strips; k += 32) {
+      w += partial[(uint64_t)k * 2 * cols + c];
+      b += partial[(uint64_t)k * 2 * cols + cols + c];
+    }
+  }
+  sw[threadIdx.y][threadIdx.x] = w;
+  sb[threadIdx.y][threadIdx.x] = b;
+  __syncthreads();
+  w = warp_sum(sw[threadIdx.x][threadIdx.y]);
+  b = warp_sum(sb[threadIdx.x][threadIdx.y]);
+  const uint64_t oc = (uint64_t)blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && oc < cols) {
+    if (dweight) store_as(dweight, dtype, oc, w);
+    if (dbias) store_as(dbias, dtype, oc, b);
+  }
+}
+
+// What every entry point checks of its shape.
+vs_status check_shape(vs_ctx* ctx, const char* what, uint64_t rows, uint32_t cols, int32_t dtype, int32_t wdtype) {
+  if (!vs_dtype_valid(dtype)) return vs_fail(ctx, VS_ERR_UNSUPPORTED, "%s: element type %d", what, dtype);
+  if (wdtype != VS_F32 && wdtype != dtype)
+    return vs_fail(ctx, VS_ERR_UNSUPPORTED, "%s: weights of type %d beside rows of type %d (f32 or the rows' type)",
+                   what, wdtype, dtype);
+  if (cols == 0) return vs_fail(ctx, VS_ERR_INVALID, "%s: rows without columns", what);
+  if (cols > 0x7fffffffu || rows > (1ull << 60) / cols)
+    return vs_fail(ctx, VS_ERR_CAPACITY, "%s: %llu rows of %u columns", what, (unsigned long long)rows, cols);
+  return VS_OK;
+}
+
+// An input's buffer; a stride of 0 stands for `cols`.
+template <typename T>
+vs_status check_in(vs_ctx* ctx, const char* what, const char* name, Shape s, const void* p, uint64_t stride,
+                   Mat<const T>* out) {
+  if (stride == 0) stride = s.cols;
+  if (!p && s.rows) return vs_fail(ctx, VS_ERR_INVALID, "%s: null %s", what, name);
+  if (stride < s.cols || (s.rows > 1 && stride > (1ull << 60) / s.rows))
+    return vs_fail(ctx, VS_ERR_INVALID, "%s: %s rows %llu apart, %u wide", what, name, (unsigned long long)stride, s.cols);
+  if ((uintptr_t)p & (sizeof(T) - 1)) return vs_fail(ctx, VS_ERR_INVALID, "%s: %s is not aligned to its element", what, name);
+  *out = {static_cast<const T*>(p), stride};
+  return VS_OK;
+}
+
+vs_status check_ptr(vs_ctx* ctx, const char* what, const char* name, const void* p, size_t align, bool needed) {
+  if (needed && !p) return vs_fail(ctx, VS_ERR_INVALID, "%s: null %s", what, name);
+  if ((uintptr_t)p & (align - 1)) return vs_fail(ctx, VS_ERR_INVALID, "%s: %s is not aligned to its element", what, name);
+  return VS_OK;
+}
+
+uint32_t row_grid(uint64_t rows) { return (uint32_t)(rows < 0x7fffffffull ? rows : 0x7fffffffull); }
+
+template <typename T, bool kJoin>
+vs_status norm_forward(vs_ctx* ctx, const char* what, Shape s, const void* x, uint64_t x_stride, const void* residual,
+                       uint64_t residual_stride, Weights wt, float eps, const Dropout& d, void* y, void* z,
+                       float* mean, float* rstd) {
+  Mat<const T> mx, mr{};
+  VS_TRY(check_in<T>(ctx, what, "x", s, x, x_stride, &mx));
+  if (kJoin) VS_TRY(check_in<T>(ctx, what, "residual", s, residual, residual_stride, &mr));
+  VS_TRY(check_ptr(ctx, what, "y", y, sizeof(T), s.rows > 0));
+  if (kJoin) VS_TRY(check_ptr(ctx, what, "z", z, sizeof(T), s.rows > 0));
+  VS_TRY(check_ptr(ctx, what, "mean", mean, 4, false));
+  VS_TRY(check_ptr(ctx, what, "rstd", rstd, 4, false));
+  VS_TRY(check_ptr(ctx, what, "weight", wt.weight, vs_dtype_size(wt.dtype), false));
+  VS_TRY(check_ptr(ctx, what, "bias", wt.bias, vs_dtype_size(wt.dtype), false));
+  if (!(eps >= 0.0f) || eps > 3e38f) return vs_fail(ctx, VS_ERR_INVALID, "%s: eps = %g", what, (double)eps);
+  if (s.rows == 0) return VS_OK;
+  VS_CUDA(ctx, cudaSetDevice(ctx->device));
+  norm_fwd_rows_kernel<T, kJoin><<<row_grid(s.rows), 256, 0, ctx->stream>>>(s, mx, mr, wt, eps, d, (T*)y, (T*)z, mean,
+                                                                            rstd);
+  ++ctx->launches;
+  return vs_cuda(ctx, cudaGetLastError(), "norm launch");
+}
+
+template <typename T, bool kJoin>
+vs_status norm_backward(vs_ctx* ctx, const char* what, Shape s, const void* dy, uint64_t dy_stride, const void* dz,
+                        uint64_t dz_stride, const void* z, uint64_t z_stride, Weights wt, const float* mean,
+                        const float* rstd, const Dropout& d, void* dx, void* dresidual, void* dweight, void* dbias) {
+  Mat<const T> mdy, mdz{}, mz;
+  VS_TRY(check_in<T>(ctx, what, "dy", s, dy, dy_stride, &mdy));
+  if (kJoin && dz) VS_TRY(check_in<T>(ctx, what, "dz", s, dz, dz_stride, &mdz));
+  VS_TRY(check_in<T>(ctx, what, kJoin ? "z" : "x", s, z, z_stride, &mz));
+  VS_TRY(check_ptr(ctx, what, "mean", mean, 4, s.rows > 0));
+  VS_TRY(check_ptr(ctx, what, "rstd", rstd, 4, s.rows > 0));
+  VS_TRY(check_ptr(ctx, what, "dx", dx, sizeof(T), s.rows > 0));
+  if (kJoin) VS_TRY(check_ptr(ctx, what, "dresidual", dresidual, sizeof(T), s.rows > 0));
+  VS_TRY(check_ptr(ctx, what, "weight", wt.weight, vs_dtype_size(wt.dtype), false));
+  VS_TRY(check_ptr(ctx, what, "dweight", dweight, vs_dtype_size(wt.dtype), false));
+  VS_TRY(check_ptr(ctx, what, "dbias", dbias, vs_dtype_size(wt.dtype), false));
+  VS_CUDA(ctx, cudaSetDevice(ctx->device));
+  if (s.rows == 0) {
+    if (dweight) VS_CUDA(ctx, cudaMemsetAsync(dweight, 0, s.cols * vs_dtype_size(wt.dtype), ctx->stream));
+    if (dbias) VS_CUDA(ctx, cudaMemsetAsync(dbias, 0, s.cols * vs_dtype_size(wt.dtype), ctx->stream));
+    return VS_OK;
+  }
+  // the column sums read dy, which dx may overwrite, so they come first
+  if (dweight || dbias) {
+    const uint32_t col_blocks = (s.cols + 31) / 32;
+    const uint64_t want = 1184 / col_blocks + 1;  // CTAs for every SM
+    const uint64_t most = (s.rows + 63) / 64;
+    const uint32_t strips = (uint32_t)(want < most ? want : most);
+    const uint64_t strip = (s.rows + strips - 1) / strips;
+    float* partial = nullptr;
+    // from the stream-ordered pool: calls of one ctx on several streams do not share it
+    VS_CUDA(ctx, cudaMallocAsync((void**)&partial, (size_t)strips * 2 * s.cols * 4, ctx->stream));
+    norm_cols_kernel<T><<<dim3(col_blocks, strips), dim3(32, 8), 0, ctx->stream>>>(s, mdy, mz, mean, rstd, strip,
+                                                                                  partial);
+    norm_join_kernel<<<col_blocks, dim3(32, 32), 0, ctx->stream>>>(s.cols, strips, partial, wt.dtype, dweight, dbias);
+    ctx->launches += 2;
+    const vs_status st = vs_cuda(ctx, cudaGetLastError(), "norm column sums launch");
+    VS_CUDA(ctx, cudaFreeAsync(partial, ctx->stream));
+    VS_TRY(st);
+  }
+  norm_bwd_rows_kernel<T, kJoin><<<row_grid(s.rows), 256, 0, ctx->stream>>>(s, mdy, mdz, mz, wt, mean, rstd, d, (T*)dx,
+                                                                            (T*)dresidual);
+  ++ctx->launches;
+  return vs_cuda(ctx, cudaGetLastError(), "norm backward launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+VS_API vs_status vs_layer_norm(vs_ctx* ctx, uint64_t rows, uint32_t cols, int32_t dtype, int32_t weight_dtype,
+                               const void* x, uint64_t x_stride, const void* weight, const void* bias, float eps,
+                               void* y, float* mean, float* rstd) {
+  if (!ctx) return VS_ERR_INVALID;
+  VS_TRY(check_shape(ctx, "layer_norm", rows, cols, dtype, weight_dtype));
+  return vs_with_dtype(dtype, [&](auto tag) {
+    return norm_forward<decltype(tag), false>(ctx, "layer_norm", {rows, cols}, x, x_stride, nullptr, 0,
+                                              {weight, bias, weight_dtype}, eps, vs::Dropout{}, y, nullptr, mean,
+                                              rstd);
+  });
+}
+
+VS_API vs_status vs_layer_norm_backward(vs_ctx* ctx, uint64_t rows, uint32_t cols, int32_t dtype,
+                                        int32_t weight_dtype, const void* dy, uint64_t dy_stride, const void* x,
+                                        uint64_t x_stride, const void* weight, const float* mean, const float* rstd,
+                                        void* dx, void* dweight, void* dbias) {
+  if (!ctx) return VS_ERR_INVALID;
+  VS_TRY(check_shape(ctx, "layer_norm_backward", rows, cols, dtype, weight_dtype));
+  return vs_with_dtype(dtype, [&](auto tag) {
+    return norm_backward<decltype(tag), false>(ctx, "layer_norm_backward", {rows, cols}, dy, dy_stride, nullptr, 0, x,
+                                               x_stride, {weight, nullptr, weight_dtype}, mean, rstd, vs::Dropout{},
+                                               dx, nullptr, dweight, dbias);
+  });
+}
+
+VS_API vs_status vs_dropout_add_norm(vs_ctx* ctx, uint64_t rows, uint32_t cols, int32_t dtype, int32_t weight_dtype,
+                                     const void* x, uint64_t x_stride, const void* residual, uint64_t residual_stride,
+                                     const void* weight, const void* bias, double p, uint64_t seed, uint64_t offset,
+                                     float eps, void* y, void* z, float* mean, float* rstd) {
+  if (!ctx) return VS_ERR_INVALID;
+  VS_TRY(check_shape(ctx, "dropout_add_norm", rows, cols, dtype, weight_dtype));
+  vs::Dropout d;
+  VS_TRY(vs_make_dropout(ctx, "dropout_add_norm", p, seed, offset, &d));
+  return vs_with_dtype(dtype, [&](auto tag) {
+    return norm_forward<decltype(tag), true>(ctx, "dropout_add_norm", {rows, cols}, x, x_stride, residual,
+                                             residual_stride, {weight, bias, weight_dtype}, eps, d, y, z, mean, rstd);
+  });
+}
+
+VS_API vs_status vs_dropout_add_norm_backward(vs_ctx* ctx, uint64_t rows, uint32_t cols, int32_t dtype,
+                                              int32_t weight_dtype, const void* dy, uint64_t dy_stride,
+                                              const void* dz, uint64_t dz_stride, const void* z, uint64_t z_stride,
+                                              const void* weight, const float* mean, const float* rstd, double p,
+                                              uint64_t seed, uint64_t offset, void* dx, void* dresidual,
+                                              void* dweight, void* dbias) {
+  if (!ctx) return VS_ERR_INVALID;
+  VS_TRY(check_shape(ctx, "dropout_add_norm_backward", rows, cols, dtype, weight_dtype));
+  vs::Dropout d;
+  VS_TRY(vs_make_dropout(ctx, "dropout_add_norm_backward", p, seed, offset, &d));
+  return vs_with_dtype(dtype, [&](auto tag) {
+    return norm_backward<decltype(tag), true>(ctx, "dropout_add_norm_backward", {rows, cols}, dy, dy_stride, dz,
+                                              dz_stride, z, z_stride, {weight, nullptr, weight_dtype}, mean, rstd, d,
+                                              dx, dresidual, dweight, dbias);
+  });
+}
+
+}  // extern "C"

@@ -17,6 +17,7 @@ from . import _native as N
 from .camera import Camera
 
 _contexts: dict[int, "Context"] = {}
+_U64 = (1 << 64) - 1
 
 
 def _ptr(t: torch.Tensor | None):
@@ -393,6 +394,197 @@ def noise_means(transforms, opacities, visible, scale: float, limit: float, seed
     ctx = context(transforms.device)
     ctx.check(ctx.lib.vs_noise_means(ctx.h, transforms.shape[0], _ptr(transforms), _ptr(opacities), _ptr(visible),
                                      ctypes.c_float(scale), ctypes.c_float(limit), ctypes.c_uint32(seed)))
+
+
+# ---- row operators of a learned head over splats ---------------------------
+# Rows are the last dimension: [..., cols] tensors of one element type (f32,
+# f16 or bf16).  Inputs are contiguous, or 2-D with unit column stride (columns
+# of a wider row buffer); outputs are contiguous and may be passed in (`out`,
+# what an earlier call of the same shape returned).
+
+_DTYPES = {torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16, torch.bfloat16: N.DTYPE_BF16}
+
+
+def _row_input(t: torch.Tensor, like: torch.Tensor):
+    """(address, row stride) of a row operator's input; a stride of 0 means contiguous rows."""
+    assert t.is_cuda and t.device == like.device and t.dtype == like.dtype and t.shape == like.shape, \
+        f"row inputs share device, type and shape: {t.dtype} {tuple(t.shape)} beside {like.dtype} {tuple(like.shape)}"
+    if t.is_contiguous():
+        return t.data_ptr(), 0
+    assert t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1], \
+        f"row inputs are contiguous or 2-D with unit column stride: strides {t.stride()}"
+    return t.data_ptr(), t.stride(0)
+
+
+def _row_shape(t: torch.Tensor):
+    assert t.dim() >= 1 and t.dtype in _DTYPES, f"rows are f32, f16 or bf16 tensors [..., cols]: {t.dtype} {tuple(t.shape)}"
+    cols = t.shape[-1]
+    assert cols > 0, "rows without columns"
+    return t.numel() // cols, cols, _DTYPES[t.dtype]
+
+
+def _row_output(t: torch.Tensor, shape, dtype, like: torch.Tensor) -> int:
+    assert t.device == like.device and t.shape == shape and t.dtype == dtype and t.is_contiguous(), \
+        f"`out` holds contiguous {dtype} {tuple(shape)}: got {t.dtype} {tuple(t.shape)}"
+    return t.data_ptr()
+
+
+def _weight(w: torch.Tensor | None, x: torch.Tensor):
+    if w is None:
+        return None
+    assert w.shape == x.shape[-1:] and w.device == x.device and w.is_contiguous() and w.dtype in (torch.float32, x.dtype), \
+        f"layer-norm weights are contiguous [cols] in f32 or the rows' type: {w.dtype} {tuple(w.shape)}"
+    return w.data_ptr()
+
+
+def _weight_dtype(weight, bias, x) -> torch.dtype:
+    assert weight is None or bias is None or weight.dtype == bias.dtype, "weight and bias are of one type"
+    w = weight if weight is not None else bias
+    return torch.float32 if w is None else w.dtype
+
+
+def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Zeroes each value with probability ``p`` and scales the others so that the expectation stays.  The mask is
+    a function of (seed, offset, the value's index in x) and is never stored (vs_dropout in the header defines it);
+    give every call of a step its own ``offset``.  Any contiguous shape; ``out`` may be ``x``."""
+    assert x.is_cuda and x.is_contiguous() and x.dtype in _DTYPES, "dropout takes contiguous CUDA f32, f16 or bf16"
+    if out is None:
+        out = torch.empty_like(x)
+    y = _row_output(out, x.shape, x.dtype, x)
+    ctx = context(x.device)
+    ctx.check(ctx.lib.vs_dropout(ctx.h, x.numel(), _DTYPES[x.dtype], x.data_ptr(), p, seed & _U64, offset & _U64, y))
+    return out
+
+
+def dropout_bwd(dy: torch.Tensor, p: float, seed: int, offset: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of ``dropout``'s input: the same mask and scale on ``dy``."""
+    return dropout(dy, p, seed, offset, out)
+
+
+@dataclass
+class LayerNormOutput:
+    y: torch.Tensor  # [..., cols]
+    mean: torch.Tensor  # [rows] f32
+    rstd: torch.Tensor  # [rows] f32
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5, out: LayerNormOutput | None = None) -> LayerNormOutput:
+    """y = (x - mean) rstd weight + bias over each row, with the row statistics its backward reads."""
+    rows, cols, dtype = _row_shape(x)
+    wdtype = _weight_dtype(weight, bias, x)
+    if out is None:
+        out = LayerNormOutput(torch.empty(x.shape, dtype=x.dtype, device=x.device),
+                              torch.empty(rows, dtype=torch.float32, device=x.device),
+                              torch.empty(rows, dtype=torch.float32, device=x.device))
+    px, sx = _row_input(x, x)
+    y = _row_output(out.y, x.shape, x.dtype, x)
+    mean, rstd = (_row_output(t, (rows,), torch.float32, x) for t in (out.mean, out.rstd))
+    ctx = context(x.device)
+    ctx.check(ctx.lib.vs_layer_norm(ctx.h, rows, cols, dtype, _DTYPES[wdtype], px, sx, _weight(weight, x),
+                                    _weight(bias, x), eps, y, mean, rstd))
+    return out
+
+
+@dataclass
+class LayerNormGrads:
+    dx: torch.Tensor  # [..., cols]
+    dweight: torch.Tensor | None  # [cols], of the weight's type
+    dbias: torch.Tensor | None
+
+
+def _stat(t: torch.Tensor, rows: int, x: torch.Tensor) -> int:
+    assert t.device == x.device and t.dtype == torch.float32 and t.numel() == rows and t.is_contiguous(), \
+        f"row statistics are contiguous f32 [rows]: {t.dtype} {tuple(t.shape)}"
+    return t.data_ptr()
+
+
+def _weight_grads(cols: int, wdtype: torch.dtype, weight, with_bias, x):
+    with_bias = weight is not None if with_bias is None else with_bias
+    return (torch.empty(cols, dtype=wdtype, device=x.device) if weight is not None else None,
+            torch.empty(cols, dtype=wdtype, device=x.device) if with_bias else None)
+
+
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, mean: torch.Tensor,
+                   rstd: torch.Tensor, with_bias: bool | None = None,
+                   out: LayerNormGrads | None = None) -> LayerNormGrads:
+    """Gradients of ``layer_norm``'s input, weight and bias; the sums over the rows are taken in a fixed order.
+    ``with_bias`` asks for dbias (by default where there is a weight); ``out.dx`` may be ``dy``."""
+    rows, cols, dtype = _row_shape(x)
+    wdtype = _weight_dtype(weight, None, x)
+    if out is None:
+        out = LayerNormGrads(torch.empty(x.shape, dtype=x.dtype, device=x.device),
+                             *_weight_grads(cols, wdtype, weight, with_bias, x))
+    (pdy, sdy), (px, sx) = _row_input(dy, x), _row_input(x, x)
+    dx = _row_output(out.dx, x.shape, x.dtype, x)
+    dw, db = (None if t is None else _row_output(t, (cols,), wdtype, x) for t in (out.dweight, out.dbias))
+    ctx = context(x.device)
+    ctx.check(ctx.lib.vs_layer_norm_backward(ctx.h, rows, cols, dtype, _DTYPES[wdtype], pdy, sdy, px, sx,
+                                             _weight(weight, x), _stat(mean, rows, x), _stat(rstd, rows, x), dx, dw,
+                                             db))
+    return out
+
+
+@dataclass
+class DropoutAddNormOutput:
+    y: torch.Tensor  # [..., cols]
+    z: torch.Tensor  # residual + dropout(x), the residual stream
+    mean: torch.Tensor  # [rows] f32
+    rstd: torch.Tensor  # [rows] f32
+
+
+def dropout_add_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None,
+                     bias: torch.Tensor | None, p: float, seed: int, offset: int = 0, eps: float = 1e-5,
+                     out: DropoutAddNormOutput | None = None) -> DropoutAddNormOutput:
+    """z = residual + dropout(x) and y = layer_norm(z) in one pass (what stands between two residual blocks);
+    the mask is that of ``dropout`` on a contiguous x.  ``out.z`` may be ``residual``, ``out.y`` may be ``x``."""
+    rows, cols, dtype = _row_shape(x)
+    wdtype = _weight_dtype(weight, bias, x)
+    if out is None:
+        out = DropoutAddNormOutput(torch.empty(x.shape, dtype=x.dtype, device=x.device),
+                                   torch.empty(x.shape, dtype=x.dtype, device=x.device),
+                                   torch.empty(rows, dtype=torch.float32, device=x.device),
+                                   torch.empty(rows, dtype=torch.float32, device=x.device))
+    (px, sx), (pr, sr) = _row_input(x, x), _row_input(residual, x)
+    y, z = (_row_output(t, x.shape, x.dtype, x) for t in (out.y, out.z))
+    mean, rstd = (_row_output(t, (rows,), torch.float32, x) for t in (out.mean, out.rstd))
+    ctx = context(x.device)
+    ctx.check(ctx.lib.vs_dropout_add_norm(ctx.h, rows, cols, dtype, _DTYPES[wdtype], px, sx, pr, sr,
+                                          _weight(weight, x), _weight(bias, x), p, seed & _U64, offset & _U64, eps, y,
+                                          z, mean, rstd))
+    return out
+
+
+@dataclass
+class DropoutAddNormGrads:
+    dx: torch.Tensor  # [..., cols]
+    dresidual: torch.Tensor  # [..., cols]
+    dweight: torch.Tensor | None  # [cols], of the weight's type
+    dbias: torch.Tensor | None
+
+
+def dropout_add_norm_bwd(dy: torch.Tensor, dz: torch.Tensor | None, z: torch.Tensor, weight: torch.Tensor | None,
+                         mean: torch.Tensor, rstd: torch.Tensor, p: float, seed: int, offset: int = 0,
+                         with_bias: bool | None = None,
+                         out: DropoutAddNormGrads | None = None) -> DropoutAddNormGrads:
+    """Gradients of ``dropout_add_norm``: dresidual = dz + the norm's gradient, dx = dropout_bwd of it.  ``dz`` is
+    what reaches z past the norm (None: nothing does); ``out.dx`` may be ``dy``, ``out.dresidual`` may be ``dz``."""
+    rows, cols, dtype = _row_shape(z)
+    wdtype = _weight_dtype(weight, None, z)
+    if out is None:
+        out = DropoutAddNormGrads(torch.empty(z.shape, dtype=z.dtype, device=z.device),
+                                  torch.empty(z.shape, dtype=z.dtype, device=z.device),
+                                  *_weight_grads(cols, wdtype, weight, with_bias, z))
+    (pdy, sdy), (pz, sz) = _row_input(dy, z), _row_input(z, z)
+    pdz, sdz = (None, 0) if dz is None else _row_input(dz, z)
+    dx, dres = (_row_output(t, z.shape, z.dtype, z) for t in (out.dx, out.dresidual))
+    dw, db = (None if t is None else _row_output(t, (cols,), wdtype, z) for t in (out.dweight, out.dbias))
+    ctx = context(z.device)
+    ctx.check(ctx.lib.vs_dropout_add_norm_backward(ctx.h, rows, cols, dtype, _DTYPES[wdtype], pdy, sdy, pdz, sdz, pz,
+                                                   sz, _weight(weight, z), _stat(mean, rows, z),
+                                                   _stat(rstd, rows, z), p, seed & _U64, offset & _U64, dx, dres, dw,
+                                                   db))
+    return out
 
 
 def radix_sort_pairs(keys: torch.Tensor, values: torch.Tensor, key_bits: int = 32):
