@@ -6,23 +6,15 @@
 //   backward  h = (z - m) q, g = dy w,
 //             t = q (g - mean g - h mean(g h)) (+ dz),
 //             dresidual = t, dx = dropout(t), dw = sum_rows dy h, db = sum_rows dy
-#include "rows.cuh"
+#include <initializer_list>
+
+#include "norm.cuh"
 
 namespace {
 
 using namespace vs;
 
-// Rows of `cols` values that start `stride` values apart.
-template <typename T> struct Mat {
-  T* p;
-  uint64_t stride;
-  VSD T* row(uint64_t r) const { return p + r * stride; }
-};
-
-struct Shape {
-  uint64_t rows;
-  uint32_t cols;
-};
+using Shape = NormShape;
 
 // One CTA per row, three passes over it: any width, stride and alignment.  The
 // mean is a quotient, not a product with 1 / cols, so that a constant row whose
@@ -189,10 +181,20 @@ vs_status check_ptr(vs_ctx* ctx, const char* what, const char* name, const void*
   return VS_OK;
 }
 
+// Whether the streaming kernels can take the rows: contiguous, on 16-byte
+// aligned buffers (NULL passes).
+bool vector_rows(Shape s, std::initializer_list<uint64_t> strides, std::initializer_list<const void*> buffers) {
+  for (uint64_t stride : strides)
+    if (stride != s.cols && s.rows > 1) return false;
+  for (const void* p : buffers)
+    if ((uintptr_t)p & 15u) return false;
+  return true;
+}
+
 uint32_t row_grid(uint64_t rows) { return (uint32_t)(rows < 0x7fffffffull ? rows : 0x7fffffffull); }
 
 template <typename T, bool kJoin>
-vs_status norm_forward(vs_ctx* ctx, const char* what, Shape s, const void* x, uint64_t x_stride, const void* residual,
+vs_status norm_forward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, const void* x, uint64_t x_stride, const void* residual,
                        uint64_t residual_stride, Weights wt, float eps, const Dropout& d, void* y, void* z,
                        float* mean, float* rstd) {
   Mat<const T> mx, mr{};
@@ -207,6 +209,12 @@ vs_status norm_forward(vs_ctx* ctx, const char* what, Shape s, const void* x, ui
   if (!(eps >= 0.0f) || eps > 3e38f) return vs_fail(ctx, VS_ERR_INVALID, "%s: eps = %g", what, (double)eps);
   if (s.rows == 0) return VS_OK;
   VS_CUDA(ctx, cudaSetDevice(ctx->device));
+  if (vector_rows(s, {mx.stride, kJoin ? mr.stride : mx.stride}, {x, residual, y, z})) {
+    bool taken = false;
+    const NormFwd f{s, x, residual, wt, eps, d, y, z, mean, rstd};
+    VS_TRY(norm_stream_forward(ctx, dtype, kJoin, f, &taken));
+    if (taken) return VS_OK;
+  }
   norm_fwd_rows_kernel<T, kJoin><<<row_grid(s.rows), 256, 0, ctx->stream>>>(s, mx, mr, wt, eps, d, (T*)y, (T*)z, mean,
                                                                             rstd);
   ++ctx->launches;
@@ -214,7 +222,7 @@ vs_status norm_forward(vs_ctx* ctx, const char* what, Shape s, const void* x, ui
 }
 
 template <typename T, bool kJoin>
-vs_status norm_backward(vs_ctx* ctx, const char* what, Shape s, const void* dy, uint64_t dy_stride, const void* dz,
+vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, const void* dy, uint64_t dy_stride, const void* dz,
                         uint64_t dz_stride, const void* z, uint64_t z_stride, Weights wt, const float* mean,
                         const float* rstd, const Dropout& d, void* dx, void* dresidual, void* dweight, void* dbias) {
   Mat<const T> mdy, mdz{}, mz;
@@ -234,6 +242,13 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, Shape s, const void* dy, 
     if (dbias) VS_CUDA(ctx, cudaMemsetAsync(dbias, 0, s.cols * vs_dtype_size(wt.dtype), ctx->stream));
     return VS_OK;
   }
+  if (vector_rows(s, {mdy.stride, mz.stride, kJoin && dz ? mdz.stride : mz.stride},
+                  {dy, dz, z, dx, dresidual, mean, rstd})) {
+    bool taken = false;
+    const NormBwd f{s, dy, kJoin ? dz : nullptr, z, wt, mean, rstd, d, dx, dresidual, wt.dtype, dweight, dbias};
+    VS_TRY(norm_stream_backward(ctx, dtype, kJoin, f, &taken));
+    if (taken) return VS_OK;
+  }
   // the column sums read dy, which dx may overwrite, so they come first
   if (dweight || dbias) {
     const uint32_t col_blocks = (s.cols + 31) / 32;
@@ -246,9 +261,9 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, Shape s, const void* dy, 
     VS_CUDA(ctx, cudaMallocAsync((void**)&partial, (size_t)strips * 2 * s.cols * 4, ctx->stream));
     norm_cols_kernel<T><<<dim3(col_blocks, strips), dim3(32, 8), 0, ctx->stream>>>(s, mdy, mz, mean, rstd, strip,
                                                                                   partial);
-    norm_join_kernel<<<col_blocks, dim3(32, 32), 0, ctx->stream>>>(s.cols, strips, partial, wt.dtype, dweight, dbias);
-    ctx->launches += 2;
-    const vs_status st = vs_cuda(ctx, cudaGetLastError(), "norm column sums launch");
+    ++ctx->launches;
+    vs_status st = vs_cuda(ctx, cudaGetLastError(), "norm column sums launch");
+    if (st == VS_OK) st = norm_join_partials(ctx, s.cols, strips, partial, wt.dtype, dweight, dbias);
     VS_CUDA(ctx, cudaFreeAsync(partial, ctx->stream));
     VS_TRY(st);
   }
@@ -260,6 +275,13 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, Shape s, const void* dy, 
 
 }  // namespace
 
+vs_status norm_join_partials(vs_ctx* ctx, uint32_t cols, uint32_t strips, const float* partial, int32_t dtype,
+                             void* dweight, void* dbias) {
+  norm_join_kernel<<<(cols + 31) / 32, dim3(32, 32), 0, ctx->stream>>>(cols, strips, partial, dtype, dweight, dbias);
+  ++ctx->launches;
+  return vs_cuda(ctx, cudaGetLastError(), "norm weight gradient launch");
+}
+
 extern "C" {
 
 VS_API vs_status vs_layer_norm(vs_ctx* ctx, uint64_t rows, uint32_t cols, int32_t dtype, int32_t weight_dtype,
@@ -268,7 +290,7 @@ VS_API vs_status vs_layer_norm(vs_ctx* ctx, uint64_t rows, uint32_t cols, int32_
   if (!ctx) return VS_ERR_INVALID;
   VS_TRY(check_shape(ctx, "layer_norm", rows, cols, dtype, weight_dtype));
   return vs_with_dtype(dtype, [&](auto tag) {
-    return norm_forward<decltype(tag), false>(ctx, "layer_norm", {rows, cols}, x, x_stride, nullptr, 0,
+    return norm_forward<decltype(tag), false>(ctx, "layer_norm", dtype, {rows, cols}, x, x_stride, nullptr, 0,
                                               {weight, bias, weight_dtype}, eps, vs::Dropout{}, y, nullptr, mean,
                                               rstd);
   });
@@ -281,7 +303,7 @@ VS_API vs_status vs_layer_norm_backward(vs_ctx* ctx, uint64_t rows, uint32_t col
   if (!ctx) return VS_ERR_INVALID;
   VS_TRY(check_shape(ctx, "layer_norm_backward", rows, cols, dtype, weight_dtype));
   return vs_with_dtype(dtype, [&](auto tag) {
-    return norm_backward<decltype(tag), false>(ctx, "layer_norm_backward", {rows, cols}, dy, dy_stride, nullptr, 0, x,
+    return norm_backward<decltype(tag), false>(ctx, "layer_norm_backward", dtype, {rows, cols}, dy, dy_stride, nullptr, 0, x,
                                                x_stride, {weight, nullptr, weight_dtype}, mean, rstd, vs::Dropout{},
                                                dx, nullptr, dweight, dbias);
   });
@@ -296,7 +318,7 @@ VS_API vs_status vs_dropout_add_norm(vs_ctx* ctx, uint64_t rows, uint32_t cols, 
   vs::Dropout d;
   VS_TRY(vs_make_dropout(ctx, "dropout_add_norm", p, seed, offset, &d));
   return vs_with_dtype(dtype, [&](auto tag) {
-    return norm_forward<decltype(tag), true>(ctx, "dropout_add_norm", {rows, cols}, x, x_stride, residual,
+    return norm_forward<decltype(tag), true>(ctx, "dropout_add_norm", dtype, {rows, cols}, x, x_stride, residual,
                                              residual_stride, {weight, bias, weight_dtype}, eps, d, y, z, mean, rstd);
   });
 }
@@ -312,7 +334,7 @@ VS_API vs_status vs_dropout_add_norm_backward(vs_ctx* ctx, uint64_t rows, uint32
   vs::Dropout d;
   VS_TRY(vs_make_dropout(ctx, "dropout_add_norm_backward", p, seed, offset, &d));
   return vs_with_dtype(dtype, [&](auto tag) {
-    return norm_backward<decltype(tag), true>(ctx, "dropout_add_norm_backward", {rows, cols}, dy, dy_stride, dz,
+    return norm_backward<decltype(tag), true>(ctx, "dropout_add_norm_backward", dtype, {rows, cols}, dy, dy_stride, dz,
                                               dz_stride, z, z_stride, {weight, nullptr, weight_dtype}, mean, rstd, d,
                                               dx, dresidual, dweight, dbias);
   });

@@ -1,0 +1,220 @@
+// The layer-norm kernels' shared pieces: shapes, the bulk-copy ring that feeds
+// the streaming kernels, and the launchers norm.cu chooses between.
+#pragma once
+
+#include "rows.cuh"
+
+namespace vs {
+
+// Rows of `cols` values that start `stride` values apart.
+template <typename T> struct Mat {
+  T* p;
+  uint64_t stride;
+  VSD T* row(uint64_t r) const { return p + r * stride; }
+};
+
+struct NormShape {
+  uint64_t rows;
+  uint32_t cols;
+};
+
+// ---- bulk copies into shared memory ---------------------------------------
+VSD uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+VSD void mbar_init(uint64_t* b, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
+}
+VSD void mbar_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+VSD void mbar_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
+}
+VSD bool mbar_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Waits for a copy to land; false after about a second without it.
+constexpr uint32_t COPY_SPIN_LIMIT = 1u << 22;
+VSD bool mbar_wait(uint64_t* b, uint32_t parity) {
+  for (uint32_t spins = 0; spins < COPY_SPIN_LIMIT; ++spins)
+    if (mbar_try(b, parity)) return true;
+  return false;
+}
+// dst, src 16-byte aligned, bytes a multiple of 16
+VSD void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+VSD void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)),
+               "r"(bytes)
+               : "memory");
+}
+VSD void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// all but the newest `N` groups of stores have been read out of shared memory
+template <int N> VSD void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+template <int N> VSD void bulk_wait() { asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory"); }
+VSD void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A run [begin, end) of bytes of a 16-byte aligned buffer of `total` bytes, as
+// bulk copies see it: they move the aligned pieces that cover the run, [lo, hi);
+// where the buffer's last piece is not whole, its bytes [hi, end) are copied by
+// hand.  In shared memory the run starts `shift` bytes into its slot.
+struct Span {
+  uint64_t begin, end, lo;
+  uint32_t bytes;  // hi - lo
+  uint32_t shift;
+};
+VSD Span span_of(uint64_t begin, uint64_t end, uint64_t total) {
+  Span s;
+  s.begin = begin;
+  s.end = end;
+  s.lo = begin & ~15ull;
+  uint64_t hi = (end + 15) & ~15ull;
+  if (hi > (total & ~15ull)) hi = total & ~15ull;
+  s.bytes = hi > s.lo ? (uint32_t)(hi - s.lo) : 0;
+  s.shift = (uint32_t)begin & 15u;
+  return s;
+}
+
+VSD void span_load(const Span& s, void* slot, const void* base, uint64_t* bar) {
+  if (s.bytes) bulk_load(slot, static_cast<const char*>(base) + s.lo, s.bytes, bar);
+}
+// The bytes the bulk copy left out, by `threads` threads; the caller
+// synchronises them.
+template <typename U>
+VSD void span_tail(const Span& s, void* slot, const void* base, uint32_t thread, uint32_t threads) {
+  uint64_t at = s.lo + s.bytes;
+  if (at < s.begin) at = s.begin;
+  for (uint64_t i = at / sizeof(U) + thread; i < s.end / sizeof(U); i += threads)
+    reinterpret_cast<U*>(static_cast<char*>(slot) + (i * sizeof(U) - s.lo))[0] = static_cast<const U*>(base)[i];
+}
+VSD bool span_has_tail(const Span& s) { return s.lo + s.bytes < s.end; }
+// Writes the run back: whole 16-byte pieces by one thread's bulk store, the
+// ragged ends (which belong to neighbouring runs too) value by value.
+template <typename U> VSD void span_store(const Span& s, const void* slot, void* base, uint32_t lane) {
+  const uint64_t a = (s.begin + 15) & ~15ull, b = s.end & ~15ull;
+  if (lane == 0 && a < b)
+    bulk_store(static_cast<char*>(base) + a, static_cast<const char*>(slot) + (a - s.lo), (uint32_t)(b - a));
+  if (a == s.begin && b == s.end) return;
+  const uint64_t head = a < s.end ? a : s.end;
+  for (uint64_t i = s.begin / sizeof(U) + lane; i < head / sizeof(U); i += 32)
+    static_cast<U*>(base)[i] = reinterpret_cast<const U*>(static_cast<const char*>(slot) + (i * sizeof(U) - s.lo))[0];
+  const uint64_t tail = b > head ? b : head;
+  for (uint64_t i = tail / sizeof(U) + lane; i < s.end / sizeof(U); i += 32)
+    static_cast<U*>(base)[i] = reinterpret_cast<const U*>(static_cast<const char*>(slot) + (i * sizeof(U) - s.lo))[0];
+}
+
+// ---- VEC values at once -----------------------------------------------------
+template <int BYTES> struct Word;
+template <> struct Word<2> { using type = uint16_t; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<16> { using type = uint4; };
+
+VSD float2 pair_f32(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
+VSD float2 pair_f32(const __nv_bfloat16* p) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p)); }
+VSD void pair_from(__half* p, float a, float b) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b); }
+VSD void pair_from(__nv_bfloat16* p, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
+}
+
+template <int VEC, typename T> VSD void load_vec(const T* p, float* out) {
+  using W = typename Word<VEC * sizeof(T)>::type;
+  __align__(16) T t[VEC];
+  *reinterpret_cast<W*>(t) = *reinterpret_cast<const W*>(p);
+  if constexpr (sizeof(T) == 2 && VEC > 1) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      const float2 f = pair_f32(t + j);
+      out[j] = f.x;
+      out[j + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) out[j] = to_f32(t[j]);
+  }
+}
+template <int VEC, typename T> VSD void store_vec(T* p, const float* in) {
+  using W = typename Word<VEC * sizeof(T)>::type;
+  __align__(16) T t[VEC];
+  if constexpr (sizeof(T) == 2 && VEC > 1) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) pair_from(t + j, in[j], in[j + 1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) t[j] = from_f32<T>(in[j]);
+  }
+  *reinterpret_cast<W*>(p) = *reinterpret_cast<const W*>(t);
+}
+
+// The sum over groups of `lanes` (a power of two) neighbouring lanes.
+VSD float lanes_sum(float v, uint32_t lanes) {
+#pragma unroll
+  for (uint32_t o = 16; o > 0; o >>= 1)
+    if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// sum / n with inv = 1 / n, correctly rounded for finite quotients
+VSD float quotient(float sum, float n, float inv) {
+  const float q = sum * inv;
+  const float r = fmaf(fmaf(-q, n, sum), inv, q);
+  return fabsf(q) <= 3.402823466e38f ? r : q;
+}
+
+// The keep decisions of one group as bits.
+VSD uint32_t keep_bits(const Words& w, uint32_t threshold) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j) bits |= (keeps(w, j, threshold) ? 1u : 0u) << j;
+  return bits;
+}
+
+constexpr uint32_t NORM_WARPS = 4;   // warps of a CTA whose warps work on their own
+constexpr uint32_t NORM_STAGES = 4;  // ring slots at most
+constexpr uint32_t NORM_ELEMS = 16;  // values of a row that a thread holds at most
+constexpr uint32_t NORM_MAX_SMEM = 226 * 1024;
+// Threads of an SM that the CTA-per-row kernels' registers leave room for.  The
+// grids follow from this and the shape alone, never from an occupancy query, so
+// the order of the weight gradients' sums does too.
+constexpr uint32_t NORM_FWD_THREADS = 768;
+constexpr uint32_t NORM_BWD_THREADS = 512;
+
+}  // namespace vs
+
+// What the forward and the backward take; unused buffers are NULL.
+struct NormFwd {
+  vs::NormShape s;
+  const void *x, *residual;
+  vs::Weights w;
+  float eps;
+  vs::Dropout d;
+  void *y, *z;
+  float *mean, *rstd;
+};
+struct NormBwd {
+  vs::NormShape s;
+  const void *dy, *dz, *z;
+  vs::Weights w;
+  const float *mean, *rstd;
+  vs::Dropout d;
+  void *dx, *dresidual;
+  int32_t wdtype;
+  void *dweight, *dbias;
+};
+
+// The streaming kernels take contiguous rows on 16-byte aligned buffers;
+// *taken tells whether the shape is one of theirs.
+vs_status norm_stream_forward(vs_ctx* ctx, int32_t dtype, bool join, const NormFwd& a, bool* taken);
+vs_status norm_stream_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBwd& a, bool* taken);
+// dw and db from `strips` partial sums [strips][2][cols]
+vs_status norm_join_partials(vs_ctx* ctx, uint32_t cols, uint32_t strips, const float* partial, int32_t dtype,
+                             void* dweight, void* dbias);
