@@ -96,7 +96,6 @@ VSD void span_tail(const Span& s, void* slot, const void* base, uint32_t thread,
   for (uint64_t i = at / sizeof(U) + thread; i < s.end / sizeof(U); i += threads)
     reinterpret_cast<U*>(static_cast<char*>(slot) + (i * sizeof(U) - s.lo))[0] = static_cast<const U*>(base)[i];
 }
-VSD bool span_has_tail(const Span& s) { return s.lo + s.bytes < s.end; }
 // Writes the run back: whole 16-byte pieces by one thread's bulk store, the
 // ragged ends (which belong to neighbouring runs too) value by value.
 template <typename U> VSD void span_store(const Span& s, const void* slot, void* base, uint32_t lane) {
@@ -112,48 +111,92 @@ template <typename U> VSD void span_store(const Span& s, const void* slot, void*
     static_cast<U*>(base)[i] = reinterpret_cast<const U*>(static_cast<const char*>(slot) + (i * sizeof(U) - s.lo))[0];
 }
 
-// ---- VEC values at once -----------------------------------------------------
+// Two f32 operations in one instruction.
+VSD unsigned long long bits2(float2 a) { return reinterpret_cast<unsigned long long&>(a); }
+VSD float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return reinterpret_cast<float2&>(r);
+}
+VSD float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return reinterpret_cast<float2&>(r);
+}
+VSD float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return reinterpret_cast<float2&>(r);
+}
+VSD float2 both(float v) { return make_float2(v, v); }
+
+// ---- VEC values at once, as they lie in memory ------------------------------
 template <int BYTES> struct Word;
 template <> struct Word<2> { using type = uint16_t; };
 template <> struct Word<4> { using type = uint32_t; };
 template <> struct Word<8> { using type = uint2; };
 template <> struct Word<16> { using type = uint4; };
+template <int VEC, typename T> VSD void copy_vec(T* to, const T* from) {
+  using W = typename Word<VEC * sizeof(T)>::type;
+  *reinterpret_cast<W*>(to) = *reinterpret_cast<const W*>(from);
+}
 
+VSD float2 pair_f32(const float* p) { return make_float2(p[0], p[1]); }
 VSD float2 pair_f32(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
 VSD float2 pair_f32(const __nv_bfloat16* p) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p)); }
-VSD void pair_from(__half* p, float a, float b) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b); }
-VSD void pair_from(__nv_bfloat16* p, float a, float b) {
-  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
+VSD void pair_from(float* p, float2 v) {
+  p[0] = v.x;
+  p[1] = v.y;
 }
+VSD void pair_from(__half* p, float2 v) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(v); }
+VSD void pair_from(__nv_bfloat16* p, float2 v) { *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(v); }
 
-template <int VEC, typename T> VSD void load_vec(const T* p, float* out) {
-  using W = typename Word<VEC * sizeof(T)>::type;
-  __align__(16) T t[VEC];
-  *reinterpret_cast<W*>(t) = *reinterpret_cast<const W*>(p);
-  if constexpr (sizeof(T) == 2 && VEC > 1) {
+// The values of a row that one thread holds: K runs of VEC.  Rows of whole
+// 16-byte vectors are dealt out vector by vector, so that a warp's accesses are
+// contiguous; the runs' order turns with the row's place in the warp, which
+// keeps neighbouring rows of 64 bytes apart off each other's shared-memory
+// banks.  Other rows are dealt out in blocks of K runs, K odd, so that a warp's
+// narrow accesses fall into different banks and every offset is a constant.
+template <typename T, int VEC, int K> struct Part {
+  static constexpr int E = VEC * K;
+  static constexpr int PAIRS = (E + 1) / 2;
+  static constexpr bool kDirect = VEC * sizeof(T) == 16;
+  uint32_t at, lanes, sub, cols;
+
+  VSD uint32_t col(int k) const {
+    if (kDirect) return (at + (K == 1 ? 0 : lanes * ((k + sub) & (K - 1)))) * VEC;
+    return (at * K + k) * VEC;
+  }
+  VSD bool has(int k) const { return col(k) < cols; }
+  // raw values; those beyond the row are zeros
+  VSD void load(const T* row, T* t) const {
 #pragma unroll
-    for (int j = 0; j < VEC; j += 2) {
-      const float2 f = pair_f32(t + j);
-      out[j] = f.x;
-      out[j + 1] = f.y;
+    for (int k = 0; k < K; ++k) {
+      if (has(k)) {
+        copy_vec<VEC>(t + k * VEC, row + col(k));
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) t[k * VEC + j] = from_f32<T>(0.0f);
+      }
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) out[j] = to_f32(t[j]);
+    if (E % 2) t[E] = from_f32<T>(0.0f);
   }
-}
-template <int VEC, typename T> VSD void store_vec(T* p, const float* in) {
-  using W = typename Word<VEC * sizeof(T)>::type;
-  __align__(16) T t[VEC];
-  if constexpr (sizeof(T) == 2 && VEC > 1) {
+  VSD void store(T* row, const T* t) const {
 #pragma unroll
-    for (int j = 0; j < VEC; j += 2) pair_from(t + j, in[j], in[j + 1]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) t[j] = from_f32<T>(in[j]);
+    for (int k = 0; k < K; ++k)
+      if (has(k)) copy_vec<VEC>(row + col(k), t + k * VEC);
   }
-  *reinterpret_cast<W*>(p) = *reinterpret_cast<const W*>(t);
-}
+  // acc + a b, where the thread has the pair's values
+  VSD float2 fma_if(float2 a, float2 b, float2 acc, int pair) const {
+    if constexpr (VEC > 1) {
+      return has(2 * pair / VEC) ? fma2(a, b, acc) : acc;
+    } else {
+      if (!has(2 * pair)) return acc;
+      if (2 * pair + 1 >= E || !has(2 * pair + 1)) a.y = 0.0f;
+      return fma2(a, b, acc);
+    }
+  }
+};
 
 // The sum over groups of `lanes` (a power of two) neighbouring lanes.
 VSD float lanes_sum(float v, uint32_t lanes) {
@@ -178,9 +221,49 @@ VSD uint32_t keep_bits(const Words& w, uint32_t threshold) {
   return bits;
 }
 
+// Dropout of a thread's values: v holds pairs, i0 is the row's first index.
+// Runs of eight are groups of the generator; for others the group's bits have
+// been left in `bits`, whose first bit is the decision of index i0 & ~7.
+template <typename T, int VEC, int K>
+VSD void drop_part(const Part<T, VEC, K>& part, float2* v, uint64_t i0, const Dropout& d, const unsigned char* bits) {
+  const float2 scale = both(d.scale);
+#pragma unroll
+  for (int i = 0; i < part.PAIRS; ++i) v[i] = mul2(v[i], scale);
+  float* f = reinterpret_cast<float*>(v);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (!part.has(k)) continue;
+    if (VEC == 8) {
+      const Words words = philox(d, (i0 + part.col(k)) >> 3);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[k * VEC + j] = keeps(words, j, d.threshold) ? f[k * VEC + j] : 0.0f;
+    } else {
+      const uint32_t e = ((uint32_t)i0 & 7u) + part.col(k);
+      const uint32_t kept = bits[e >> 3] >> (e & 7u);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[k * VEC + j] = kept >> j & 1u ? f[k * VEC + j] : 0.0f;
+    }
+  }
+}
+// Leaves the bits of indices [i0, i0 + count) for drop_part.
+VSD void fill_bits(const Dropout& d, uint64_t i0, uint32_t count, unsigned char* bits, uint32_t id, uint32_t members) {
+  const uint64_t g0 = i0 >> 3;
+  const uint32_t groups = (((uint32_t)i0 & 7u) + count + 7) >> 3;
+  for (uint32_t g = id; g < groups; g += members) bits[g] = (unsigned char)keep_bits(philox(d, g0 + g), d.threshold);
+}
+
+// The sum over a CTA of `warps` warps, the same in every thread; `part` holds a
+// value per warp and is free for the next use after another barrier.
+VSD float cta_sum(float v, float* part, uint32_t warps) {
+  v = warp_sum(v);
+  const uint32_t lane = threadIdx.x & 31u;
+  if (lane == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_sum(lane < warps ? part[lane] : 0.0f);
+}
+
 constexpr uint32_t NORM_WARPS = 4;   // warps of a CTA whose warps work on their own
 constexpr uint32_t NORM_STAGES = 4;  // ring slots at most
-constexpr uint32_t NORM_ELEMS = 16;  // values of a row that a thread holds at most
 constexpr uint32_t NORM_MAX_SMEM = 226 * 1024;
 // Threads of an SM that the CTA-per-row kernels' registers leave room for.  The
 // grids follow from this and the shape alone, never from an occupancy query, so

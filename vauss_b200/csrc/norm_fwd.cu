@@ -2,11 +2,11 @@
 // sum before it, for contiguous rows.
 //
 // The work is one read and one write of the rows, so the kernels keep bulk
-// copies in flight all the time: each worker (a warp, or a CTA for rows over
-// 512 values) owns a ring of shared-memory slots that one thread refills with
-// cp.async.bulk, and holds its row in registers for the two sums (mean, then
-// squares about it).  A lane's columns are the same for every row, so weights
-// stay in registers too.
+// copies in flight all the time: each worker (a warp with a tile of rows, or a
+// CTA with one row of more than about 500 values) owns a ring of shared-memory
+// slots that one thread refills with cp.async.bulk, and holds its row in
+// registers for the two sums (mean, then squares about it).  A thread's columns
+// are the same for every row, so the weights stay in registers too.
 #include <atomic>
 
 #include "norm.cuh"
@@ -15,13 +15,13 @@ namespace {
 
 using namespace vs;
 
-// CTAs of the warp kernel on an SM, by the values a lane holds: the registers
-// they need fix it.
-constexpr int warp_ctas(int elems) { return elems == 16 ? 4 : 7; }
+// CTAs of the warp workers on an SM, by the values a lane holds: their
+// registers fix it.
+constexpr int warp_ctas(int elems) { return elems > 8 ? 4 : 7; }
 
 struct FwdArgs {
-  uint64_t rows, tiles;
-  uint32_t cols, tile_rows, lanes, slot, bits, stages;
+  uint64_t rows;
+  uint32_t cols, tile_rows, log_lanes, slot, bits, stages;
   const void *x, *residual;
   Weights w;
   float eps;
@@ -30,409 +30,239 @@ struct FwdArgs {
   uint32_t* err;
 };
 
-// One warp per tile of rows, `lanes` lanes per row, VEC x K values per lane.
-// Rows of whole 16-byte vectors are written from registers; others go back
-// into their slot and out by a bulk store, so that no access is narrower than
-// its run of bytes.
-template <typename T, int VEC, int K, bool kJoin>
-__global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas(VEC * K))
-    norm_fwd_warp_kernel(const FwdArgs a, const __grid_constant__ Dropout d) {
-  constexpr int E = VEC * K;
-  constexpr uint32_t NIN = kJoin ? 2 : 1;
-  constexpr bool kDirect = VEC * sizeof(T) == 16;
+// Rows of whole 16-byte vectors are written from registers; others go back into
+// their slot and out by a bulk store, so that no access is narrower than its
+// run of bytes.
+template <typename T, int VEC, int K, bool kJoin, bool kCta>
+__global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCta ? 1 : warp_ctas(VEC * K))
+    norm_fwd_kernel(const FwdArgs a, const __grid_constant__ Dropout d) {
+  using P = Part<T, VEC, K>;
+  constexpr int PAIRS = P::PAIRS;
+  constexpr bool kDirect = P::kDirect;
   constexpr bool kBits = kJoin && VEC != 8;
+  constexpr uint32_t NIN = kJoin ? 2 : 1, WORKERS = kCta ? 1 : NORM_WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t bars[NORM_WARPS][NORM_STAGES];
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  unsigned char* ring = smem + (size_t)warp * (NORM_STAGES * NIN * a.slot + a.bits);
-  unsigned char* bits = ring + NORM_STAGES * NIN * a.slot;
-  uint64_t* full = bars[warp];
-  const uint64_t total = a.rows * a.cols * sizeof(T);
-  const uint64_t step = (uint64_t)gridDim.x * NORM_WARPS;
-  const uint64_t first = (uint64_t)blockIdx.x * NORM_WARPS + warp;
+  __shared__ __align__(8) uint64_t bars[WORKERS][NORM_STAGES];
+  __shared__ float red[2][kCta ? 32 : 1];
+  __shared__ uint32_t late;
+  const uint32_t worker = kCta ? 0 : threadIdx.x >> 5;
+  const uint32_t id = kCta ? threadIdx.x : threadIdx.x & 31u, members = kCta ? blockDim.x : 32;
+  const uint32_t warps = blockDim.x >> 5;
+  const uint32_t lanes = kCta ? members : 1u << a.log_lanes;
+  const uint32_t sub = kCta ? 0 : id >> a.log_lanes, per_pass = kCta ? 1 : 32u >> a.log_lanes;
+  const P part{kCta ? id : id & (lanes - 1), lanes, sub, a.cols};
+  unsigned char* ring = smem + (size_t)worker * (a.stages * NIN * a.slot + a.bits);
+  unsigned char* bits = ring + a.stages * NIN * a.slot;
+  uint64_t* full = bars[worker];
 
-  auto tile_span = [&](uint64_t tile) {
-    const uint64_t r0 = tile * a.tile_rows;
-    const uint64_t r1 = r0 + a.tile_rows < a.rows ? r0 + a.tile_rows : a.rows;
-    return span_of(r0 * a.cols * sizeof(T), r1 * a.cols * sizeof(T), total);
+  const uint64_t first = (uint64_t)blockIdx.x * WORKERS + worker, step = (uint64_t)gridDim.x * WORKERS;
+  const uint32_t tile_bytes = a.tile_rows * a.cols * (uint32_t)sizeof(T);
+  const uint64_t total = a.rows * a.cols * sizeof(T), step_bytes = step * tile_bytes;
+  uint64_t begin = first * tile_bytes;  // of the tile at hand
+  uint64_t load_at = begin;             // of the tile to be copied next (thread 0's)
+  auto span_at = [&](uint64_t b) {
+    const uint64_t end = total - b < tile_bytes ? total : b + tile_bytes;
+    return kDirect ? Span{b, end, b, (uint32_t)(end - b), 0} : span_of(b, end, total);
   };
-  auto refill = [&](uint64_t tile, uint32_t slot) {  // lane 0
-    const Span s = tile_span(tile);
-    mbar_expect(&full[slot], s.bytes * NIN);
-    span_load(s, ring + slot * NIN * a.slot, a.x, &full[slot]);
-    if (kJoin) span_load(s, ring + (slot * NIN + 1) * a.slot, a.residual, &full[slot]);
+  auto refill = [&](uint32_t slot) {
+    if (load_at < total) {
+      const Span s = span_at(load_at);
+      unsigned char* to = ring + slot * NIN * a.slot;
+      mbar_expect(&full[slot], s.bytes * NIN);
+      span_load(s, to, a.x, &full[slot]);
+      if (kJoin) span_load(s, to + a.slot, a.residual, &full[slot]);
+    }
+    load_at += step_bytes;
   };
-  if (lane == 0) {
-    for (uint32_t k = 0; k < NORM_STAGES; ++k) mbar_init(&full[k], 1);
+  if (id == 0) {
+    if (kCta) late = 0;
+    for (uint32_t k = 0; k < a.stages; ++k) mbar_init(&full[k], 1);
     mbar_init_fence();
-    for (uint32_t k = 0; k < NORM_STAGES; ++k)
-      if (first + k * step < a.tiles) refill(first + k * step, k);
+    for (uint32_t k = 0; k < a.stages; ++k) refill(k);
   }
-  const uint32_t lanes = a.lanes, sub = lane / lanes, at = lane % lanes, per_pass = 32 / lanes;
-  float w[E], b[E];
+  float2 w[PAIRS], b[PAIRS];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const uint32_t c = (at + lanes * (e / VEC)) * VEC + e % VEC;
-    w[e] = c < a.cols && a.w.weight ? load_as(a.w.weight, a.w.dtype, c) : 1.0f;
-    b[e] = c < a.cols && a.w.bias ? load_as(a.w.bias, a.w.dtype, c) : 0.0f;
+  for (int e = 0; e < 2 * PAIRS; ++e) {
+    const uint32_t c = part.col(e / VEC) + e % VEC;
+    const bool has = e < P::E && part.has(e / VEC);
+    (&w[e / 2].x)[e % 2] = has && a.w.weight ? load_as(a.w.weight, a.w.dtype, c) : 1.0f;
+    (&b[e / 2].x)[e % 2] = has && a.w.bias ? load_as(a.w.bias, a.w.dtype, c) : 0.0f;
   }
   const float n = (float)a.cols, inv = 1.0f / n;
-  __syncwarp();
+  if (kCta) __syncthreads(); else __syncwarp();
 
   uint32_t slot = 0, parity = 0;
-  uint64_t left = 0;  // first tile whose copies have not been waited for
   bool ok = true;
-  for (uint64_t tile = first; tile < a.tiles; tile += step) {
-    ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], parity));
-    left = tile;
-    if (!ok) break;
+  uint64_t row0 = first * a.tile_rows;
+  for (; row0 < a.rows; row0 += step * a.tile_rows, begin += step_bytes) {
+    ok = mbar_wait(&full[slot], parity);
+    if (kCta) {
+      if (!ok) late = 1;
+    } else if (!(ok = __all_sync(0xffffffffu, ok))) {
+      break;
+    }
     unsigned char* in = ring + slot * NIN * a.slot;
     unsigned char* res = in + a.slot;
-    const Span s = tile_span(tile);
-    const uint64_t r0 = tile * a.tile_rows;
-    const uint32_t rows = a.rows - r0 < a.tile_rows ? (uint32_t)(a.rows - r0) : a.tile_rows;
-    if (span_has_tail(s)) {
-      span_tail<T>(s, in, a.x, lane, 32);
-      if (kJoin) span_tail<T>(s, res, a.residual, lane, 32);
-      __syncwarp();
+    const uint32_t rows = a.rows - row0 < a.tile_rows ? (uint32_t)(a.rows - row0) : a.tile_rows;
+    const uint64_t i0 = begin / sizeof(T);
+    const uint32_t shift = kDirect ? 0 : (uint32_t)begin & 15u;
+    if (!kDirect && total - begin < tile_bytes + 16u) {  // the last 16-byte piece, where it is not whole
+      const Span s = span_at(begin);
+      span_tail<T>(s, in, a.x, id, members);
+      if (kJoin) span_tail<T>(s, res, a.residual, id, members);
+      if (kCta) __syncthreads(); else __syncwarp();
     }
-    const uint64_t i0 = r0 * a.cols;
     if (kBits && d.threshold) {
-      const uint64_t g0 = i0 >> 3, g1 = (i0 + (uint64_t)rows * a.cols + 7) >> 3;
-      for (uint64_t g = g0 + lane; g < g1; g += 32) bits[g - g0] = (unsigned char)keep_bits(philox(d, g), d.threshold);
-      __syncwarp();
+      fill_bits(d, i0, rows * a.cols, bits, id, members);
+      if (kCta) __syncthreads(); else __syncwarp();
     }
     for (uint32_t p = 0; p < rows; p += per_pass) {
+      // a lane beyond the tile's rows computes its last row and writes nothing
       const bool live = p + sub < rows;
-      const uint32_t r = live ? p + sub : rows - 1;
-      T* xr = reinterpret_cast<T*>(in + s.shift) + r * a.cols;
-      T* rr = reinterpret_cast<T*>(res + s.shift) + r * a.cols;
-      float v[E];
-      float sum = 0.0f;
+      const uint32_t r = live ? p + sub : rows - 1, r_at = r * a.cols;
+      T* xr = reinterpret_cast<T*>(in + shift) + r_at;
+      T* rr = reinterpret_cast<T*>(res + shift) + r_at;
+      float2 v[PAIRS];
+      __align__(16) T t[2 * PAIRS];
+      part.load(xr, t);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const uint32_t c = (at + lanes * k) * VEC;
-        float* vk = v + k * VEC;
-        if (c < a.cols) {
-          load_vec<VEC>(xr + c, vk);
-          if (kJoin) {
-            if (d.threshold) {
-              if (VEC == 8) {
-                const Words words = philox(d, (i0 + (uint64_t)r * a.cols + c) >> 3);
+      for (int i = 0; i < PAIRS; ++i) v[i] = pair_f32(t + 2 * i);
+      if (kJoin) {
+        if (d.threshold) drop_part(part, v, i0 + r_at, d, kBits ? bits + ((((uint32_t)i0 & 7u) + r_at) >> 3) : bits);
+        part.load(rr, t);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) vk[j] = dropped(vk[j], keeps(words, j, d.threshold), d.scale);
-              } else {
-                const uint32_t e0 = ((uint32_t)i0 & 7u) + r * a.cols + c;
-                const uint32_t kept = bits[e0 >> 3] >> (e0 & 7u);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) vk[j] = dropped(vk[j], kept >> j & 1u, d.scale);
-              }
-            }
-            float rv[VEC];
-            load_vec<VEC>(rr + c, rv);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) vk[j] = to_f32(from_f32<T>(vk[j] + rv[j]));
-          }
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) sum += vk[j];
+        for (int i = 0; i < PAIRS; ++i) {
+          pair_from(t + 2 * i, add2(v[i], pair_f32(t + 2 * i)));  // z, rounded as it is stored
+          v[i] = pair_f32(t + 2 * i);
         }
       }
-      const float m = quotient(lanes_sum(sum, lanes), n, inv);
-      float sq = 0.0f;
+      float2 s = both(0.0f);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if ((at + lanes * k) * VEC < a.cols) {
+      for (int i = 0; i < PAIRS; ++i) s = add2(s, v[i]);
+      float m = s.x + s.y;
+      m = quotient(kCta ? cta_sum(m, red[0], warps) : lanes_sum(m, lanes), n, inv);
+      if (kCta) ok = !late;  // between two barriers: the same for all
+      s = both(0.0f);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float e = v[k * VEC + j] - m;
-            sq = fmaf(e, e, sq);
-          }
-        }
+      for (int i = 0; i < PAIRS; ++i) {
+        v[i] = add2(v[i], both(-m));
+        s = part.fma_if(v[i], v[i], s, i);
       }
-      const float q = rsqrtf(fmaf(lanes_sum(sq, lanes), inv, a.eps));
-      if (!kDirect) __syncwarp();  // a row beyond the tile stands for the last one, which is read before it is written
-      if (live) {
-        T* yr = kDirect ? static_cast<T*>(a.y) + i0 + (uint64_t)r * a.cols : xr;
-        T* zr = kDirect ? static_cast<T*>(a.z) + i0 + (uint64_t)r * a.cols : rr;
+      float q = s.x + s.y;
+      q = rsqrtf(fmaf(kCta ? cta_sum(q, red[1], warps) : lanes_sum(q, lanes), inv, a.eps));
+      if (!kCta && !kDirect) __syncwarp();  // the last row is read by all before it is written
+      if (live && ok) {
+        if (kJoin) part.store(kDirect ? static_cast<T*>(a.z) + i0 + r_at : rr, t);
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const uint32_t c = (at + lanes * k) * VEC;
-          if (c < a.cols) {
-            float* vk = v + k * VEC;
-            if (kJoin) store_vec<VEC>(zr + c, vk);
-            float o[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) o[j] = fmaf((vk[j] - m) * q, w[k * VEC + j], b[k * VEC + j]);
-            store_vec<VEC>(yr + c, o);
-          }
-        }
-        if (at == 0) {
-          if (a.mean) a.mean[r0 + r] = m;
-          if (a.rstd) a.rstd[r0 + r] = q;
+        for (int i = 0; i < PAIRS; ++i) pair_from(t + 2 * i, fma2(mul2(v[i], both(q)), w[i], b[i]));
+        part.store(kDirect ? static_cast<T*>(a.y) + i0 + r_at : xr, t);
+        if (part.at == 0) {
+          if (a.mean) a.mean[row0 + r] = m;
+          if (a.rstd) a.rstd[row0 + r] = q;
         }
       }
     }
+    if (kCta && !ok) break;
     if (kDirect) {
-      __syncwarp();
-      if (lane == 0 && tile + NORM_STAGES * step < a.tiles) refill(tile + NORM_STAGES * step, slot);
+      // every thread has its part of the tile in registers (the sums' barriers tell)
+      if (!kCta) __syncwarp();
+      if (id == 0) refill(slot);
     } else {
       proxy_fence();
-      __syncwarp();
-      span_store<T>(s, in, a.y, lane);
-      if (kJoin) span_store<T>(s, res, a.z, lane);
-      if (lane == 0) {
+      if (kCta) __syncthreads(); else __syncwarp();
+      if (id < 32) {
+        const Span s = span_at(begin);
+        span_store<T>(s, in, a.y, id);
+        if (kJoin) span_store<T>(s, res, a.z, id);
+      }
+      if (id == 0) {
         bulk_commit();
         // the slot before this one has been read out by now: it is filled again
         bulk_wait_read<1>();
-        if (tile != first && tile + (NORM_STAGES - 1) * step < a.tiles)
-          refill(tile + (NORM_STAGES - 1) * step, slot == 0 ? NORM_STAGES - 1 : slot - 1);
+        if (row0 >= step * a.tile_rows) refill(slot == 0 ? a.stages - 1 : slot - 1);
       }
-      __syncwarp();
-    }
-    if (++slot == NORM_STAGES) {
-      slot = 0;
-      parity ^= 1;
-    }
-  }
-  if (!ok) {  // a copy did not land in time: report, and let those in flight end
-    if (lane == 0) atomicOr(a.err, VS_DERR_WAIT);
-    for (uint32_t k = 0; k < NORM_STAGES && left + k * step < a.tiles; ++k) {
-      mbar_wait(&full[slot], parity);
-      if (++slot == NORM_STAGES) {
-        slot = 0;
-        parity ^= 1;
-      }
-    }
-  }
-  if (!kDirect && lane == 0) bulk_wait<0>();
-}
-
-// One CTA per row of more than 512 values; the row's slot is free again once
-// every thread holds its part, which the first sum's barrier tells.
-template <typename T, int VEC, int K, bool kJoin>
-__global__ void __launch_bounds__(NORM_FWD_THREADS)
-    norm_fwd_cta_kernel(const FwdArgs a, const __grid_constant__ Dropout d) {
-  constexpr int E = VEC * K;
-  constexpr uint32_t NIN = kJoin ? 2 : 1;
-  constexpr bool kBits = kJoin && VEC != 8;
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t full[NORM_STAGES];
-  __shared__ float red[2][NORM_FWD_THREADS / 32];
-  __shared__ uint32_t late;
-  unsigned char* bits = smem + a.stages * NIN * a.slot;  // two rows' keep bits
-  const uint32_t tid = threadIdx.x, threads = blockDim.x, warps = threads >> 5;
-  const uint64_t total = a.rows * a.cols * sizeof(T);
-
-  auto row_span = [&](uint64_t r) { return span_of(r * a.cols * sizeof(T), (r + 1) * a.cols * sizeof(T), total); };
-  auto refill = [&](uint64_t r, uint32_t slot) {  // thread 0
-    const Span s = row_span(r);
-    mbar_expect(&full[slot], s.bytes * NIN);
-    span_load(s, smem + slot * NIN * a.slot, a.x, &full[slot]);
-    if (kJoin) span_load(s, smem + (slot * NIN + 1) * a.slot, a.residual, &full[slot]);
-  };
-  auto fill_bits = [&](uint64_t r, uint32_t half) {
-    const uint64_t i0 = r * a.cols, g0 = i0 >> 3, g1 = (i0 + a.cols + 7) >> 3;
-    for (uint64_t g = g0 + tid; g < g1; g += threads)
-      bits[half * (a.bits / 2) + (g - g0)] = (unsigned char)keep_bits(philox(d, g), d.threshold);
-  };
-  auto cta_sum = [&](float v, float* part) {
-    v = warp_sum(v);
-    if ((tid & 31u) == 0) part[tid >> 5] = v;
-    __syncthreads();
-    float s = part[0];
-    for (uint32_t k = 1; k < warps; ++k) s += part[k];
-    return s;
-  };
-  if (tid == 0) {
-    late = 0;
-    for (uint32_t k = 0; k < a.stages; ++k) mbar_init(&full[k], 1);
-    mbar_init_fence();
-    for (uint32_t k = 0; k < a.stages; ++k)
-      if (blockIdx.x + (uint64_t)k * gridDim.x < a.rows) refill(blockIdx.x + (uint64_t)k * gridDim.x, k);
-  }
-  float w[E], b[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const uint32_t c = (tid + threads * (e / VEC)) * VEC + e % VEC;
-    w[e] = c < a.cols && a.w.weight ? load_as(a.w.weight, a.w.dtype, c) : 1.0f;
-    b[e] = c < a.cols && a.w.bias ? load_as(a.w.bias, a.w.dtype, c) : 0.0f;
-  }
-  if (kBits && d.threshold) fill_bits(blockIdx.x, 0);
-  const float n = (float)a.cols, inv = 1.0f / n;
-  __syncthreads();
-
-  uint32_t slot = 0, parity = 0, half = 0;
-  for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    if (!mbar_wait(&full[slot], parity)) late = 1;
-    unsigned char* in = smem + slot * NIN * a.slot;
-    unsigned char* res = in + a.slot;
-    const Span s = row_span(r);
-    if (span_has_tail(s)) {
-      span_tail<T>(s, in, a.x, tid, threads);
-      if (kJoin) span_tail<T>(s, res, a.residual, tid, threads);
-      __syncthreads();
-    }
-    const uint64_t i0 = r * a.cols;
-    const T* xr = reinterpret_cast<const T*>(in + s.shift);
-    const T* rr = reinterpret_cast<const T*>(res + s.shift);
-    float v[E];
-    float sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const uint32_t c = (tid + threads * k) * VEC;
-      float* vk = v + k * VEC;
-      if (c < a.cols) {
-        load_vec<VEC>(xr + c, vk);
-        if (kJoin) {
-          if (d.threshold) {
-            if (VEC == 8) {
-              const Words words = philox(d, (i0 + c) >> 3);
-#pragma unroll
-              for (int j = 0; j < VEC; ++j) vk[j] = dropped(vk[j], keeps(words, j, d.threshold), d.scale);
-            } else {
-              const uint32_t e0 = ((uint32_t)i0 & 7u) + c;
-              const uint32_t kept = bits[half * (a.bits / 2) + (e0 >> 3)] >> (e0 & 7u);
-#pragma unroll
-              for (int j = 0; j < VEC; ++j) vk[j] = dropped(vk[j], kept >> j & 1u, d.scale);
-            }
-          }
-          float rv[VEC];
-          load_vec<VEC>(rr + c, rv);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) vk[j] = to_f32(from_f32<T>(vk[j] + rv[j]));
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sum += vk[j];
-      }
-    }
-    const float m = quotient(cta_sum(sum, red[0]), n, inv);
-    if (late) break;  // uniform: set before the barrier, never cleared
-    if (tid == 0 && r + (uint64_t)a.stages * gridDim.x < a.rows) refill(r + (uint64_t)a.stages * gridDim.x, slot);
-    half ^= 1;
-    if (kBits && d.threshold && r + gridDim.x < a.rows) fill_bits(r + gridDim.x, half);
-    float sq = 0.0f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if ((tid + threads * k) * VEC < a.cols) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float e = v[k * VEC + j] - m;
-          sq = fmaf(e, e, sq);
-        }
-      }
-    }
-    const float q = rsqrtf(fmaf(cta_sum(sq, red[1]), inv, a.eps));
-    T* yr = static_cast<T*>(a.y) + i0;
-    T* zr = static_cast<T*>(a.z) + i0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const uint32_t c = (tid + threads * k) * VEC;
-      if (c < a.cols) {
-        float* vk = v + k * VEC;
-        if (kJoin) store_vec<VEC>(zr + c, vk);
-        float o[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = fmaf((vk[j] - m) * q, w[k * VEC + j], b[k * VEC + j]);
-        store_vec<VEC>(yr + c, o);
-      }
-    }
-    if (tid == 0) {
-      if (a.mean) a.mean[r] = m;
-      if (a.rstd) a.rstd[r] = q;
+      if (!kCta) __syncwarp();
     }
     if (++slot == a.stages) {
       slot = 0;
       parity ^= 1;
     }
   }
-  if (late && tid == 0) {  // as in the warp kernel
+  if (!ok && id == 0) {  // a copy did not land in time: report, and let those in flight end
     atomicOr(a.err, VS_DERR_WAIT);
-    for (uint32_t k = 0; k < a.stages; ++k) mbar_wait(&full[(slot + k) % a.stages], parity ^ (slot + k >= a.stages));
+    for (uint32_t k = 0; k < a.stages && row0 < a.rows; ++k, row0 += step * a.tile_rows) {
+      mbar_wait(&full[slot], parity);
+      if (++slot == a.stages) {
+        slot = 0;
+        parity ^= 1;
+      }
+    }
   }
+  if (!kDirect && id == 0) bulk_wait<0>();
 }
 
-// Launches `kernel` with `per_sm` CTAs on each SM, at most `most`.
-template <typename Kernel>
-vs_status launch_full(vs_ctx* ctx, Kernel kernel, std::atomic<uint64_t>& ready, uint32_t threads, uint32_t per_sm,
-                      size_t smem, uint64_t most, const FwdArgs& a, const Dropout& d) {
+// One warp's lanes hold up to 32 * VEC * K values of a row; longer rows take a
+// CTA each, if its threads' registers can hold one.
+template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kernel(vs_ctx* ctx, const NormFwd& f) {
+  static std::atomic<uint64_t> ready{0};
+  constexpr uint32_t NIN = kJoin ? 2 : 1, WORKERS = kCta ? 1 : NORM_WARPS;
+  auto kernel = norm_fwd_kernel<T, VEC, K, kJoin, kCta>;
   const uint64_t bit = 1ull << (ctx->device & 63);
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
     VS_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)NORM_MAX_SMEM));
     ready.fetch_or(bit);
   }
+  FwdArgs a{};
+  a.rows = f.s.rows;
+  a.cols = f.s.cols;
+  const uint32_t chunks = (a.cols + VEC - 1) / VEC, row_bytes = a.cols * (uint32_t)sizeof(T);
+  uint32_t threads = NORM_WARPS * 32, per_sm = warp_ctas(VEC * K);
+  a.tile_rows = 1;
+  if (kCta) {
+    threads = ((chunks + K - 1) / K + 31) & ~31u;
+    per_sm = NORM_FWD_THREADS / threads;
+  } else {
+    while ((1u << a.log_lanes) * K < chunks) ++a.log_lanes;
+    // about 2 KB of copies per slot, in whole passes; fewer where that would
+    // leave warps without rows
+    const uint32_t per_pass = 32u >> a.log_lanes;
+    uint32_t passes = 2048 / NIN / (row_bytes * per_pass);
+    const uint64_t share = (uint64_t)B200_SMS * per_sm * WORKERS * per_pass;
+    const uint64_t even = (a.rows + share - 1) / share;
+    if (passes > even) passes = (uint32_t)even;
+    a.tile_rows = (passes < 1 ? 1 : passes) * per_pass;
+  }
+  a.slot = (a.tile_rows * row_bytes + 30u) & ~15u;
+  a.bits = kJoin && VEC != 8 ? (a.tile_rows * a.cols / 8 + 2 + 15) & ~15u : 0;
+  a.stages = NORM_STAGES;
+  while (a.stages > 2 && WORKERS * (a.stages * NIN * a.slot + a.bits) * per_sm > 216 * 1024) --a.stages;
+  a.x = f.x; a.residual = f.residual; a.w = f.w; a.eps = f.eps; a.y = f.y; a.z = f.z; a.mean = f.mean; a.rstd = f.rstd;
+  a.err = ctx->d_err;
+  const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + WORKERS - 1) / WORKERS;
   const uint64_t grid = (uint64_t)per_sm * B200_SMS;
-  kernel<<<(uint32_t)(grid < most ? grid : most), threads, smem, ctx->stream>>>(a, d);
+  const size_t smem = (size_t)WORKERS * (a.stages * NIN * a.slot + a.bits);
+  kernel<<<(uint32_t)(grid < most ? grid : most), threads, smem, ctx->stream>>>(a, f.d);
   ++ctx->launches;
   return vs_cuda(ctx, cudaGetLastError(), "norm launch");
 }
 
-template <typename T, int VEC, int K, bool kJoin>
-vs_status run_warp(vs_ctx* ctx, const NormFwd& f) {
-  static std::atomic<uint64_t> ready{0};
-  constexpr uint32_t NIN = kJoin ? 2 : 1;
-  FwdArgs a{};
-  a.rows = f.s.rows;
-  a.cols = f.s.cols;
-  const uint32_t chunks = (a.cols + VEC - 1) / VEC;
-  a.lanes = 1;
-  while (a.lanes * K < chunks) a.lanes *= 2;
-  const uint32_t per_pass = 32 / a.lanes, row_bytes = a.cols * sizeof(T);
-  // about 2 KB of copies per slot, in whole passes; fewer where that would
-  // leave warps without rows
-  uint32_t passes = 2048 / NIN / (row_bytes * per_pass);
-  const uint64_t share = (uint64_t)B200_SMS * warp_ctas(VEC * K) * NORM_WARPS * per_pass;
-  const uint64_t even = (a.rows + share - 1) / share;
-  if (passes > even) passes = (uint32_t)even;
-  if (passes < 1) passes = 1;
-  a.tile_rows = passes * per_pass;
-  a.tiles = (a.rows + a.tile_rows - 1) / a.tile_rows;
-  a.slot = (a.tile_rows * row_bytes + 30u) & ~15u;
-  a.bits = kJoin && VEC != 8 ? (a.tile_rows * a.cols / 8 + 2 + 15) & ~15u : 0;
-  a.x = f.x; a.residual = f.residual; a.w = f.w; a.eps = f.eps; a.y = f.y; a.z = f.z; a.mean = f.mean; a.rstd = f.rstd;
-  a.err = ctx->d_err;
-  const size_t smem = (size_t)NORM_WARPS * (NORM_STAGES * NIN * a.slot + a.bits);
-  return launch_full(ctx, norm_fwd_warp_kernel<T, VEC, K, kJoin>, ready, NORM_WARPS * 32, warp_ctas(VEC * K), smem,
-                     (a.tiles + NORM_WARPS - 1) / NORM_WARPS, a, f.d);
-}
-
-template <typename T, int VEC, int K, bool kJoin>
-vs_status run_cta(vs_ctx* ctx, const NormFwd& f, bool* taken) {
-  static std::atomic<uint64_t> ready{0};
-  constexpr uint32_t NIN = kJoin ? 2 : 1;
-  FwdArgs a{};
-  a.rows = f.s.rows;
-  a.cols = f.s.cols;
-  const uint32_t chunks = (a.cols + VEC - 1) / VEC;
-  const uint32_t threads = ((chunks + K - 1) / K + 31) & ~31u;
-  if (threads > NORM_FWD_THREADS) return VS_OK;
-  a.slot = (a.cols * (uint32_t)sizeof(T) + 30u) & ~15u;
-  a.bits = kJoin && VEC != 8 ? 2 * ((a.cols / 8 + 2 + 15) & ~15u) : 0;
-  a.stages = NORM_STAGES;
-  while (a.stages > 2 && a.stages * NIN * a.slot * (NORM_FWD_THREADS / threads) > 200 * 1024) --a.stages;
-  a.x = f.x; a.residual = f.residual; a.w = f.w; a.eps = f.eps; a.y = f.y; a.z = f.z; a.mean = f.mean; a.rstd = f.rstd;
-  a.err = ctx->d_err;
+// KS values per lane where they are enough for the row, KL otherwise.
+template <typename T, int VEC, int KS, int KL, bool kJoin>
+vs_status run_vec(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   *taken = true;
-  return launch_full(ctx, norm_fwd_cta_kernel<T, VEC, K, kJoin>, ready, threads,
-                     NORM_FWD_THREADS / threads,
-                     (size_t)a.stages * NIN * a.slot + a.bits, a.rows, a, f.d);
-}
-
-// Few values per lane where a warp's lanes still cover the row (fewer
-// registers, more rows per pass), NORM_ELEMS otherwise.
-template <typename T, int VEC, int KS, bool kJoin> vs_status run_vec(vs_ctx* ctx, const NormFwd& f, bool* taken) {
-  constexpr int KL = NORM_ELEMS / VEC;
-  *taken = true;
-  if (f.s.cols <= 32 * VEC * KS) return run_warp<T, VEC, KS, kJoin>(ctx, f);
-  if (f.s.cols <= 32 * VEC * KL) return run_warp<T, VEC, KL, kJoin>(ctx, f);
+  if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin, false>(ctx, f);
+  if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin, false>(ctx, f);
+  if (f.s.cols <= NORM_FWD_THREADS * VEC * KL) return run_kernel<T, VEC, KL, kJoin, true>(ctx, f);
   *taken = false;
-  return run_cta<T, VEC, KL, kJoin>(ctx, f, taken);
+  return VS_OK;
 }
 
 template <typename T, bool kJoin> vs_status run(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   constexpr int V = 16 / sizeof(T);
-  if (f.s.cols % V == 0) return run_vec<T, V, 1, kJoin>(ctx, f, taken);
-  if (sizeof(T) == 2 && f.s.cols % 2 == 0) return run_vec<T, 2, 2, kJoin>(ctx, f, taken);
-  return run_vec<T, 1, 4, kJoin>(ctx, f, taken);
+  if (f.s.cols % V == 0) return run_vec<T, V, 1, 16 / V, kJoin>(ctx, f, taken);
+  if constexpr (sizeof(T) == 2)
+    if (f.s.cols % 2 == 0) return run_vec<T, 2, 3, 7, kJoin>(ctx, f, taken);
+  return run_vec<T, 1, 5, 15, kJoin>(ctx, f, taken);
 }
 
 }  // namespace
