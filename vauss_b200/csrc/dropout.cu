@@ -15,7 +15,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(uint64_t count, const T* x
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
       const uint64_t i = g * 8 + j;
-      if (i < count) y[i] = from_f32<T>(dropped(to_f32(x[i]), keeps(w, j, d.threshold), d.scale));
+      if (i < count) y[i] = from_f32<T>(dropped(to_f32(x[i]), (d.threshold == 0 || keeps(w, j, d.limit)), d.scale));
     }
   }
 }
@@ -27,6 +27,7 @@ vs_status vs_make_dropout(vs_ctx* ctx, const char* what, double p, uint64_t seed
   uint32_t t = (uint32_t)(p * 65536.0 + 0.5);
   if (p < 1.0 && t > 65535u) t = 65535u;  // only p = 1 drops everything
   out->threshold = t;
+  out->limit = (uint32_t)(((uint64_t)t << 16) - 1);
   out->scale = t < 65536u ? (float)(65536.0 / (65536.0 - t)) : 0.0f;
   out->offset[0] = (uint32_t)offset;
   out->offset[1] = (uint32_t)(offset >> 32);

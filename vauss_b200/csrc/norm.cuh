@@ -130,71 +130,165 @@ VSD float2 fma2(float2 a, float2 b, float2 c) {
 }
 VSD float2 both(float v) { return make_float2(v, v); }
 
-// ---- VEC values at once, as they lie in memory ------------------------------
-template <int BYTES> struct Word;
-template <> struct Word<2> { using type = uint16_t; };
-template <> struct Word<4> { using type = uint32_t; };
-template <> struct Word<8> { using type = uint2; };
-template <> struct Word<16> { using type = uint4; };
-template <int VEC, typename T> VSD void copy_vec(T* to, const T* from) {
-  using W = typename Word<VEC * sizeof(T)>::type;
-  *reinterpret_cast<W*>(to) = *reinterpret_cast<const W*>(from);
-}
+// ---- pairs of values as they lie in memory ----------------------------------
+// Two neighbouring values: one word for 16-bit types, or two where every value
+// is read on its own (VEC = 1).
+template <typename T, int VEC> struct Raw { using type = uint32_t; };
+template <int VEC> struct Raw<float, VEC> { using type = float2; };
+template <> struct Raw<__half, 1> { using type = uint2; };
+template <> struct Raw<__nv_bfloat16, 1> { using type = uint2; };
 
-VSD float2 pair_f32(const float* p) { return make_float2(p[0], p[1]); }
-VSD float2 pair_f32(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
-VSD float2 pair_f32(const __nv_bfloat16* p) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p)); }
-VSD void pair_from(float* p, float2 v) {
-  p[0] = v.x;
-  p[1] = v.y;
+VSD float2 unpack(const __half*, uint32_t u) { return __half22float2(reinterpret_cast<const __half2&>(u)); }
+VSD float2 unpack(const __half*, uint2 u) {
+  return make_float2(__half2float(__ushort_as_half((unsigned short)u.x)),
+                     __half2float(__ushort_as_half((unsigned short)u.y)));
 }
-VSD void pair_from(__half* p, float2 v) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(v); }
-VSD void pair_from(__nv_bfloat16* p, float2 v) { *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(v); }
+VSD float2 unpack(const __nv_bfloat16*, uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+VSD float2 unpack(const __nv_bfloat16*, uint2 u) {
+  return make_float2(__uint_as_float(u.x << 16), __uint_as_float(u.y << 16));
+}
+VSD float2 unpack(const float*, float2 u) { return u; }
+VSD void pack(const float*, float2 v, float2& u) { u = v; }
+VSD void pack(const __half*, float2 v, uint32_t& u) {
+  const __half2 h = __float22half2_rn(v);
+  u = reinterpret_cast<const uint32_t&>(h);
+}
+VSD void pack(const __nv_bfloat16*, float2 v, uint32_t& u) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(v);
+  u = reinterpret_cast<const uint32_t&>(h);
+}
+template <typename T> VSD void pack(const T* t, float2 v, uint2& u) {
+  uint32_t both_values;
+  pack(t, v, both_values);
+  u = make_uint2(both_values & 0xffffu, both_values >> 16);
+}
+VSD float keep_if(float v, uint32_t mask) { return __uint_as_float(__float_as_uint(v) & mask); }
 
 // The values of a row that one thread holds: K runs of VEC.  Rows of whole
 // 16-byte vectors are dealt out vector by vector, so that a warp's accesses are
 // contiguous; the runs' order turns with the row's place in the warp, which
 // keeps neighbouring rows of 64 bytes apart off each other's shared-memory
-// banks.  Other rows are dealt out in blocks of K runs, K odd, so that a warp's
-// narrow accesses fall into different banks and every offset is a constant.
+// banks; a run beyond the row reads the row's first one.  Other rows are dealt
+// out in blocks of K runs, K odd, so that a warp's narrow accesses fall into
+// different banks and every offset is a constant; there a run beyond the row
+// reads what lies behind it (the next row, or the slot's padding).  Where a row
+// does not fill its threads (`full` is false, the same for all) such values are
+// cleared before they are used.
+constexpr uint32_t NORM_PADDING = 128;  // bytes behind the last slot that such reads may reach
 template <typename T, int VEC, int K> struct Part {
   static constexpr int E = VEC * K;
   static constexpr int PAIRS = (E + 1) / 2;
   static constexpr bool kDirect = VEC * sizeof(T) == 16;
-  uint32_t at, lanes, sub, cols;
+  using R = typename Raw<T, VEC>::type;
+  uint32_t at, lanes, sub;
+  bool full;
+  uint32_t off[kDirect ? K : 1];  // where the runs are read
+  uint32_t mask[K];               // all ones for the runs that are the row's
 
+  VSD Part(uint32_t at_, uint32_t lanes_, uint32_t sub_, uint32_t cols) : at(at_), lanes(lanes_), sub(sub_) {
+    full = cols == lanes * E;
+#pragma unroll
+    for (int k = 0; k < K; ++k) mask[k] = col(k) < cols ? 0xffffffffu : 0;
+    if constexpr (kDirect) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) off[k] = mask[k] ? col(k) : 0;
+    } else {
+      // a thread wholly beyond the row reads what the row's last thread reads
+      const uint32_t last = (cols - 1) / E;
+      off[0] = (at < last ? at : last) * E;
+    }
+  }
   VSD uint32_t col(int k) const {
     if (kDirect) return (at + (K == 1 ? 0 : lanes * ((k + sub) & (K - 1)))) * VEC;
     return (at * K + k) * VEC;
   }
-  VSD bool has(int k) const { return col(k) < cols; }
-  // raw values; those beyond the row are zeros
-  VSD void load(const T* row, T* t) const {
+  VSD bool has(int k) const { return mask[k] != 0; }
+  VSD void load(const T* row, R* t) const {
+    if constexpr (kDirect) {
+      constexpr int W = 16 / sizeof(R);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (has(k)) {
-        copy_vec<VEC>(t + k * VEC, row + col(k));
-      } else {
+      for (int k = 0; k < K; ++k) {
+        const uint4 q = *reinterpret_cast<const uint4*>(row + off[k]);
+        if constexpr (W == 4) {
+          t[k * W] = q.x; t[k * W + 1] = q.y; t[k * W + 2] = q.z; t[k * W + 3] = q.w;
+        } else {
+          t[k * W] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
+          t[k * W + 1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
+        }
+      }
+    } else if constexpr (VEC == 2 && sizeof(T) == 2) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) t[k * VEC + j] = from_f32<T>(0.0f);
+      for (int k = 0; k < K; ++k) t[k] = reinterpret_cast<const uint32_t*>(row + off[0])[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        if constexpr (sizeof(T) == 2) (&t[k / 2].x)[k % 2] = reinterpret_cast<const uint16_t*>(row + off[0])[k];
+        else (&t[k / 2].x)[k % 2] = reinterpret_cast<const float*>(row + off[0])[k];
+      }
+      if constexpr (E % 2 == 1) t[E / 2].y = 0;
+    }
+  }
+  VSD void store(T* row, const R* t) const {
+    if constexpr (kDirect) {
+      constexpr int W = 16 / sizeof(R);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (!mask[k]) continue;
+        uint4 q;
+        if constexpr (W == 4) q = make_uint4(t[k * W], t[k * W + 1], t[k * W + 2], t[k * W + 3]);
+        else q = make_uint4(__float_as_uint(t[k * W].x), __float_as_uint(t[k * W].y), __float_as_uint(t[k * W + 1].x),
+                            __float_as_uint(t[k * W + 1].y));
+        *reinterpret_cast<uint4*>(row + off[k]) = q;
+      }
+    } else if constexpr (VEC == 2 && sizeof(T) == 2) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (mask[k]) reinterpret_cast<uint32_t*>(row + off[0])[k] = t[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        if (!mask[k]) continue;
+        if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t*>(row + off[0])[k] = (uint16_t)(&t[k / 2].x)[k % 2];
+        else reinterpret_cast<float*>(row + off[0])[k] = (&t[k / 2].x)[k % 2];
       }
     }
-    if (E % 2) t[E] = from_f32<T>(0.0f);
   }
-  VSD void store(T* row, const T* t) const {
+  // Zero for the values that are not the row's.
+  VSD void clear(R* t) const {
+    if (full) return;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (has(k)) copy_vec<VEC>(row + col(k), t + k * VEC);
-  }
-  // acc + a b, where the thread has the pair's values
-  VSD float2 fma_if(float2 a, float2 b, float2 acc, int pair) const {
-    if constexpr (VEC > 1) {
-      return has(2 * pair / VEC) ? fma2(a, b, acc) : acc;
-    } else {
-      if (!has(2 * pair)) return acc;
-      if (2 * pair + 1 >= E || !has(2 * pair + 1)) a.y = 0.0f;
-      return fma2(a, b, acc);
+    for (int i = 0; i < PAIRS; ++i) {
+      const uint32_t mx = mask[2 * i / VEC], my = 2 * i + 1 < E ? mask[(2 * i + 1 < E ? 2 * i + 1 : 0) / VEC] : 0;
+      if constexpr (sizeof(T) == 4) {
+        t[i].x = keep_if(t[i].x, mx);
+        t[i].y = keep_if(t[i].y, my);
+      } else if constexpr (VEC == 1) {
+        t[i].x &= mx;
+        t[i].y &= my;
+      } else {
+        t[i] &= mx;
+      }
     }
+  }
+  VSD float2 value(const R* t, int pair) const { return unpack(static_cast<const T*>(nullptr), t[pair]); }
+  VSD void set(R* t, int pair, float2 v) const { pack(static_cast<const T*>(nullptr), v, t[pair]); }
+  // The sum of the squares of the row's values among v.
+  VSD float squares(const float2* v) const {
+    float2 s = both(0.0f);
+    if (full) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) s = fma2(v[i], v[i], s);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        const uint32_t my = 2 * i + 1 < E ? mask[(2 * i + 1 < E ? 2 * i + 1 : 0) / VEC] : 0;
+        const float2 u = make_float2(keep_if(v[i].x, mask[2 * i / VEC]), keep_if(v[i].y, my));
+        s = fma2(u, u, s);
+      }
+    }
+    return s.x + s.y;
   }
 };
 
@@ -214,10 +308,10 @@ VSD float quotient(float sum, float n, float inv) {
 }
 
 // The keep decisions of one group as bits.
-VSD uint32_t keep_bits(const Words& w, uint32_t threshold) {
+VSD uint32_t keep_bits(const Words& w, uint32_t limit) {
   uint32_t bits = 0;
 #pragma unroll
-  for (uint32_t j = 0; j < 8; ++j) bits |= (keeps(w, j, threshold) ? 1u : 0u) << j;
+  for (uint32_t j = 0; j < 8; ++j) bits |= (keeps(w, j, limit) ? 1u : 0u) << j;
   return bits;
 }
 
@@ -232,13 +326,12 @@ VSD void drop_part(const Part<T, VEC, K>& part, float2* v, uint64_t i0, const Dr
   float* f = reinterpret_cast<float*>(v);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    if (!part.has(k)) continue;
     if (VEC == 8) {
-      const Words words = philox(d, (i0 + part.col(k)) >> 3);
+      const Words words = philox(d, (i0 + part.off[part.kDirect ? k : 0]) >> 3);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f[k * VEC + j] = keeps(words, j, d.threshold) ? f[k * VEC + j] : 0.0f;
+      for (int j = 0; j < VEC; ++j) f[k * VEC + j] = keeps(words, j, d.limit) ? f[k * VEC + j] : 0.0f;
     } else {
-      const uint32_t e = ((uint32_t)i0 & 7u) + part.col(k);
+      const uint32_t e = ((uint32_t)i0 & 7u) + (part.kDirect ? part.off[part.kDirect ? k : 0] : part.off[0] + k * VEC);
       const uint32_t kept = bits[e >> 3] >> (e & 7u);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) f[k * VEC + j] = kept >> j & 1u ? f[k * VEC + j] : 0.0f;
@@ -249,17 +342,30 @@ VSD void drop_part(const Part<T, VEC, K>& part, float2* v, uint64_t i0, const Dr
 VSD void fill_bits(const Dropout& d, uint64_t i0, uint32_t count, unsigned char* bits, uint32_t id, uint32_t members) {
   const uint64_t g0 = i0 >> 3;
   const uint32_t groups = (((uint32_t)i0 & 7u) + count + 7) >> 3;
-  for (uint32_t g = id; g < groups; g += members) bits[g] = (unsigned char)keep_bits(philox(d, g0 + g), d.threshold);
+  for (uint32_t g = id; g < groups; g += members) bits[g] = (unsigned char)keep_bits(philox(d, g0 + g), d.limit);
 }
 
-// The sum over a CTA of `warps` warps, the same in every thread; `part` holds a
-// value per warp and is free for the next use after another barrier.
+// The sum over a CTA, the same in every thread; `part` holds a value per warp,
+// with zeros up to a multiple of four, and is free for the next use after
+// another barrier.
+constexpr uint32_t NORM_MAX_WARPS = 32;
+VSD float parts_sum(const float* part, uint32_t warps) {
+  const float4* p = reinterpret_cast<const float4*>(part);
+  float4 s = p[0];
+  for (uint32_t k = 1; k < (warps + 3) / 4; ++k) {
+    const float4 q = p[k];
+    s.x += q.x;
+    s.y += q.y;
+    s.z += q.z;
+    s.w += q.w;
+  }
+  return (s.x + s.y) + (s.z + s.w);
+}
 VSD float cta_sum(float v, float* part, uint32_t warps) {
   v = warp_sum(v);
-  const uint32_t lane = threadIdx.x & 31u;
-  if (lane == 0) part[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31u) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
-  return warp_sum(lane < warps ? part[lane] : 0.0f);
+  return parts_sum(part, warps);
 }
 
 constexpr uint32_t NORM_WARPS = 4;   // warps of a CTA whose warps work on their own

@@ -33,20 +33,21 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta>
 __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCta ? 1 : warp_ctas(VEC * K))
     norm_bwd_kernel(const BwdArgs a, const __grid_constant__ Dropout d) {
   using P = Part<T, VEC, K>;
+  using R = typename P::R;
   constexpr int PAIRS = P::PAIRS;
   constexpr bool kDirect = P::kDirect;
   constexpr bool kBits = kJoin && VEC != 8;
   constexpr uint32_t WORKERS = kCta ? 1 : NORM_WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[WORKERS][NORM_STAGES];
-  __shared__ float red[2][2][kCta ? 32 : 1];
+  __shared__ __align__(16) float red[2][2][kCta ? NORM_MAX_WARPS : 4];
   __shared__ uint32_t late[2];
   const uint32_t worker = kCta ? 0 : threadIdx.x >> 5;
   const uint32_t id = kCta ? threadIdx.x : threadIdx.x & 31u, members = kCta ? blockDim.x : 32;
   const uint32_t warps = blockDim.x >> 5;
   const uint32_t lanes = kCta ? members : 1u << a.log_lanes;
   const uint32_t sub = kCta ? 0 : id >> a.log_lanes, per_pass = kCta ? 1 : 32u >> a.log_lanes;
-  const P part{kCta ? id : id & (lanes - 1), lanes, sub, a.cols};
+  const P part(kCta ? id : id & (lanes - 1), lanes, sub, a.cols);
   const uint32_t stage = a.inputs * a.slot + 2 * a.stat_slot;  // dy, z, (dz), mean, rstd
   unsigned char* ring = smem + (size_t)worker * (a.stages * stage + a.bits);
   unsigned char* bits = ring + a.stages * stage;  // two rows' for a CTA
@@ -95,6 +96,8 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
     dw[e / 2] = db[e / 2] = both(0.0f);
   }
   const float n = (float)a.cols, inv = 1.0f / n;
+  if (kCta)
+    for (uint32_t k = id; k < 4 * NORM_MAX_WARPS; k += members) (&red[0][0][0])[k] = 0.0f;
   if (kCta) __syncthreads(); else __syncwarp();
 
   uint32_t slot = 0, parity = 0, half = 0;
@@ -141,22 +144,25 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
       const T* dr = reinterpret_cast<const T*>(rbuf + shift) + r_at;
       const float m = ms[r], q = qs[r];
       float2 g[PAIRS], h[PAIRS];
-      __align__(16) T t[2 * PAIRS];
-      __align__(16) T res[2 * PAIRS];
+      R t[PAIRS], res[PAIRS];
       part.load(gr, t);
+      part.clear(t);
+      if (p + per_pass > rows && !live) {  // the first test is the same for all
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) g[i] = pair_f32(t + 2 * i);
+        for (int i = 0; i < PAIRS; ++i) t[i] = R{};
+      }
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) g[i] = part.value(t, i);
       part.load(zr, t);
+      if (!kDirect) part.clear(t);
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) h[i] = mul2(add2(pair_f32(t + 2 * i), both(-m)), both(q));
+      for (int i = 0; i < PAIRS; ++i) h[i] = mul2(add2(part.value(t, i), both(-m)), both(q));
       if (kJoin && a.inputs == 3) part.load(dr, res);
       float2 s1 = both(0.0f), s2 = both(0.0f);
-      if (live) {  // g is zero where the thread has no value
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
-          dw[i] = fma2(g[i], h[i], dw[i]);
-          db[i] = add2(db[i], g[i]);
-        }
+      for (int i = 0; i < PAIRS; ++i) {  // g is zero for values that are not the row's
+        dw[i] = fma2(g[i], h[i], dw[i]);
+        db[i] = add2(db[i], g[i]);
       }
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
@@ -176,8 +182,8 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
         // barrier per row is enough
         __syncthreads();
         ok = !late[half];
-        m1 = warp_sum((id & 31u) < warps ? red[half][0][id & 31u] : 0.0f);
-        m2 = warp_sum((id & 31u) < warps ? red[half][1][id & 31u] : 0.0f);
+        m1 = parts_sum(red[half][0], warps);
+        m2 = parts_sum(red[half][1], warps);
       } else {
         m1 = lanes_sum(m1, lanes);
         m2 = lanes_sum(m2, lanes);
@@ -191,15 +197,15 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
         if (kJoin) {
           if (a.inputs == 3) {
 #pragma unroll
-            for (int i = 0; i < PAIRS; ++i) g[i] = add2(g[i], pair_f32(res + 2 * i));
+            for (int i = 0; i < PAIRS; ++i) g[i] = add2(g[i], part.value(res, i));
           }
 #pragma unroll
-          for (int i = 0; i < PAIRS; ++i) pair_from(t + 2 * i, g[i]);
+          for (int i = 0; i < PAIRS; ++i) part.set(t, i, g[i]);
           part.store(kDirect ? static_cast<T*>(a.dresidual) + i0 + r_at : zr, t);
           if (d.threshold) drop_part(part, g, i0 + r_at, d, kBits ? kept + ((((uint32_t)i0 & 7u) + r_at) >> 3) : kept);
         }
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) pair_from(t + 2 * i, g[i]);
+        for (int i = 0; i < PAIRS; ++i) part.set(t, i, g[i]);
         part.store(kDirect ? static_cast<T*>(a.dx) + i0 + r_at : gr, t);
       }
     }
@@ -247,7 +253,7 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
 #pragma unroll
     for (int e = 0; e < P::E; ++e) {
       const uint32_t c = part.col(e / VEC) + e % VEC;
-      if (c < a.cols) {
+      if (part.has(e / VEC)) {
         out[c] = (&dw[e / 2].x)[e % 2];
         out[a.cols + c] = (&db[e / 2].x)[e % 2];
       }
@@ -324,7 +330,7 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + WORKERS - 1) / WORKERS;
   const uint64_t room = (uint64_t)per_sm * B200_SMS;
   const uint32_t grid = (uint32_t)(room < most ? room : most);
-  size_t smem = (size_t)WORKERS * (a.stages * stage + a.bits);
+  size_t smem = (size_t)WORKERS * (a.stages * stage + a.bits) + NORM_PADDING;
   const size_t sums = kCta ? 0 : (size_t)WORKERS * 2 * a.cols * 4;
   if (smem < sums) smem = sums;
   const bool want = f.dweight || f.dbias;

@@ -37,20 +37,21 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta>
 __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCta ? 1 : warp_ctas(VEC * K))
     norm_fwd_kernel(const FwdArgs a, const __grid_constant__ Dropout d) {
   using P = Part<T, VEC, K>;
+  using R = typename P::R;
   constexpr int PAIRS = P::PAIRS;
   constexpr bool kDirect = P::kDirect;
   constexpr bool kBits = kJoin && VEC != 8;
   constexpr uint32_t NIN = kJoin ? 2 : 1, WORKERS = kCta ? 1 : NORM_WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[WORKERS][NORM_STAGES];
-  __shared__ float red[2][kCta ? 32 : 1];
+  __shared__ __align__(16) float red[2][kCta ? NORM_MAX_WARPS : 4];
   __shared__ uint32_t late;
   const uint32_t worker = kCta ? 0 : threadIdx.x >> 5;
   const uint32_t id = kCta ? threadIdx.x : threadIdx.x & 31u, members = kCta ? blockDim.x : 32;
   const uint32_t warps = blockDim.x >> 5;
   const uint32_t lanes = kCta ? members : 1u << a.log_lanes;
   const uint32_t sub = kCta ? 0 : id >> a.log_lanes, per_pass = kCta ? 1 : 32u >> a.log_lanes;
-  const P part{kCta ? id : id & (lanes - 1), lanes, sub, a.cols};
+  const P part(kCta ? id : id & (lanes - 1), lanes, sub, a.cols);
   unsigned char* ring = smem + (size_t)worker * (a.stages * NIN * a.slot + a.bits);
   unsigned char* bits = ring + a.stages * NIN * a.slot;
   uint64_t* full = bars[worker];
@@ -89,6 +90,7 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
     (&b[e / 2].x)[e % 2] = has && a.w.bias ? load_as(a.w.bias, a.w.dtype, c) : 0.0f;
   }
   const float n = (float)a.cols, inv = 1.0f / n;
+  if (kCta && id < 2 * NORM_MAX_WARPS) red[id / NORM_MAX_WARPS][id % NORM_MAX_WARPS] = 0.0f;
   if (kCta) __syncthreads(); else __syncwarp();
 
   uint32_t slot = 0, parity = 0;
@@ -123,38 +125,36 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
       T* xr = reinterpret_cast<T*>(in + shift) + r_at;
       T* rr = reinterpret_cast<T*>(res + shift) + r_at;
       float2 v[PAIRS];
-      __align__(16) T t[2 * PAIRS];
+      R t[PAIRS];
       part.load(xr, t);
+      part.clear(t);
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) v[i] = pair_f32(t + 2 * i);
+      for (int i = 0; i < PAIRS; ++i) v[i] = part.value(t, i);
       if (kJoin) {
         if (d.threshold) drop_part(part, v, i0 + r_at, d, kBits ? bits + ((((uint32_t)i0 & 7u) + r_at) >> 3) : bits);
         part.load(rr, t);
+        part.clear(t);
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {
-          pair_from(t + 2 * i, add2(v[i], pair_f32(t + 2 * i)));  // z, rounded as it is stored
-          v[i] = pair_f32(t + 2 * i);
+          part.set(t, i, add2(v[i], part.value(t, i)));  // z, rounded as it is stored
+          v[i] = part.value(t, i);
         }
       }
       float2 s = both(0.0f);
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) s = add2(s, v[i]);
+      for (int i = 0; i < PAIRS; ++i) s = add2(v[i], s);
       float m = s.x + s.y;
       m = quotient(kCta ? cta_sum(m, red[0], warps) : lanes_sum(m, lanes), n, inv);
       if (kCta) ok = !late;  // between two barriers: the same for all
-      s = both(0.0f);
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) {
-        v[i] = add2(v[i], both(-m));
-        s = part.fma_if(v[i], v[i], s, i);
-      }
-      float q = s.x + s.y;
+      for (int i = 0; i < PAIRS; ++i) v[i] = add2(v[i], both(-m));
+      float q = part.squares(v);
       q = rsqrtf(fmaf(kCta ? cta_sum(q, red[1], warps) : lanes_sum(q, lanes), inv, a.eps));
       if (!kCta && !kDirect) __syncwarp();  // the last row is read by all before it is written
       if (live && ok) {
         if (kJoin) part.store(kDirect ? static_cast<T*>(a.z) + i0 + r_at : rr, t);
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) pair_from(t + 2 * i, fma2(mul2(v[i], both(q)), w[i], b[i]));
+        for (int i = 0; i < PAIRS; ++i) part.set(t, i, fma2(mul2(v[i], both(q)), w[i], b[i]));
         part.store(kDirect ? static_cast<T*>(a.y) + i0 + r_at : xr, t);
         if (part.at == 0) {
           if (a.mean) a.mean[row0 + r] = m;
@@ -240,7 +240,7 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   a.err = ctx->d_err;
   const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + WORKERS - 1) / WORKERS;
   const uint64_t grid = (uint64_t)per_sm * B200_SMS;
-  const size_t smem = (size_t)WORKERS * (a.stages * NIN * a.slot + a.bits);
+  const size_t smem = (size_t)WORKERS * (a.stages * NIN * a.slot + a.bits) + NORM_PADDING;
   kernel<<<(uint32_t)(grid < most ? grid : most), threads, smem, ctx->stream>>>(a, f.d);
   ++ctx->launches;
   return vs_cuda(ctx, cudaGetLastError(), "norm launch");

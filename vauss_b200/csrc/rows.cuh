@@ -50,6 +50,7 @@ struct Dropout {
   uint32_t keys[10][2];  // the key of each round
   uint32_t offset[2];
   uint32_t threshold;    // 0: nothing is dropped, 65536: everything
+  uint32_t limit;        // 65536 threshold - 1, for `keeps` where the threshold is not 0
   float scale;
 };
 
@@ -69,15 +70,18 @@ VSD Words philox(const Dropout& d, uint64_t group) {
   return {{c0, c1, c2, c3}};
 }
 
-VSD bool keeps(const Words& w, uint32_t lane, uint32_t threshold) {
-  return ((w.w[lane >> 1] >> (16 * (lane & 1))) & 0xffffu) >= threshold;
+// Whether the value with half-word `lane` (low half first) is kept: its number,
+// moved into a word's upper half, is above `limit` = 65536 threshold - 1, which
+// no number is when the threshold is 65536.
+VSD bool keeps(const Words& w, uint32_t lane, uint32_t limit) {
+  return (lane & 1 ? w.w[lane >> 1] : w.w[lane >> 1] << 16) > limit;
 }
 // One value's decision on its own.
 VSD bool keep_at(const Dropout& d, uint64_t index) {
   const Words w = philox(d, index >> 3);
   const uint32_t j = (uint32_t)index & 7u;
   const uint32_t word = j < 4 ? (j < 2 ? w.w[0] : w.w[1]) : (j < 6 ? w.w[2] : w.w[3]);
-  return ((word >> (16 * (j & 1))) & 0xffffu) >= d.threshold;
+  return (j & 1 ? word : word << 16) > d.limit;
 }
 // A dropped value gives zero whatever it holds (NaN and infinities too).
 VSD float dropped(float v, bool keep, float scale) { return keep ? v * scale : 0.0f; }
