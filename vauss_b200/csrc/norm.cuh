@@ -174,8 +174,7 @@ VSD float keep_if(float v, uint32_t mask) { return __uint_as_float(__float_as_ui
 // out in blocks of K runs, K odd, so that a warp's narrow accesses fall into
 // different banks and every offset is a constant; there a run beyond the row
 // reads what lies behind it (the next row, or the slot's padding).  Where a row
-// does not fill its threads (`full` is false, the same for all) such values are
-// cleared before they are used.
+// does not fill a warp's lanes such values are cleared before they are used.
 constexpr uint32_t NORM_PADDING = 128;  // bytes behind the last slot that such reads may reach
 template <typename T, int VEC, int K> struct Part {
   static constexpr int E = VEC * K;
@@ -183,17 +182,17 @@ template <typename T, int VEC, int K> struct Part {
   static constexpr bool kDirect = VEC * sizeof(T) == 16;
   using R = typename Raw<T, VEC>::type;
   uint32_t at, lanes, sub;
-  bool full;
+  bool full;                      // the same for a warp
   uint32_t off[kDirect ? K : 1];  // where the runs are read
-  uint32_t mask[K];               // all ones for the runs that are the row's
+  uint32_t have;                  // the runs that are the row's, as bits (vectors) or their number (blocks)
 
-  VSD Part(uint32_t at_, uint32_t lanes_, uint32_t sub_, uint32_t cols) : at(at_), lanes(lanes_), sub(sub_) {
-    full = cols == lanes * E;
+  VSD Part(uint32_t at_, uint32_t lanes_, uint32_t sub_, uint32_t cols) : at(at_), lanes(lanes_), sub(sub_), have(0) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) mask[k] = col(k) < cols ? 0xffffffffu : 0;
+    for (int k = 0; k < K; ++k) have += col(k) < cols ? (kDirect ? 1u << k : 1u) : 0u;
+    full = __all_sync(0xffffffffu, have == (kDirect ? (1u << K) - 1 : (uint32_t)K));
     if constexpr (kDirect) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) off[k] = mask[k] ? col(k) : 0;
+      for (int k = 0; k < K; ++k) off[k] = has(k) ? col(k) : 0;
     } else {
       // a thread wholly beyond the row reads what the row's last thread reads
       const uint32_t last = (cols - 1) / E;
@@ -204,7 +203,8 @@ template <typename T, int VEC, int K> struct Part {
     if (kDirect) return (at + (K == 1 ? 0 : lanes * ((k + sub) & (K - 1)))) * VEC;
     return (at * K + k) * VEC;
   }
-  VSD bool has(int k) const { return mask[k] != 0; }
+  VSD bool has(int k) const { return kDirect ? have >> k & 1u : k < (int)have; }
+  VSD uint32_t mask(int k) const { return has(k) ? 0xffffffffu : 0u; }
   VSD void load(const T* row, R* t) const {
     if constexpr (kDirect) {
       constexpr int W = 16 / sizeof(R);
@@ -235,7 +235,7 @@ template <typename T, int VEC, int K> struct Part {
       constexpr int W = 16 / sizeof(R);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        if (!mask[k]) continue;
+        if (!has(k)) continue;
         uint4 q;
         if constexpr (W == 4) q = make_uint4(t[k * W], t[k * W + 1], t[k * W + 2], t[k * W + 3]);
         else q = make_uint4(__float_as_uint(t[k * W].x), __float_as_uint(t[k * W].y), __float_as_uint(t[k * W + 1].x),
@@ -245,11 +245,11 @@ template <typename T, int VEC, int K> struct Part {
     } else if constexpr (VEC == 2 && sizeof(T) == 2) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        if (mask[k]) reinterpret_cast<uint32_t*>(row + off[0])[k] = t[k];
+        if (has(k)) reinterpret_cast<uint32_t*>(row + off[0])[k] = t[k];
     } else {
 #pragma unroll
       for (int k = 0; k < E; ++k) {
-        if (!mask[k]) continue;
+        if (!has(k)) continue;
         if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t*>(row + off[0])[k] = (uint16_t)(&t[k / 2].x)[k % 2];
         else reinterpret_cast<float*>(row + off[0])[k] = (&t[k / 2].x)[k % 2];
       }
@@ -260,7 +260,7 @@ template <typename T, int VEC, int K> struct Part {
     if (full) return;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
-      const uint32_t mx = mask[2 * i / VEC], my = 2 * i + 1 < E ? mask[(2 * i + 1 < E ? 2 * i + 1 : 0) / VEC] : 0;
+      const uint32_t mx = mask(2 * i / VEC), my = 2 * i + 1 < E ? mask((2 * i + 1) / VEC) : 0;
       if constexpr (sizeof(T) == 4) {
         t[i].x = keep_if(t[i].x, mx);
         t[i].y = keep_if(t[i].y, my);
@@ -279,12 +279,15 @@ template <typename T, int VEC, int K> struct Part {
     float2 s = both(0.0f);
     if (full) {
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) s = fma2(v[i], v[i], s);
+      for (int i = 0; i < PAIRS; ++i) {
+        const float2 u = make_float2(v[i].x, 2 * i + 1 < E ? v[i].y : 0.0f);
+        s = fma2(u, u, s);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        const uint32_t my = 2 * i + 1 < E ? mask[(2 * i + 1 < E ? 2 * i + 1 : 0) / VEC] : 0;
-        const float2 u = make_float2(keep_if(v[i].x, mask[2 * i / VEC]), keep_if(v[i].y, my));
+        const uint32_t my = 2 * i + 1 < E ? mask((2 * i + 1) / VEC) : 0;
+        const float2 u = make_float2(keep_if(v[i].x, mask(2 * i / VEC)), keep_if(v[i].y, my));
         s = fma2(u, u, s);
       }
     }
@@ -374,8 +377,17 @@ constexpr uint32_t NORM_MAX_SMEM = 226 * 1024;
 // Threads of an SM that the CTA-per-row kernels' registers leave room for.  The
 // grids follow from this and the shape alone, never from an occupancy query, so
 // the order of the weight gradients' sums does too.
-constexpr uint32_t NORM_FWD_THREADS = 768;
-constexpr uint32_t NORM_BWD_THREADS = 512;
+constexpr uint32_t NORM_FWD_THREADS = 512;
+constexpr uint32_t NORM_BWD_THREADS = 384;
+
+// The sums of a and b over a warp in one chain: lanes 0 to 15 get a's, the others b's.
+VSD float warp_sum2(float a, float b) {
+  const bool low = (threadIdx.x & 16u) == 0;
+  float v = (low ? a : b) + __shfl_xor_sync(0xffffffffu, low ? b : a, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 
 }  // namespace vs
 

@@ -87,13 +87,19 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
     mbar_init_fence();
     for (uint32_t k = 0; k < a.stages; ++k) refill(k);
   }
-  float2 w[PAIRS], dw[PAIRS], db[PAIRS];
+  // the weights: a lane's in registers, a CTA's threads' in shared memory, each
+  // thread's own at places of its own
+  float2 w[kCta ? 1 : PAIRS], dw[PAIRS], db[PAIRS];
+  float2* ws = reinterpret_cast<float2*>(ring + a.stages * stage + a.bits) + id;
 #pragma unroll
-  for (int e = 0; e < 2 * PAIRS; ++e) {
-    const uint32_t c = part.col(e / VEC) + e % VEC;
-    const bool has = e < P::E && part.has(e / VEC);
-    (&w[e / 2].x)[e % 2] = has && a.w.weight ? load_as(a.w.weight, a.w.dtype, c) : 1.0f;
-    dw[e / 2] = db[e / 2] = both(0.0f);
+  for (int i = 0; i < PAIRS; ++i) {
+    float2 v = both(1.0f);
+#pragma unroll
+    for (int e = 2 * i; e < 2 * i + 2 && e < P::E; ++e)
+      if (part.has(e / VEC) && a.w.weight) (&v.x)[e % 2] = load_as(a.w.weight, a.w.dtype, part.col(e / VEC) + e % VEC);
+    if constexpr (kCta) ws[i * members] = v;
+    else w[i] = v;
+    dw[i] = db[i] = both(0.0f);
   }
   const float n = (float)a.cols, inv = 1.0f / n;
   if (kCta)
@@ -115,7 +121,7 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
     unsigned char* rbuf = zbuf + a.slot;  // dz, where there is one
     unsigned char* mbuf = gbuf + a.inputs * a.slot;
     unsigned char* kept = bits + (kCta ? half * (a.bits / 2) : 0);
-    const uint32_t rows = a.rows - row0 < a.tile_rows ? (uint32_t)(a.rows - row0) : a.tile_rows;
+    const uint32_t rows = kCta ? 1 : a.rows - row0 < a.tile_rows ? (uint32_t)(a.rows - row0) : a.tile_rows;
     const uint64_t i0 = begin / sizeof(T);
     const uint32_t shift = kDirect ? 0 : (uint32_t)begin & 15u;
     // the buffers' last 16-byte pieces, where they are not whole
@@ -137,8 +143,8 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
     }
     for (uint32_t p = 0; p < rows; p += per_pass) {
       // a lane beyond the tile's rows computes its last row and leaves nothing
-      const bool live = p + sub < rows;
-      const uint32_t r = live ? p + sub : rows - 1, r_at = r * a.cols;
+      const bool live = kCta || p + sub < rows;
+      const uint32_t r = kCta ? 0 : live ? p + sub : rows - 1, r_at = r * a.cols;
       T* gr = reinterpret_cast<T*>(gbuf + shift) + r_at;
       T* zr = reinterpret_cast<T*>(zbuf + shift) + r_at;
       const T* dr = reinterpret_cast<const T*>(rbuf + shift) + r_at;
@@ -147,7 +153,7 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
       R t[PAIRS], res[PAIRS];
       part.load(gr, t);
       part.clear(t);
-      if (p + per_pass > rows && !live) {  // the first test is the same for all
+      if (!kCta && p + per_pass > rows && !live) {  // the first test is the same for all
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) t[i] = R{};
       }
@@ -166,18 +172,14 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
       }
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        g[i] = mul2(g[i], w[i]);
+        g[i] = mul2(g[i], kCta ? ws[i * members] : w[kCta ? 0 : i]);
         s1 = add2(s1, g[i]);
         s2 = fma2(g[i], h[i], s2);
       }
       float m1 = s1.x + s1.y, m2 = s2.x + s2.y;
       if (kCta) {
-        m1 = warp_sum(m1);
-        m2 = warp_sum(m2);
-        if ((id & 31u) == 0) {
-          red[half][0][id >> 5] = m1;
-          red[half][1][id >> 5] = m2;
-        }
+        m1 = warp_sum2(m1, m2);
+        if ((id & 15u) == 0) red[half][id >> 4 & 1u][id >> 5] = m1;
         // `red`, `late` and the keep bits alternate between two rows, so one
         // barrier per row is enough
         __syncthreads();
@@ -287,7 +289,8 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
   }
 }
 
-template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kernel(vs_ctx* ctx, const NormBwd& f) {
+// Leaves *taken as it is where the slots do not fit.
+template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kernel(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   static std::atomic<uint64_t> ready{0};
   constexpr uint32_t WORKERS = kCta ? 1 : NORM_WARPS;
   auto kernel = norm_bwd_kernel<T, VEC, K, kJoin, kCta>;
@@ -320,23 +323,33 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   }
   a.slot = (a.tile_rows * row_bytes + 30u) & ~15u;
   a.stat_slot = (a.tile_rows * 4 + 30u) & ~15u;
-  a.bits = kJoin && VEC != 8 ? ((a.tile_rows * a.cols / 8 + 2 + 15) & ~15u) * (kCta ? 2 : 1) : 0;
-  const uint32_t stage = a.inputs * a.slot + 2 * a.stat_slot;
+  a.bits = VEC != 8 ? ((a.tile_rows * a.cols / 8 + 2 + 15) & ~15u) * (kCta ? 2 : 1) : 0;
+  // Slots and CTAs as in the forward, the CTAs as for the joined kernel's three
+  // inputs; the rings' memory also takes the warps' column sums, and a CTA's
+  // threads keep their weights behind theirs.
+  constexpr uint32_t least = Part<T, VEC, K>::kDirect ? 1 : 2;
+  const uint32_t sums = kCta ? 0 : WORKERS * 2 * a.cols * 4;
+  const uint32_t ws = kCta ? threads * Part<T, VEC, K>::PAIRS * 8 : 0;
+  auto bytes = [&](uint32_t inputs, uint32_t stages) {
+    const uint32_t rings = WORKERS * (stages * (inputs * a.slot + 2 * a.stat_slot) + a.bits);
+    return (!kCta && rings < sums ? sums : rings) + ws + NORM_PADDING;
+  };
+  auto room = [&] { return NORM_MAX_SMEM / per_sm - 1024; };
+  while (per_sm > 1 && bytes(3, 2) > room()) --per_sm;
+  if (bytes(3, least) > room()) return VS_OK;
   a.stages = NORM_STAGES;
-  while (a.stages > 2 && WORKERS * (a.stages * stage + a.bits) * per_sm > 216 * 1024) --a.stages;
+  while (a.stages > least && bytes(a.inputs, a.stages) > room()) --a.stages;
+  *taken = true;
   a.dy = f.dy; a.z = f.z; a.dz = f.dz; a.w = f.w; a.mean = f.mean; a.rstd = f.rstd;
   a.dx = f.dx; a.dresidual = f.dresidual;
   a.err = ctx->d_err;
   const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + WORKERS - 1) / WORKERS;
-  const uint64_t room = (uint64_t)per_sm * B200_SMS;
-  const uint32_t grid = (uint32_t)(room < most ? room : most);
-  size_t smem = (size_t)WORKERS * (a.stages * stage + a.bits) + NORM_PADDING;
-  const size_t sums = kCta ? 0 : (size_t)WORKERS * 2 * a.cols * 4;
-  if (smem < sums) smem = sums;
+  const uint64_t all = (uint64_t)per_sm * B200_SMS;
+  const uint32_t grid = (uint32_t)(all < most ? all : most);
   const bool want = f.dweight || f.dbias;
   // from the stream-ordered pool: calls of one ctx on several streams do not share it
   if (want) VS_CUDA(ctx, cudaMallocAsync((void**)&a.partial, (size_t)grid * 2 * a.cols * 4, ctx->stream));
-  kernel<<<grid, threads, smem, ctx->stream>>>(a, f.d);
+  kernel<<<grid, threads, bytes(a.inputs, a.stages), ctx->stream>>>(a, f.d);
   ++ctx->launches;
   vs_status st = vs_cuda(ctx, cudaGetLastError(), "norm backward launch");
   if (want) {
@@ -346,23 +359,22 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   return st;
 }
 
-// As in the forward.
-template <typename T, int VEC, int KS, int KL, bool kJoin>
+// A lane holds KS runs where one lane can hold the row, KM (16 values) up to 512
+// columns; the threads of a CTA hold KL (32).
+template <typename T, int VEC, int KS, int KM, int KL, bool kJoin>
 vs_status run_vec(vs_ctx* ctx, const NormBwd& f, bool* taken) {
-  *taken = true;
-  if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin, false>(ctx, f);
-  if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin, false>(ctx, f);
-  if (f.s.cols <= NORM_BWD_THREADS * VEC * KL) return run_kernel<T, VEC, KL, kJoin, true>(ctx, f);
-  *taken = false;
+  if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin, false>(ctx, f, taken);
+  if (f.s.cols <= 32 * VEC * KM) return run_kernel<T, VEC, KM, kJoin, false>(ctx, f, taken);
+  if (f.s.cols <= NORM_BWD_THREADS * VEC * KL) return run_kernel<T, VEC, KL, kJoin, true>(ctx, f, taken);
   return VS_OK;
 }
 
 template <typename T, bool kJoin> vs_status run(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   constexpr int V = 16 / sizeof(T);
-  if (f.s.cols % V == 0) return run_vec<T, V, 1, 16 / V, kJoin>(ctx, f, taken);
+  if (f.s.cols % V == 0) return run_vec<T, V, 1, 16 / V, 32 / V, kJoin>(ctx, f, taken);
   if constexpr (sizeof(T) == 2)
-    if (f.s.cols % 2 == 0) return run_vec<T, 2, 3, 7, kJoin>(ctx, f, taken);
-  return run_vec<T, 1, 5, 15, kJoin>(ctx, f, taken);
+    if (f.s.cols % 2 == 0) return run_vec<T, 2, 3, 7, 15, kJoin>(ctx, f, taken);
+  return run_vec<T, 1, 5, 15, 31, kJoin>(ctx, f, taken);
 }
 
 }  // namespace

@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
     (&b[e / 2].x)[e % 2] = has && a.w.bias ? load_as(a.w.bias, a.w.dtype, c) : 0.0f;
   }
   const float n = (float)a.cols, inv = 1.0f / n;
-  if (kCta && id < 2 * NORM_MAX_WARPS) red[id / NORM_MAX_WARPS][id % NORM_MAX_WARPS] = 0.0f;
+  if (kCta)
+    for (uint32_t k = id; k < 2 * NORM_MAX_WARPS; k += members) (&red[0][0])[k] = 0.0f;
   if (kCta) __syncthreads(); else __syncwarp();
 
   uint32_t slot = 0, parity = 0;
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
     }
     unsigned char* in = ring + slot * NIN * a.slot;
     unsigned char* res = in + a.slot;
-    const uint32_t rows = a.rows - row0 < a.tile_rows ? (uint32_t)(a.rows - row0) : a.tile_rows;
+    const uint32_t rows = kCta ? 1 : a.rows - row0 < a.tile_rows ? (uint32_t)(a.rows - row0) : a.tile_rows;
     const uint64_t i0 = begin / sizeof(T);
     const uint32_t shift = kDirect ? 0 : (uint32_t)begin & 15u;
     if (!kDirect && total - begin < tile_bytes + 16u) {  // the last 16-byte piece, where it is not whole
@@ -120,8 +121,8 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
     }
     for (uint32_t p = 0; p < rows; p += per_pass) {
       // a lane beyond the tile's rows computes its last row and writes nothing
-      const bool live = p + sub < rows;
-      const uint32_t r = live ? p + sub : rows - 1, r_at = r * a.cols;
+      const bool live = kCta || p + sub < rows;
+      const uint32_t r = kCta ? 0 : live ? p + sub : rows - 1, r_at = r * a.cols;
       T* xr = reinterpret_cast<T*>(in + shift) + r_at;
       T* rr = reinterpret_cast<T*>(res + shift) + r_at;
       float2 v[PAIRS];
@@ -201,9 +202,8 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
   if (!kDirect && id == 0) bulk_wait<0>();
 }
 
-// One warp's lanes hold up to 32 * VEC * K values of a row; longer rows take a
-// CTA each, if its threads' registers can hold one.
-template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kernel(vs_ctx* ctx, const NormFwd& f) {
+// Leaves *taken as it is where the slots do not fit.
+template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kernel(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   static std::atomic<uint64_t> ready{0};
   constexpr uint32_t NIN = kJoin ? 2 : 1, WORKERS = kCta ? 1 : NORM_WARPS;
   auto kernel = norm_fwd_kernel<T, VEC, K, kJoin, kCta>;
@@ -234,35 +234,42 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   }
   a.slot = (a.tile_rows * row_bytes + 30u) & ~15u;
   a.bits = kJoin && VEC != 8 ? (a.tile_rows * a.cols / 8 + 2 + 15) & ~15u : 0;
+  // as many slots as the SM's shared memory gives its CTAs, and fewer CTAs where
+  // that is less than two; a slot that is written back needs another beside it
+  constexpr uint32_t least = Part<T, VEC, K>::kDirect ? 1 : 2;
+  auto bytes = [&](uint32_t stages) { return WORKERS * (stages * NIN * a.slot + a.bits) + NORM_PADDING; };
+  auto room = [&] { return NORM_MAX_SMEM / per_sm - 1024; };
+  while (per_sm > 1 && bytes(2) > room()) --per_sm;
   a.stages = NORM_STAGES;
-  while (a.stages > 2 && WORKERS * (a.stages * NIN * a.slot + a.bits) * per_sm > 216 * 1024) --a.stages;
+  while (a.stages > least && bytes(a.stages) > room()) --a.stages;
+  if (bytes(a.stages) > room()) return VS_OK;
+  *taken = true;
   a.x = f.x; a.residual = f.residual; a.w = f.w; a.eps = f.eps; a.y = f.y; a.z = f.z; a.mean = f.mean; a.rstd = f.rstd;
   a.err = ctx->d_err;
   const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + WORKERS - 1) / WORKERS;
   const uint64_t grid = (uint64_t)per_sm * B200_SMS;
-  const size_t smem = (size_t)WORKERS * (a.stages * NIN * a.slot + a.bits) + NORM_PADDING;
-  kernel<<<(uint32_t)(grid < most ? grid : most), threads, smem, ctx->stream>>>(a, f.d);
+  kernel<<<(uint32_t)(grid < most ? grid : most), threads, bytes(a.stages), ctx->stream>>>(a, f.d);
   ++ctx->launches;
   return vs_cuda(ctx, cudaGetLastError(), "norm launch");
 }
 
-// KS values per lane where they are enough for the row, KL otherwise.
-template <typename T, int VEC, int KS, int KL, bool kJoin>
+// A lane holds KS runs where one lane can hold the row, KM (16 values) up to 512
+// columns and KL (32) beyond, on a warp or, over 1024 columns, on a CTA.
+template <typename T, int VEC, int KS, int KM, int KL, bool kJoin>
 vs_status run_vec(vs_ctx* ctx, const NormFwd& f, bool* taken) {
-  *taken = true;
-  if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin, false>(ctx, f);
-  if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin, false>(ctx, f);
-  if (f.s.cols <= NORM_FWD_THREADS * VEC * KL) return run_kernel<T, VEC, KL, kJoin, true>(ctx, f);
-  *taken = false;
+  if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin, false>(ctx, f, taken);
+  if (f.s.cols <= 32 * VEC * KM) return run_kernel<T, VEC, KM, kJoin, false>(ctx, f, taken);
+  if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin, false>(ctx, f, taken);
+  if (f.s.cols <= NORM_FWD_THREADS * VEC * KL) return run_kernel<T, VEC, KL, kJoin, true>(ctx, f, taken);
   return VS_OK;
 }
 
 template <typename T, bool kJoin> vs_status run(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   constexpr int V = 16 / sizeof(T);
-  if (f.s.cols % V == 0) return run_vec<T, V, 1, 16 / V, kJoin>(ctx, f, taken);
+  if (f.s.cols % V == 0) return run_vec<T, V, 1, 16 / V, 32 / V, kJoin>(ctx, f, taken);
   if constexpr (sizeof(T) == 2)
-    if (f.s.cols % 2 == 0) return run_vec<T, 2, 3, 7, kJoin>(ctx, f, taken);
-  return run_vec<T, 1, 5, 15, kJoin>(ctx, f, taken);
+    if (f.s.cols % 2 == 0) return run_vec<T, 2, 3, 7, 15, kJoin>(ctx, f, taken);
+  return run_vec<T, 1, 5, 15, 31, kJoin>(ctx, f, taken);
 }
 
 }  // namespace
