@@ -168,9 +168,8 @@ VSD float keep_if(float v, uint32_t mask) { return __uint_as_float(__float_as_ui
 
 // The values of a row that one thread holds: K runs of VEC.  Rows of whole
 // 16-byte vectors are dealt out vector by vector, so that a warp's accesses are
-// contiguous; the runs' order turns with the row's place in the warp, which
-// keeps neighbouring rows of 64 bytes apart off each other's shared-memory
-// banks; a run beyond the row reads the row's first one.  Other rows are dealt
+// contiguous; where K is even the runs' order turns with the row's place in the
+// warp, which keeps the rows' like runs off each other's shared-memory banks; a run beyond the row reads the row's first one.  Other rows are dealt
 // out in blocks of K runs, K odd, so that a warp's narrow accesses fall into
 // different banks and every offset is a constant; there a run beyond the row
 // reads what lies behind it (the next row, or the slot's padding).  Where a row
@@ -185,11 +184,17 @@ template <typename T, int VEC, int K> struct Part {
   bool full;                      // the same for a warp
   uint32_t off[kDirect ? K : 1];  // where the runs are read
   uint32_t have;                  // the runs that are the row's, as bits (vectors) or their number (blocks)
+  static constexpr bool kMasks = K <= 15;
+  uint32_t masks[kMasks ? K : 1];  // all ones for the row's runs, where registers allow
 
   VSD Part(uint32_t at_, uint32_t lanes_, uint32_t sub_, uint32_t cols) : at(at_), lanes(lanes_), sub(sub_), have(0) {
 #pragma unroll
     for (int k = 0; k < K; ++k) have += col(k) < cols ? (kDirect ? 1u << k : 1u) : 0u;
     full = __all_sync(0xffffffffu, have == (kDirect ? (1u << K) - 1 : (uint32_t)K));
+    if constexpr (kMasks) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) masks[k] = has(k) ? 0xffffffffu : 0u;
+    }
     if constexpr (kDirect) {
 #pragma unroll
       for (int k = 0; k < K; ++k) off[k] = has(k) ? col(k) : 0;
@@ -200,11 +205,14 @@ template <typename T, int VEC, int K> struct Part {
     }
   }
   VSD uint32_t col(int k) const {
-    if (kDirect) return (at + (K == 1 ? 0 : lanes * ((k + sub) & (K - 1)))) * VEC;
+    if (kDirect) return (at + lanes * (K % 2 ? k : (k + sub) % K)) * VEC;
     return (at * K + k) * VEC;
   }
   VSD bool has(int k) const { return kDirect ? have >> k & 1u : k < (int)have; }
-  VSD uint32_t mask(int k) const { return has(k) ? 0xffffffffu : 0u; }
+  VSD uint32_t mask(int k) const {
+    if constexpr (kMasks) return masks[k];
+    else return has(k) ? 0xffffffffu : 0u;
+  }
   VSD void load(const T* row, R* t) const {
     if constexpr (kDirect) {
       constexpr int W = 16 / sizeof(R);
@@ -274,24 +282,19 @@ template <typename T, int VEC, int K> struct Part {
   }
   VSD float2 value(const R* t, int pair) const { return unpack(static_cast<const T*>(nullptr), t[pair]); }
   VSD void set(R* t, int pair, float2 v) const { pack(static_cast<const T*>(nullptr), v, t[pair]); }
-  // The sum of the squares of the row's values among v.
-  VSD float squares(const float2* v) const {
-    float2 s = both(0.0f);
+  // v - m for the row's values, zero for the others (which hold zero)
+  VSD void subtract(float2* v, float m) const {
     if (full) {
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) {
-        const float2 u = make_float2(v[i].x, 2 * i + 1 < E ? v[i].y : 0.0f);
-        s = fma2(u, u, s);
-      }
+      for (int i = 0; i < PAIRS; ++i) v[i] = add2(v[i], 2 * i + 1 < E ? both(-m) : make_float2(-m, 0.0f));
     } else {
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        const uint32_t my = 2 * i + 1 < E ? mask((2 * i + 1) / VEC) : 0;
-        const float2 u = make_float2(keep_if(v[i].x, mask(2 * i / VEC)), keep_if(v[i].y, my));
-        s = fma2(u, u, s);
+        const float x = keep_if(-m, mask(2 * i / VEC));
+        const float y = 2 * i + 1 >= E ? 0.0f : VEC > 1 ? x : keep_if(-m, mask((2 * i + 1) / VEC));
+        v[i] = add2(v[i], make_float2(x, y));
       }
     }
-    return s.x + s.y;
   }
 };
 
@@ -319,33 +322,43 @@ VSD uint32_t keep_bits(const Words& w, uint32_t limit) {
 }
 
 // Dropout of a thread's values: v holds pairs, i0 is the row's first index.
-// Runs of eight are groups of the generator; for others the group's bits have
-// been left in `bits`, whose first bit is the decision of index i0 & ~7.
+// Runs of eight are groups of the generator; for others the decisions have been
+// left in `bits`, the row's first at bit `at`.
 template <typename T, int VEC, int K>
-VSD void drop_part(const Part<T, VEC, K>& part, float2* v, uint64_t i0, const Dropout& d, const unsigned char* bits) {
+VSD void drop_part(const Part<T, VEC, K>& part, float2* v, uint64_t i0, const Dropout& d, const uint32_t* bits,
+                   uint32_t at) {
   const float2 scale = both(d.scale);
 #pragma unroll
   for (int i = 0; i < part.PAIRS; ++i) v[i] = mul2(v[i], scale);
   float* f = reinterpret_cast<float*>(v);
+  if constexpr (VEC == 8) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (VEC == 8) {
-      const Words words = philox(d, (i0 + part.off[part.kDirect ? k : 0]) >> 3);
+    for (int k = 0; k < K; ++k) {
+      const Words words = philox(d, (i0 + part.off[k]) >> 3);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) f[k * VEC + j] = keeps(words, j, d.limit) ? f[k * VEC + j] : 0.0f;
-    } else {
-      const uint32_t e = ((uint32_t)i0 & 7u) + (part.kDirect ? part.off[part.kDirect ? k : 0] : part.off[0] + k * VEC);
-      const uint32_t kept = bits[e >> 3] >> (e & 7u);
+    }
+  } else if constexpr (part.kDirect) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const uint32_t e = at + part.off[k];
+      const uint32_t kept = reinterpret_cast<const unsigned char*>(bits)[e >> 3] >> (e & 7u);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) f[k * VEC + j] = kept >> j & 1u ? f[k * VEC + j] : 0.0f;
     }
+  } else {  // a block of at most 32 values
+    const uint32_t e = at + part.off[0];
+    const uint32_t kept = __funnelshift_r(bits[e >> 5], bits[(e >> 5) + 1], e & 31u);
+#pragma unroll
+    for (int j = 0; j < part.E; ++j) f[j] = kept >> j & 1u ? f[j] : 0.0f;
   }
 }
-// Leaves the bits of indices [i0, i0 + count) for drop_part.
-VSD void fill_bits(const Dropout& d, uint64_t i0, uint32_t count, unsigned char* bits, uint32_t id, uint32_t members) {
+// Leaves the decisions of indices [i0, i0 + count) for drop_part, the first at bit i0 & 7.
+VSD void fill_bits(const Dropout& d, uint64_t i0, uint32_t count, uint32_t* bits, uint32_t id, uint32_t members) {
   const uint64_t g0 = i0 >> 3;
   const uint32_t groups = (((uint32_t)i0 & 7u) + count + 7) >> 3;
-  for (uint32_t g = id; g < groups; g += members) bits[g] = (unsigned char)keep_bits(philox(d, g0 + g), d.limit);
+  for (uint32_t g = id; g < groups; g += members)
+    reinterpret_cast<unsigned char*>(bits)[g] = (unsigned char)keep_bits(philox(d, g0 + g), d.limit);
 }
 
 // The sum over a CTA, the same in every thread; `part` holds a value per warp,
@@ -411,6 +424,23 @@ struct NormBwd {
   int32_t wdtype;
   void *dweight, *dbias;
 };
+
+// The runs a lane holds of a row of `chunks` runs, 1 to `most`, with the fewest
+// idle places on the row's lanes (a power of two of them), then the most runs; 0
+// where a warp cannot hold the row.
+inline int norm_runs(uint32_t chunks, int most) {
+  int best = 0;
+  uint32_t places = ~0u;
+  for (int k = 1; k <= most; ++k) {
+    uint32_t lanes = 1;
+    while (lanes * k < chunks) lanes *= 2;
+    if (lanes <= 32 && lanes * k <= places) {
+      best = k;
+      places = lanes * k;
+    }
+  }
+  return best;
+}
 
 // The streaming kernels take contiguous rows on 16-byte aligned buffers;
 // *taken tells whether the shape is one of theirs.

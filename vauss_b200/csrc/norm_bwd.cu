@@ -13,8 +13,15 @@ namespace {
 
 using namespace vs;
 
-// As in the forward.
-constexpr int warp_ctas(int elems) { return elems > 8 ? 3 : 5; }
+// As in the forward: f32 rows of 256 reach 94 % of the copy rate with 8 warps
+// and 85 % with 12; bf16 rows of 256 93 % with 12 warps of 16 values a lane and
+// slots of 3 KB, 80 % with 8 warps of 32 values.
+template <typename T, int VEC, int K> constexpr int warp_ctas() {
+  if (VEC * K <= 8) return 5;
+  if (VEC * K > 16) return 2;
+  return VEC * sizeof(T) == 16 && sizeof(T) == 4 ? 2 : 3;
+}
+template <typename T, int VEC> constexpr uint32_t warp_slot() { return VEC * sizeof(T) == 16 && sizeof(T) == 4 ? 2048 : 3072; }
 
 struct BwdArgs {
   uint64_t rows;
@@ -30,7 +37,7 @@ struct BwdArgs {
 // Whole-vector rows are written from registers, others through their slots, as
 // in the forward.
 template <typename T, int VEC, int K, bool kJoin, bool kCta>
-__global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCta ? 1 : warp_ctas(VEC * K))
+__global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCta ? 1 : warp_ctas<T, VEC, K>())
     norm_bwd_kernel(const BwdArgs a, const __grid_constant__ Dropout d) {
   using P = Part<T, VEC, K>;
   using R = typename P::R;
@@ -120,7 +127,7 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
     unsigned char* zbuf = gbuf + a.slot;
     unsigned char* rbuf = zbuf + a.slot;  // dz, where there is one
     unsigned char* mbuf = gbuf + a.inputs * a.slot;
-    unsigned char* kept = bits + (kCta ? half * (a.bits / 2) : 0);
+    uint32_t* kept = reinterpret_cast<uint32_t*>(bits + (kCta ? half * (a.bits / 2) : 0));
     const uint32_t rows = kCta ? 1 : a.rows - row0 < a.tile_rows ? (uint32_t)(a.rows - row0) : a.tile_rows;
     const uint64_t i0 = begin / sizeof(T);
     const uint32_t shift = kDirect ? 0 : (uint32_t)begin & 15u;
@@ -204,7 +211,7 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
 #pragma unroll
           for (int i = 0; i < PAIRS; ++i) part.set(t, i, g[i]);
           part.store(kDirect ? static_cast<T*>(a.dresidual) + i0 + r_at : zr, t);
-          if (d.threshold) drop_part(part, g, i0 + r_at, d, kBits ? kept + ((((uint32_t)i0 & 7u) + r_at) >> 3) : kept);
+          if (d.threshold) drop_part(part, g, i0 + r_at, d, kept, ((uint32_t)i0 & 7u) + r_at);
         }
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) part.set(t, i, g[i]);
@@ -228,7 +235,7 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
       if (id == 0) {
         bulk_commit();
         bulk_wait_read<1>();
-        if (row0 >= step_rows) refill(slot == 0 ? a.stages - 1 : slot - 1);
+        if (row0 != first * a.tile_rows) refill(slot == 0 ? a.stages - 1 : slot - 1);
       }
       if (!kCta) __syncwarp();
     }
@@ -304,18 +311,17 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   a.cols = f.s.cols;
   a.inputs = f.dz ? 3 : 2;
   const uint32_t chunks = (a.cols + VEC - 1) / VEC, row_bytes = a.cols * (uint32_t)sizeof(T);
-  uint32_t threads = NORM_WARPS * 32, per_sm = warp_ctas(VEC * K);
+  uint32_t threads = NORM_WARPS * 32, per_sm = warp_ctas<T, VEC, K>();
   a.tile_rows = 1;
   if (kCta) {
     threads = ((chunks + K - 1) / K + 31) & ~31u;
     per_sm = NORM_BWD_THREADS / threads;
   } else {
     while ((1u << a.log_lanes) * K < chunks) ++a.log_lanes;
-    // About 1 KB of copies per slot and input, otherwise as in the forward.
-    // The same for the plain and the joined kernel, so that their weight
-    // gradients are the same sums in the same order.
+    // As in the forward, and the same for the plain and the joined kernel, so
+    // that their weight gradients are the same sums in the same order.
     const uint32_t per_pass = 32u >> a.log_lanes;
-    uint32_t passes = 1024 / (row_bytes * per_pass);
+    uint32_t passes = warp_slot<T, VEC>() / (row_bytes * per_pass);
     const uint64_t share = (uint64_t)B200_SMS * per_sm * WORKERS * per_pass;
     const uint64_t even = (a.rows + share - 1) / share;
     if (passes > even) passes = (uint32_t)even;
@@ -337,7 +343,7 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   auto room = [&] { return NORM_MAX_SMEM / per_sm - 1024; };
   while (per_sm > 1 && bytes(3, 2) > room()) --per_sm;
   if (bytes(3, least) > room()) return VS_OK;
-  a.stages = NORM_STAGES;
+  a.stages = Part<T, VEC, K>::kDirect ? 2 : 3;
   while (a.stages > least && bytes(a.inputs, a.stages) > room()) --a.stages;
   *taken = true;
   a.dy = f.dy; a.z = f.z; a.dz = f.dz; a.w = f.w; a.mean = f.mean; a.rstd = f.rstd;
@@ -359,22 +365,40 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   return st;
 }
 
-// A lane holds KS runs where one lane can hold the row, KM (16 values) up to 512
-// columns; the threads of a CTA hold KL (32).
-template <typename T, int VEC, int KS, int KM, int KL, bool kJoin>
-vs_status run_vec(vs_ctx* ctx, const NormBwd& f, bool* taken) {
+// As in the forward, with up to 3 runs of 8 or 4 of 4 values per lane; a CTA's
+// threads hold up to 32 values.
+template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormBwd& f, bool* taken) {
+  constexpr int V = 16 / sizeof(T);
+  const uint32_t chunks = f.s.cols / V;
+  switch (norm_runs(chunks, sizeof(T) == 4 ? 4 : 3)) {
+    case 1: return run_kernel<T, V, 1, kJoin, false>(ctx, f, taken);
+    case 2: return run_kernel<T, V, 2, kJoin, false>(ctx, f, taken);
+    case 3: return run_kernel<T, V, 3, kJoin, false>(ctx, f, taken);
+    case 4:
+      if constexpr (sizeof(T) == 4) return run_kernel<T, V, 4, kJoin, false>(ctx, f, taken);
+  }
+  if (sizeof(T) == 2 || chunks <= 128 * 4) {
+    if (chunks <= NORM_BWD_THREADS * 4) return run_kernel<T, V, 4, kJoin, true>(ctx, f, taken);
+  } else if (chunks <= NORM_BWD_THREADS * 8) {
+    return run_kernel<float, 4, 8, kJoin, true>(ctx, f, taken);
+  }
+  return VS_OK;
+}
+
+template <typename T, int VEC, int KS, int KL, bool kJoin>
+vs_status run_blocks(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin, false>(ctx, f, taken);
-  if (f.s.cols <= 32 * VEC * KM) return run_kernel<T, VEC, KM, kJoin, false>(ctx, f, taken);
+  if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin, false>(ctx, f, taken);
   if (f.s.cols <= NORM_BWD_THREADS * VEC * KL) return run_kernel<T, VEC, KL, kJoin, true>(ctx, f, taken);
+  if (f.s.cols <= NORM_BWD_THREADS * VEC * (2 * KL + 1)) return run_kernel<T, VEC, 2 * KL + 1, kJoin, true>(ctx, f, taken);
   return VS_OK;
 }
 
 template <typename T, bool kJoin> vs_status run(vs_ctx* ctx, const NormBwd& f, bool* taken) {
-  constexpr int V = 16 / sizeof(T);
-  if (f.s.cols % V == 0) return run_vec<T, V, 1, 16 / V, 32 / V, kJoin>(ctx, f, taken);
+  if (f.s.cols % (16 / sizeof(T)) == 0) return run_vectors<T, kJoin>(ctx, f, taken);
   if constexpr (sizeof(T) == 2)
-    if (f.s.cols % 2 == 0) return run_vec<T, 2, 3, 7, 15, kJoin>(ctx, f, taken);
-  return run_vec<T, 1, 5, 15, 31, kJoin>(ctx, f, taken);
+    if (f.s.cols % 2 == 0) return run_blocks<T, 2, 3, 7, kJoin>(ctx, f, taken);
+  return run_blocks<T, 1, 5, 15, kJoin>(ctx, f, taken);
 }
 
 }  // namespace

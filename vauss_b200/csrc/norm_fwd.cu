@@ -15,9 +15,20 @@ namespace {
 
 using namespace vs;
 
-// CTAs of the warp workers on an SM, by the values a lane holds: their
-// registers fix it.
-constexpr int warp_ctas(int elems) { return elems > 8 ? 4 : 7; }
+// CTAs of the warp workers on an SM, and the bytes of one slot and input.  Two
+// things meet here.  Every byte in flight beyond what hides the latency only
+// queues in front of the DRAM and costs throughput (f32 rows of 256, two slots
+// of 2 KB a warp: 12 warps 97 % of the copy rate, 16 warps 86 %; joined, two
+// inputs: 8 warps 96 %, 12 warps 83 %), while 16-bit rows need the warps'
+// arithmetic (bf16 rows of 64, 16 values a lane: 16 warps 91 %, 12 warps 87 %;
+// of 512, 32 values a lane: 12 warps 92 %).  Slots that are written back need
+// longer runs (59 f32: 4 KB 97 %, 2 KB 80 %).
+template <typename T, int VEC, int K, bool kJoin> constexpr int warp_ctas() {
+  if (VEC * K <= 8) return 6;
+  if (VEC * sizeof(T) == 16 && sizeof(T) == 4) return kJoin ? 2 : 3;
+  return VEC * K > 16 || sizeof(T) == 4 ? 3 : 4;
+}
+template <typename T, int VEC> constexpr uint32_t warp_slot() { return VEC * sizeof(T) == 16 ? 2048 : 4096; }
 
 struct FwdArgs {
   uint64_t rows;
@@ -34,7 +45,7 @@ struct FwdArgs {
 // their slot and out by a bulk store, so that no access is narrower than its
 // run of bytes.
 template <typename T, int VEC, int K, bool kJoin, bool kCta>
-__global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCta ? 1 : warp_ctas(VEC * K))
+__global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCta ? 1 : warp_ctas<T, VEC, K, kJoin>())
     norm_fwd_kernel(const FwdArgs a, const __grid_constant__ Dropout d) {
   using P = Part<T, VEC, K>;
   using R = typename P::R;
@@ -53,7 +64,7 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
   const uint32_t sub = kCta ? 0 : id >> a.log_lanes, per_pass = kCta ? 1 : 32u >> a.log_lanes;
   const P part(kCta ? id : id & (lanes - 1), lanes, sub, a.cols);
   unsigned char* ring = smem + (size_t)worker * (a.stages * NIN * a.slot + a.bits);
-  unsigned char* bits = ring + a.stages * NIN * a.slot;
+  uint32_t* bits = reinterpret_cast<uint32_t*>(ring + a.stages * NIN * a.slot);
   uint64_t* full = bars[worker];
 
   const uint64_t first = (uint64_t)blockIdx.x * WORKERS + worker, step = (uint64_t)gridDim.x * WORKERS;
@@ -132,7 +143,7 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) v[i] = part.value(t, i);
       if (kJoin) {
-        if (d.threshold) drop_part(part, v, i0 + r_at, d, kBits ? bits + ((((uint32_t)i0 & 7u) + r_at) >> 3) : bits);
+        if (d.threshold) drop_part(part, v, i0 + r_at, d, bits, ((uint32_t)i0 & 7u) + r_at);
         part.load(rr, t);
         part.clear(t);
 #pragma unroll
@@ -147,9 +158,11 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
       float m = s.x + s.y;
       m = quotient(kCta ? cta_sum(m, red[0], warps) : lanes_sum(m, lanes), n, inv);
       if (kCta) ok = !late;  // between two barriers: the same for all
+      part.subtract(v, m);
+      s = both(0.0f);
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) v[i] = add2(v[i], both(-m));
-      float q = part.squares(v);
+      for (int i = 0; i < PAIRS; ++i) s = fma2(v[i], v[i], s);
+      float q = s.x + s.y;
       q = rsqrtf(fmaf(kCta ? cta_sum(q, red[1], warps) : lanes_sum(q, lanes), inv, a.eps));
       if (!kCta && !kDirect) __syncwarp();  // the last row is read by all before it is written
       if (live && ok) {
@@ -180,7 +193,7 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
         bulk_commit();
         // the slot before this one has been read out by now: it is filled again
         bulk_wait_read<1>();
-        if (row0 >= step * a.tile_rows) refill(slot == 0 ? a.stages - 1 : slot - 1);
+        if (row0 != first * a.tile_rows) refill(slot == 0 ? a.stages - 1 : slot - 1);
       }
       if (!kCta) __syncwarp();
     }
@@ -216,17 +229,16 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   a.rows = f.s.rows;
   a.cols = f.s.cols;
   const uint32_t chunks = (a.cols + VEC - 1) / VEC, row_bytes = a.cols * (uint32_t)sizeof(T);
-  uint32_t threads = NORM_WARPS * 32, per_sm = warp_ctas(VEC * K);
+  uint32_t threads = NORM_WARPS * 32, per_sm = warp_ctas<T, VEC, K, kJoin>();
   a.tile_rows = 1;
   if (kCta) {
     threads = ((chunks + K - 1) / K + 31) & ~31u;
     per_sm = NORM_FWD_THREADS / threads;
   } else {
     while ((1u << a.log_lanes) * K < chunks) ++a.log_lanes;
-    // about 2 KB of copies per slot, in whole passes; fewer where that would
-    // leave warps without rows
+    // whole passes per slot; fewer where that would leave warps without rows
     const uint32_t per_pass = 32u >> a.log_lanes;
-    uint32_t passes = 2048 / NIN / (row_bytes * per_pass);
+    uint32_t passes = warp_slot<T, VEC>() / (row_bytes * per_pass);
     const uint64_t share = (uint64_t)B200_SMS * per_sm * WORKERS * per_pass;
     const uint64_t even = (a.rows + share - 1) / share;
     if (passes > even) passes = (uint32_t)even;
@@ -234,13 +246,15 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   }
   a.slot = (a.tile_rows * row_bytes + 30u) & ~15u;
   a.bits = kJoin && VEC != 8 ? (a.tile_rows * a.cols / 8 + 2 + 15) & ~15u : 0;
-  // as many slots as the SM's shared memory gives its CTAs, and fewer CTAs where
-  // that is less than two; a slot that is written back needs another beside it
+  // Two slots: one being worked on, one on its way (a third one costs rows of
+  // 4096 bf16 13 %, see above), and a third for slots that are written back; fewer
+  // CTAs where the SM's shared memory does not hold theirs.  A slot that is
+  // written back needs at least another beside it.
   constexpr uint32_t least = Part<T, VEC, K>::kDirect ? 1 : 2;
   auto bytes = [&](uint32_t stages) { return WORKERS * (stages * NIN * a.slot + a.bits) + NORM_PADDING; };
   auto room = [&] { return NORM_MAX_SMEM / per_sm - 1024; };
   while (per_sm > 1 && bytes(2) > room()) --per_sm;
-  a.stages = NORM_STAGES;
+  a.stages = Part<T, VEC, K>::kDirect ? 2 : 3;
   while (a.stages > least && bytes(a.stages) > room()) --a.stages;
   if (bytes(a.stages) > room()) return VS_OK;
   *taken = true;
@@ -253,23 +267,37 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   return vs_cuda(ctx, cudaGetLastError(), "norm launch");
 }
 
-// A lane holds KS runs where one lane can hold the row, KM (16 values) up to 512
-// columns and KL (32) beyond, on a warp or, over 1024 columns, on a CTA.
-template <typename T, int VEC, int KS, int KM, int KL, bool kJoin>
-vs_status run_vec(vs_ctx* ctx, const NormFwd& f, bool* taken) {
+// The runs per lane, of 1 to 4, with the fewest idle places on a warp's lanes
+// (then the most, for the fewest shuffles); rows over a warp's 4 runs take a CTA.
+template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormFwd& f, bool* taken) {
+  constexpr int V = 16 / sizeof(T);
+  const uint32_t chunks = f.s.cols / V;
+  switch (norm_runs(chunks, 4)) {
+    case 1: return run_kernel<T, V, 1, kJoin, false>(ctx, f, taken);
+    case 2: return run_kernel<T, V, 2, kJoin, false>(ctx, f, taken);
+    case 3: return run_kernel<T, V, 3, kJoin, false>(ctx, f, taken);
+    case 4: return run_kernel<T, V, 4, kJoin, false>(ctx, f, taken);
+  }
+  if (chunks <= NORM_FWD_THREADS * 4) return run_kernel<T, V, 4, kJoin, true>(ctx, f, taken);
+  if (sizeof(T) == 4 && chunks <= NORM_FWD_THREADS * 8) return run_kernel<float, 4, 8, kJoin, true>(ctx, f, taken);
+  return VS_OK;
+}
+
+// KS runs in a block where they hold the row, KL otherwise.
+template <typename T, int VEC, int KS, int KL, bool kJoin>
+vs_status run_blocks(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin, false>(ctx, f, taken);
-  if (f.s.cols <= 32 * VEC * KM) return run_kernel<T, VEC, KM, kJoin, false>(ctx, f, taken);
   if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin, false>(ctx, f, taken);
   if (f.s.cols <= NORM_FWD_THREADS * VEC * KL) return run_kernel<T, VEC, KL, kJoin, true>(ctx, f, taken);
+  if (f.s.cols <= NORM_FWD_THREADS * VEC * (2 * KL + 1)) return run_kernel<T, VEC, 2 * KL + 1, kJoin, true>(ctx, f, taken);
   return VS_OK;
 }
 
 template <typename T, bool kJoin> vs_status run(vs_ctx* ctx, const NormFwd& f, bool* taken) {
-  constexpr int V = 16 / sizeof(T);
-  if (f.s.cols % V == 0) return run_vec<T, V, 1, 16 / V, 32 / V, kJoin>(ctx, f, taken);
+  if (f.s.cols % (16 / sizeof(T)) == 0) return run_vectors<T, kJoin>(ctx, f, taken);
   if constexpr (sizeof(T) == 2)
-    if (f.s.cols % 2 == 0) return run_vec<T, 2, 3, 7, 15, kJoin>(ctx, f, taken);
-  return run_vec<T, 1, 5, 15, 31, kJoin>(ctx, f, taken);
+    if (f.s.cols % 2 == 0) return run_blocks<T, 2, 3, 7, kJoin>(ctx, f, taken);
+  return run_blocks<T, 1, 5, 15, kJoin>(ctx, f, taken);
 }
 
 }  // namespace
