@@ -6,6 +6,7 @@
 //   backward  h = (z - m) q, g = dy w,
 //             t = q (g - mean g - h mean(g h)) (+ dz),
 //             dresidual = t, dx = dropout(t), dw = sum_rows dy h, db = sum_rows dy
+#include <stdlib.h>
 #include <initializer_list>
 
 #include "norm.cuh"
@@ -126,28 +127,45 @@ __global__ void __launch_bounds__(256) norm_cols_kernel(Shape s, Mat<const T> dy
   }
 }
 
-// dw and db from the strips' partial sums, 32 columns x 32 strips of threads.
+// dw and db from `strips` partial sums [strips][2][cols]: a CTA takes 32 columns
+// of one of the two, 128 groups of 8 threads take every 128th strip's 16-byte
+// pieces of them (8 loads of 16 bytes in flight for 1024 strips), and the groups'
+// sums are added in a fixed order.
 __global__ void __launch_bounds__(1024) norm_join_kernel(uint32_t cols, uint32_t strips, const float* partial,
                                                          int32_t dtype, void* dweight, void* dbias) {
-  __shared__ float sw[32][33], sb[32][33];
-  const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x;
-  float w = 0.0f, b = 0.0f;
-  if (c < cols) {
-    for (uint32_t k = threadIdx.y; k < strips; k += 32) {
-      w += partial[(uint64_t)k * 2 * cols + c];
-      b += partial[(uint64_t)k * 2 * cols + cols + c];
+  __shared__ float4 part[128][9];
+  const uint32_t piece = threadIdx.x & 7u, group = threadIdx.x >> 3;
+  const uint32_t c = blockIdx.x * 32 + piece * 4;
+  const float* from = partial + (uint64_t)blockIdx.y * cols + c;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (cols % 4 == 0) {
+    if (c < cols) {
+#pragma unroll 4
+      for (uint32_t k = group; k < strips; k += 128) {
+        const float4 v = *reinterpret_cast<const float4*>(from + (uint64_t)k * 2 * cols);
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      }
+    }
+  } else {
+#pragma unroll 2
+    for (uint32_t k = group; k < strips; k += 128) {
+      const float* p = from + (uint64_t)k * 2 * cols;
+      if (c < cols) s.x += p[0];
+      if (c + 1 < cols) s.y += p[1];
+      if (c + 2 < cols) s.z += p[2];
+      if (c + 3 < cols) s.w += p[3];
     }
   }
-  sw[threadIdx.y][threadIdx.x] = w;
-  sb[threadIdx.y][threadIdx.x] = b;
+  part[group][piece] = s;
   __syncthreads();
-  w = warp_sum(sw[threadIdx.x][threadIdx.y]);
-  b = warp_sum(sb[threadIdx.x][threadIdx.y]);
-  const uint64_t oc = (uint64_t)blockIdx.x * 32 + threadIdx.y;
-  if (threadIdx.x == 0 && oc < cols) {
-    if (dweight) store_as(dweight, dtype, oc, w);
-    if (dbias) store_as(dbias, dtype, oc, b);
-  }
+  // 32 columns x 32 threads, four groups each
+  const uint32_t col = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  float v = 0.0f;
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) v += reinterpret_cast<const float*>(&part[lane + 32 * k][col >> 2])[col & 3u];
+  v = warp_sum(v);
+  void* out = blockIdx.y ? dbias : dweight;
+  if (lane == 0 && blockIdx.x * 32 + col < cols && out) store_as(out, dtype, blockIdx.x * 32 + col, v);
 }
 
 // What every entry point checks of its shape.
@@ -191,6 +209,12 @@ bool vector_rows(Shape s, std::initializer_list<uint64_t> strides, std::initiali
   return true;
 }
 
+// Calls whose traffic the direct kernels finish before rings would be full.
+bool is_small(Shape s, size_t bytes_per_value) {
+  static const double lim = getenv("VS_SMALL") ? atof(getenv("VS_SMALL")) : 8e6;
+  return (double)s.rows * s.cols * bytes_per_value < lim;
+}
+
 uint32_t row_grid(uint64_t rows) { return (uint32_t)(rows < 0x7fffffffull ? rows : 0x7fffffffull); }
 
 template <typename T, bool kJoin>
@@ -209,12 +233,14 @@ vs_status norm_forward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, co
   if (!(eps >= 0.0f) || eps > 3e38f) return vs_fail(ctx, VS_ERR_INVALID, "%s: eps = %g", what, (double)eps);
   if (s.rows == 0) return VS_OK;
   VS_CUDA(ctx, cudaSetDevice(ctx->device));
-  if (vector_rows(s, {mx.stride, kJoin ? mr.stride : mx.stride}, {x, residual, y, z})) {
-    bool taken = false;
-    const NormFwd f{s, x, residual, wt, eps, d, y, z, mean, rstd};
-    VS_TRY(norm_stream_forward(ctx, dtype, kJoin, f, &taken));
-    if (taken) return VS_OK;
-  }
+  const NormFwd f{s, x, residual, mx.stride, mr.stride, wt, eps, d, y, z, mean, rstd};
+  const bool stream = vector_rows(s, {mx.stride, kJoin ? mr.stride : mx.stride}, {x, residual, y, z});
+  const bool small = is_small(s, sizeof(T) * (kJoin ? 4 : 2));
+  bool taken = false;
+  if (stream && !small) VS_TRY(norm_stream_forward(ctx, dtype, kJoin, f, &taken));
+  if (!taken) VS_TRY(norm_direct_forward(ctx, dtype, kJoin, f, &taken));
+  if (!taken && stream && small) VS_TRY(norm_stream_forward(ctx, dtype, kJoin, f, &taken));
+  if (taken) return VS_OK;
   norm_fwd_rows_kernel<T, kJoin><<<row_grid(s.rows), 256, 0, ctx->stream>>>(s, mx, mr, wt, eps, d, (T*)y, (T*)z, mean,
                                                                             rstd);
   ++ctx->launches;
@@ -242,13 +268,17 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, c
     if (dbias) VS_CUDA(ctx, cudaMemsetAsync(dbias, 0, s.cols * vs_dtype_size(wt.dtype), ctx->stream));
     return VS_OK;
   }
-  if (vector_rows(s, {mdy.stride, mz.stride, kJoin && dz ? mdz.stride : mz.stride},
-                  {dy, dz, z, dx, dresidual, mean, rstd})) {
-    bool taken = false;
-    const NormBwd f{s, dy, kJoin ? dz : nullptr, z, wt, mean, rstd, d, dx, dresidual, wt.dtype, dweight, dbias};
-    VS_TRY(norm_stream_backward(ctx, dtype, kJoin, f, &taken));
-    if (taken) return VS_OK;
-  }
+  const NormBwd f{s, dy, kJoin ? dz : nullptr, z, mdy.stride, mdz.stride, mz.stride, wt, mean, rstd, d, dx, dresidual,
+                  wt.dtype, dweight, dbias};
+  const bool stream = vector_rows(s, {mdy.stride, mz.stride, kJoin && dz ? mdz.stride : mz.stride},
+                                  {dy, dz, z, dx, dresidual, mean, rstd});
+  // by the plain kernel's traffic, so that the joined one's weight gradients are the same sums
+  const bool small = is_small(s, sizeof(T) * 3);
+  bool taken = false;
+  if (stream && !small) VS_TRY(norm_stream_backward(ctx, dtype, kJoin, f, &taken));
+  if (!taken) VS_TRY(norm_direct_backward(ctx, dtype, kJoin, f, &taken));
+  if (!taken && stream && small) VS_TRY(norm_stream_backward(ctx, dtype, kJoin, f, &taken));
+  if (taken) return VS_OK;
   // the column sums read dy, which dx may overwrite, so they come first
   if (dweight || dbias) {
     const uint32_t col_blocks = (s.cols + 31) / 32;
@@ -256,15 +286,15 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, c
     const uint64_t most = (s.rows + 63) / 64;
     const uint32_t strips = (uint32_t)(want < most ? want : most);
     const uint64_t strip = (s.rows + strips - 1) / strips;
-    float* partial = nullptr;
-    // from the stream-ordered pool: calls of one ctx on several streams do not share it
-    VS_CUDA(ctx, cudaMallocAsync((void**)&partial, (size_t)strips * 2 * s.cols * 4, ctx->stream));
+    NormScratch scratch;
+    VS_TRY(norm_scratch_begin(ctx, (size_t)strips * 2 * s.cols, &scratch));
     norm_cols_kernel<T><<<dim3(col_blocks, strips), dim3(32, 8), 0, ctx->stream>>>(s, mdy, mz, mean, rstd, strip,
-                                                                                  partial);
+                                                                                  scratch.p);
     ++ctx->launches;
     vs_status st = vs_cuda(ctx, cudaGetLastError(), "norm column sums launch");
-    if (st == VS_OK) st = norm_join_partials(ctx, s.cols, strips, partial, wt.dtype, dweight, dbias);
-    VS_CUDA(ctx, cudaFreeAsync(partial, ctx->stream));
+    if (st == VS_OK) st = norm_join_partials(ctx, s.cols, strips, scratch.p, wt.dtype, dweight, dbias);
+    const vs_status end = norm_scratch_end(ctx, scratch);
+    if (st == VS_OK) st = end;
     VS_TRY(st);
   }
   norm_bwd_rows_kernel<T, kJoin><<<row_grid(s.rows), 256, 0, ctx->stream>>>(s, mdy, mdz, mz, wt, mean, rstd, d, (T*)dx,
@@ -277,9 +307,31 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, c
 
 vs_status norm_join_partials(vs_ctx* ctx, uint32_t cols, uint32_t strips, const float* partial, int32_t dtype,
                              void* dweight, void* dbias) {
-  norm_join_kernel<<<(cols + 31) / 32, dim3(32, 32), 0, ctx->stream>>>(cols, strips, partial, dtype, dweight, dbias);
+  norm_join_kernel<<<dim3((cols + 31) / 32, 2), 1024, 0, ctx->stream>>>(cols, strips, partial, dtype, dweight, dbias);
   ++ctx->launches;
   return vs_cuda(ctx, cudaGetLastError(), "norm weight gradient launch");
+}
+
+// The ctx's buffer serves one call after another: a call on another stream than
+// the last one's first waits for that one.  A call being captured into a graph
+// gets memory of the graph's own, since the graph may run beside other calls.
+vs_status norm_scratch_begin(vs_ctx* ctx, size_t floats, NormScratch* out) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  VS_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
+  out->pooled = capture != cudaStreamCaptureStatusNone;
+  if (out->pooled) return vs_cuda(ctx, cudaMallocAsync((void**)&out->p, floats * 4, ctx->stream), "norm scratch");
+  unsigned long long id = 0;
+  VS_CUDA(ctx, cudaStreamGetId(ctx->stream, &id));
+  if (!ctx->norm_done) VS_CUDA(ctx, cudaEventCreateWithFlags(&ctx->norm_done, cudaEventDisableTiming));
+  else if (id != ctx->norm_stream) VS_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->norm_done, 0));
+  ctx->norm_stream = id;
+  VS_TRY(vs_ensure(ctx, ctx->norm_sums, floats * 4));
+  out->p = static_cast<float*>(ctx->norm_sums.ptr);
+  return VS_OK;
+}
+vs_status norm_scratch_end(vs_ctx* ctx, const NormScratch& scratch) {
+  if (scratch.pooled) return vs_cuda(ctx, cudaFreeAsync(scratch.p, ctx->stream), "norm scratch");
+  return vs_cuda(ctx, cudaEventRecord(ctx->norm_done, ctx->stream), "norm scratch");
 }
 
 extern "C" {

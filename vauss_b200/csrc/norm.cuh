@@ -166,36 +166,38 @@ template <typename T> VSD void pack(const T* t, float2 v, uint2& u) {
 }
 VSD float keep_if(float v, uint32_t mask) { return __uint_as_float(__float_as_uint(v) & mask); }
 
-// The values of a row that one thread holds: K runs of VEC.  Rows of whole
-// 16-byte vectors are dealt out vector by vector, so that a warp's accesses are
-// contiguous; where K is even the runs' order turns with the row's place in the
-// warp, which keeps the rows' like runs off each other's shared-memory banks; a run beyond the row reads the row's first one.  Other rows are dealt
-// out in blocks of K runs, K odd, so that a warp's narrow accesses fall into
-// different banks and every offset is a constant; there a run beyond the row
-// reads what lies behind it (the next row, or the slot's padding).  Where a row
-// does not fill a warp's lanes such values are cleared before they are used.
+// The values of a row that one thread holds: K runs of VEC.  `kSpread` deals
+// them out run by run, so that a warp's accesses are contiguous; where K is even
+// the runs' order turns with the row's place in the warp, which keeps the rows'
+// like runs off each other's shared-memory banks; a run beyond the row reads the
+// row's first one.  Otherwise a thread holds a block of K runs, K odd, so that a
+// warp's narrow accesses to shared memory fall into different banks and every
+// offset is a constant; there a run beyond the row reads what lies behind it (the
+// next row, or the slot's padding).  Where a row does not fill a warp's lanes such
+// values are cleared before they are used.
 constexpr uint32_t NORM_PADDING = 128;  // bytes behind the last slot that such reads may reach
-template <typename T, int VEC, int K> struct Part {
+template <typename T, int VEC, int K, bool kSpread = VEC * sizeof(T) == 16> struct Part {
   static constexpr int E = VEC * K;
+  static constexpr int RUNS = K;
   static constexpr int PAIRS = (E + 1) / 2;
-  static constexpr bool kDirect = VEC * sizeof(T) == 16;
+  static constexpr bool kVector = VEC * sizeof(T) == 16;
   using R = typename Raw<T, VEC>::type;
   uint32_t at, lanes, sub;
   bool full;                      // the same for a warp
-  uint32_t off[kDirect ? K : 1];  // where the runs are read
-  uint32_t have;                  // the runs that are the row's, as bits (vectors) or their number (blocks)
-  static constexpr bool kMasks = K <= 15;
+  uint32_t off[kSpread ? K : 1];  // where the runs are read
+  uint32_t have;                  // the runs that are the row's, as bits (spread) or their number (blocks)
+  static constexpr bool kMasks = K <= 16;
   uint32_t masks[kMasks ? K : 1];  // all ones for the row's runs, where registers allow
 
   VSD Part(uint32_t at_, uint32_t lanes_, uint32_t sub_, uint32_t cols) : at(at_), lanes(lanes_), sub(sub_), have(0) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) have += col(k) < cols ? (kDirect ? 1u << k : 1u) : 0u;
-    full = __all_sync(0xffffffffu, have == (kDirect ? (1u << K) - 1 : (uint32_t)K));
+    for (int k = 0; k < K; ++k) have += col(k) < cols ? (kSpread ? 1u << k : 1u) : 0u;
+    full = __all_sync(0xffffffffu, have == (kSpread ? (1u << K) - 1 : (uint32_t)K));
     if constexpr (kMasks) {
 #pragma unroll
       for (int k = 0; k < K; ++k) masks[k] = has(k) ? 0xffffffffu : 0u;
     }
-    if constexpr (kDirect) {
+    if constexpr (kSpread) {
 #pragma unroll
       for (int k = 0; k < K; ++k) off[k] = has(k) ? col(k) : 0;
     } else {
@@ -205,20 +207,22 @@ template <typename T, int VEC, int K> struct Part {
     }
   }
   VSD uint32_t col(int k) const {
-    if (kDirect) return (at + lanes * (K % 2 ? k : (k + sub) % K)) * VEC;
+    if (kSpread) return (at + lanes * (K % 2 ? k : (k + sub) % K)) * VEC;
     return (at * K + k) * VEC;
   }
-  VSD bool has(int k) const { return kDirect ? have >> k & 1u : k < (int)have; }
+  VSD bool has(int k) const { return kSpread ? have >> k & 1u : k < (int)have; }
   VSD uint32_t mask(int k) const {
     if constexpr (kMasks) return masks[k];
     else return has(k) ? 0xffffffffu : 0u;
   }
+  // where run k is read, from the row's start
+  VSD uint32_t from(int k) const { return kSpread ? off[kSpread ? k : 0] : off[0] + k * VEC; }
   VSD void load(const T* row, R* t) const {
-    if constexpr (kDirect) {
+    if constexpr (kVector) {
       constexpr int W = 16 / sizeof(R);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const uint4 q = *reinterpret_cast<const uint4*>(row + off[k]);
+        const uint4 q = *reinterpret_cast<const uint4*>(row + from(k));
         if constexpr (W == 4) {
           t[k * W] = q.x; t[k * W + 1] = q.y; t[k * W + 2] = q.z; t[k * W + 3] = q.w;
         } else {
@@ -228,40 +232,56 @@ template <typename T, int VEC, int K> struct Part {
       }
     } else if constexpr (VEC == 2 && sizeof(T) == 2) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) t[k] = reinterpret_cast<const uint32_t*>(row + off[0])[k];
+      for (int k = 0; k < K; ++k) t[k] = *reinterpret_cast<const uint32_t*>(row + from(k));
     } else {
 #pragma unroll
-      for (int k = 0; k < E; ++k) {
-        if constexpr (sizeof(T) == 2) (&t[k / 2].x)[k % 2] = reinterpret_cast<const uint16_t*>(row + off[0])[k];
-        else (&t[k / 2].x)[k % 2] = reinterpret_cast<const float*>(row + off[0])[k];
+      for (int k = 0; k < K; ++k) {
+        if constexpr (sizeof(T) == 2) (&t[k / 2].x)[k % 2] = *reinterpret_cast<const uint16_t*>(row + from(k));
+        else (&t[k / 2].x)[k % 2] = *reinterpret_cast<const float*>(row + from(k));
       }
       if constexpr (E % 2 == 1) t[E / 2].y = 0;
     }
   }
   VSD void store(T* row, const R* t) const {
-    if constexpr (kDirect) {
-      constexpr int W = 16 / sizeof(R);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!has(k)) continue;
+    for (int k = 0; k < K; ++k) {
+      if (!has(k)) continue;
+      if constexpr (kVector) {
+        constexpr int W = 16 / sizeof(R);
         uint4 q;
         if constexpr (W == 4) q = make_uint4(t[k * W], t[k * W + 1], t[k * W + 2], t[k * W + 3]);
         else q = make_uint4(__float_as_uint(t[k * W].x), __float_as_uint(t[k * W].y), __float_as_uint(t[k * W + 1].x),
                             __float_as_uint(t[k * W + 1].y));
-        *reinterpret_cast<uint4*>(row + off[k]) = q;
-      }
-    } else if constexpr (VEC == 2 && sizeof(T) == 2) {
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (has(k)) reinterpret_cast<uint32_t*>(row + off[0])[k] = t[k];
-    } else {
-#pragma unroll
-      for (int k = 0; k < E; ++k) {
-        if (!has(k)) continue;
-        if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t*>(row + off[0])[k] = (uint16_t)(&t[k / 2].x)[k % 2];
-        else reinterpret_cast<float*>(row + off[0])[k] = (&t[k / 2].x)[k % 2];
+        *reinterpret_cast<uint4*>(row + from(k)) = q;
+      } else if constexpr (VEC == 2 && sizeof(T) == 2) {
+        *reinterpret_cast<uint32_t*>(row + from(k)) = t[k];
+      } else if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint16_t*>(row + from(k)) = (uint16_t)(&t[k / 2].x)[k % 2];
+      } else {
+        *reinterpret_cast<float*>(row + from(k)) = (&t[k / 2].x)[k % 2];
       }
     }
+  }
+  // A [cols] vector of weights, `other` where there is none.
+  VSD void weights(const void* p, int32_t dtype, float other, float2* w) const {
+    if constexpr (VEC % 4 == 0) {
+      if (p && dtype == VS_F32 && ((uintptr_t)p & 15u) == 0) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+          for (int j = 0; j < VEC; j += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + from(k) + j);
+            w[(k * VEC + j) / 2] = make_float2(q.x, q.y);
+            w[(k * VEC + j) / 2 + 1] = make_float2(q.z, q.w);
+          }
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2 * PAIRS; ++e)
+      (&w[e / 2].x)[e % 2] =
+          e < E && p && has(e / VEC) ? load_as(p, dtype, col(e / VEC) + e % VEC) : other;
   }
   // Zero for the values that are not the row's.
   VSD void clear(R* t) const {
@@ -321,6 +341,28 @@ VSD uint32_t keep_bits(const Words& w, uint32_t limit) {
   return bits;
 }
 
+// Dropout of a thread's values, decided one run at a time.
+template <typename P> VSD void drop_runs(const P& part, float2* v, uint64_t i0, const Dropout& d) {
+  constexpr int VEC = P::E / P::RUNS;
+#pragma unroll
+  for (int i = 0; i < P::PAIRS; ++i) v[i] = mul2(v[i], both(d.scale));
+  float* f = reinterpret_cast<float*>(v);
+#pragma unroll
+  for (int k = 0; k < P::RUNS; ++k) {
+    const uint64_t e = i0 + part.from(k);
+    if constexpr (VEC == 1) {
+      f[k] = keep_at(d, e) ? f[k] : 0.0f;
+    } else {
+      const Words words = philox(d, e >> 3);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const bool kept = VEC == 8 ? keeps(words, j, d.limit) : e & 4u ? keeps(words, j + 4, d.limit) : keeps(words, j, d.limit);
+        f[k * VEC + j] = kept ? f[k * VEC + j] : 0.0f;
+      }
+    }
+  }
+}
+
 // Dropout of a thread's values: v holds pairs, i0 is the row's first index.
 // Runs of eight are groups of the generator; for others the decisions have been
 // left in `bits`, the row's first at bit `at`.
@@ -338,7 +380,7 @@ VSD void drop_part(const Part<T, VEC, K>& part, float2* v, uint64_t i0, const Dr
 #pragma unroll
       for (int j = 0; j < VEC; ++j) f[k * VEC + j] = keeps(words, j, d.limit) ? f[k * VEC + j] : 0.0f;
     }
-  } else if constexpr (part.kDirect) {
+  } else if constexpr (part.kVector) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const uint32_t e = at + part.off[k];
@@ -408,6 +450,7 @@ VSD float warp_sum2(float a, float b) {
 struct NormFwd {
   vs::NormShape s;
   const void *x, *residual;
+  uint64_t x_stride, residual_stride;
   vs::Weights w;
   float eps;
   vs::Dropout d;
@@ -417,6 +460,7 @@ struct NormFwd {
 struct NormBwd {
   vs::NormShape s;
   const void *dy, *dz, *z;
+  uint64_t dy_stride, dz_stride, z_stride;
   vs::Weights w;
   const float *mean, *rstd;
   vs::Dropout d;
@@ -446,6 +490,17 @@ inline int norm_runs(uint32_t chunks, int most) {
 // *taken tells whether the shape is one of theirs.
 vs_status norm_stream_forward(vs_ctx* ctx, int32_t dtype, bool join, const NormFwd& a, bool* taken);
 vs_status norm_stream_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBwd& a, bool* taken);
+// The direct kernels take rows of any stride and alignment, up to a width.
+vs_status norm_direct_forward(vs_ctx* ctx, int32_t dtype, bool join, const NormFwd& a, bool* taken);
+vs_status norm_direct_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBwd& a, bool* taken);
+// `floats` floats of scratch for one call, on the ctx stream; end it after the
+// call's last launch.
+struct NormScratch {
+  float* p = nullptr;
+  bool pooled = false;
+};
+vs_status norm_scratch_begin(vs_ctx* ctx, size_t floats, NormScratch* out);
+vs_status norm_scratch_end(vs_ctx* ctx, const NormScratch& scratch);
 // dw and db from `strips` partial sums [strips][2][cols]
 vs_status norm_join_partials(vs_ctx* ctx, uint32_t cols, uint32_t strips, const float* partial, int32_t dtype,
                              void* dweight, void* dbias);

@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
   using P = Part<T, VEC, K>;
   using R = typename P::R;
   constexpr int PAIRS = P::PAIRS;
-  constexpr bool kDirect = P::kDirect;
+  constexpr bool kDirect = P::kVector;
   constexpr bool kBits = kJoin && VEC != 8;
   constexpr uint32_t WORKERS = kCta ? 1 : NORM_WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -96,16 +96,12 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
   }
   // the weights: a lane's in registers, a CTA's threads' in shared memory, each
   // thread's own at places of its own
-  float2 w[kCta ? 1 : PAIRS], dw[PAIRS], db[PAIRS];
+  float2 w[PAIRS], dw[PAIRS], db[PAIRS];
   float2* ws = reinterpret_cast<float2*>(ring + a.stages * stage + a.bits) + id;
+  part.weights(a.w.weight, a.w.dtype, 1.0f, w);
 #pragma unroll
   for (int i = 0; i < PAIRS; ++i) {
-    float2 v = both(1.0f);
-#pragma unroll
-    for (int e = 2 * i; e < 2 * i + 2 && e < P::E; ++e)
-      if (part.has(e / VEC) && a.w.weight) (&v.x)[e % 2] = load_as(a.w.weight, a.w.dtype, part.col(e / VEC) + e % VEC);
-    if constexpr (kCta) ws[i * members] = v;
-    else w[i] = v;
+    if (kCta) ws[i * members] = w[i];
     dw[i] = db[i] = both(0.0f);
   }
   const float n = (float)a.cols, inv = 1.0f / n;
@@ -179,7 +175,7 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
       }
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        g[i] = mul2(g[i], kCta ? ws[i * members] : w[kCta ? 0 : i]);
+        g[i] = mul2(g[i], kCta ? ws[i * members] : w[i]);
         s1 = add2(s1, g[i]);
         s2 = fma2(g[i], h[i], s2);
       }
@@ -333,7 +329,7 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   // Slots and CTAs as in the forward, the CTAs as for the joined kernel's three
   // inputs; the rings' memory also takes the warps' column sums, and a CTA's
   // threads keep their weights behind theirs.
-  constexpr uint32_t least = Part<T, VEC, K>::kDirect ? 1 : 2;
+  constexpr uint32_t least = Part<T, VEC, K>::kVector ? 1 : 2;
   const uint32_t sums = kCta ? 0 : WORKERS * 2 * a.cols * 4;
   const uint32_t ws = kCta ? threads * Part<T, VEC, K>::PAIRS * 8 : 0;
   auto bytes = [&](uint32_t inputs, uint32_t stages) {
@@ -343,7 +339,7 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   auto room = [&] { return NORM_MAX_SMEM / per_sm - 1024; };
   while (per_sm > 1 && bytes(3, 2) > room()) --per_sm;
   if (bytes(3, least) > room()) return VS_OK;
-  a.stages = Part<T, VEC, K>::kDirect ? 2 : 3;
+  a.stages = Part<T, VEC, K>::kVector ? 2 : 3;
   while (a.stages > least && bytes(a.inputs, a.stages) > room()) --a.stages;
   *taken = true;
   a.dy = f.dy; a.z = f.z; a.dz = f.dz; a.w = f.w; a.mean = f.mean; a.rstd = f.rstd;
@@ -353,14 +349,16 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   const uint64_t all = (uint64_t)per_sm * B200_SMS;
   const uint32_t grid = (uint32_t)(all < most ? all : most);
   const bool want = f.dweight || f.dbias;
-  // from the stream-ordered pool: calls of one ctx on several streams do not share it
-  if (want) VS_CUDA(ctx, cudaMallocAsync((void**)&a.partial, (size_t)grid * 2 * a.cols * 4, ctx->stream));
+  NormScratch scratch;
+  if (want) VS_TRY(norm_scratch_begin(ctx, (size_t)grid * 2 * a.cols, &scratch));
+  a.partial = scratch.p;
   kernel<<<grid, threads, bytes(a.inputs, a.stages), ctx->stream>>>(a, f.d);
   ++ctx->launches;
   vs_status st = vs_cuda(ctx, cudaGetLastError(), "norm backward launch");
   if (want) {
     if (st == VS_OK) st = norm_join_partials(ctx, a.cols, grid, a.partial, f.wdtype, f.dweight, f.dbias);
-    VS_CUDA(ctx, cudaFreeAsync(a.partial, ctx->stream));
+    const vs_status end = norm_scratch_end(ctx, scratch);
+    if (st == VS_OK) st = end;
   }
   return st;
 }

@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
   using P = Part<T, VEC, K>;
   using R = typename P::R;
   constexpr int PAIRS = P::PAIRS;
-  constexpr bool kDirect = P::kDirect;
+  constexpr bool kDirect = P::kVector;
   constexpr bool kBits = kJoin && VEC != 8;
   constexpr uint32_t NIN = kJoin ? 2 : 1, WORKERS = kCta ? 1 : NORM_WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -93,13 +93,8 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
     for (uint32_t k = 0; k < a.stages; ++k) refill(k);
   }
   float2 w[PAIRS], b[PAIRS];
-#pragma unroll
-  for (int e = 0; e < 2 * PAIRS; ++e) {
-    const uint32_t c = part.col(e / VEC) + e % VEC;
-    const bool has = e < P::E && part.has(e / VEC);
-    (&w[e / 2].x)[e % 2] = has && a.w.weight ? load_as(a.w.weight, a.w.dtype, c) : 1.0f;
-    (&b[e / 2].x)[e % 2] = has && a.w.bias ? load_as(a.w.bias, a.w.dtype, c) : 0.0f;
-  }
+  part.weights(a.w.weight, a.w.dtype, 1.0f, w);
+  part.weights(a.w.bias, a.w.dtype, 0.0f, b);
   const float n = (float)a.cols, inv = 1.0f / n;
   if (kCta)
     for (uint32_t k = id; k < 2 * NORM_MAX_WARPS; k += members) (&red[0][0])[k] = 0.0f;
@@ -250,11 +245,11 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   // 4096 bf16 13 %, see above), and a third for slots that are written back; fewer
   // CTAs where the SM's shared memory does not hold theirs.  A slot that is
   // written back needs at least another beside it.
-  constexpr uint32_t least = Part<T, VEC, K>::kDirect ? 1 : 2;
+  constexpr uint32_t least = Part<T, VEC, K>::kVector ? 1 : 2;
   auto bytes = [&](uint32_t stages) { return WORKERS * (stages * NIN * a.slot + a.bits) + NORM_PADDING; };
   auto room = [&] { return NORM_MAX_SMEM / per_sm - 1024; };
   while (per_sm > 1 && bytes(2) > room()) --per_sm;
-  a.stages = Part<T, VEC, K>::kDirect ? 2 : 3;
+  a.stages = Part<T, VEC, K>::kVector ? 2 : 3;
   while (a.stages > least && bytes(a.stages) > room()) --a.stages;
   if (bytes(a.stages) > room()) return VS_OK;
   *taken = true;

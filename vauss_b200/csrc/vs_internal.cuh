@@ -27,6 +27,9 @@ struct vs_ctx {
   DevBuf sort_keys, sort_vals, sort_hist, scan_sums, misc;
   DevBuf io_stage;  // checkpoint I/O chunks (two halves)
   DevBuf vjp_rows;  // per-visible-splat VJP rows of the single-view Q8 step
+  DevBuf norm_sums;  // layer norm's column sums per CTA
+  cudaEvent_t norm_done = nullptr;  // the last call that used them,
+  unsigned long long norm_stream = 0;  // and its stream's id
 };
 
 struct vs_frame {

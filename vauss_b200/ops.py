@@ -17,6 +17,7 @@ from . import _native as N
 from .camera import Camera
 
 _contexts: dict[int, "Context"] = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 _U64 = (1 << 64) - 1
 
 
@@ -39,8 +40,8 @@ class Context:
         self.h = h
 
     def bind(self) -> "Context":
-        s = torch.cuda.current_stream(self.device).cuda_stream
-        N.check(self.h, self.lib.vs_ctx_set_stream(self.h, ctypes.c_void_p(s)))
+        s = _raw_stream(self.device)  # the current stream's handle, without a Stream object around it
+        N.check(self.h, self.lib.vs_ctx_set_stream(self.h, s))
         return self
 
     def check(self, status: int):
@@ -400,59 +401,86 @@ def noise_means(transforms, opacities, visible, scale: float, limit: float, seed
 # Rows are the last dimension: [..., cols] tensors of one element type (f32,
 # f16 or bf16).  Inputs are contiguous, or 2-D with unit column stride (columns
 # of a wider row buffer); outputs are contiguous and may be passed in (`out`,
-# what an earlier call of the same shape returned).
+# what an earlier call of the same shape returned).  The calls take a few
+# microseconds on the host, so their checks are written out flat.
 
 _DTYPES = {torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16, torch.bfloat16: N.DTYPE_BF16}
+_F32 = torch.float32
 
 
-def _row_input(t: torch.Tensor, like: torch.Tensor):
-    """(address, row stride) of a row operator's input; a stride of 0 means contiguous rows."""
-    assert t.is_cuda and t.device == like.device and t.dtype == like.dtype and t.shape == like.shape, \
-        f"row inputs share device, type and shape: {t.dtype} {tuple(t.shape)} beside {like.dtype} {tuple(like.shape)}"
-    if t.is_contiguous():
-        return t.data_ptr(), 0
-    assert t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1], \
-        f"row inputs are contiguous or 2-D with unit column stride: strides {t.stride()}"
-    return t.data_ptr(), t.stride(0)
+def _row_context(device: int) -> Context:
+    ctx = _contexts.get(device)
+    return context(device) if ctx is None else ctx.bind()
 
 
 def _row_shape(t: torch.Tensor):
-    assert t.dim() >= 1 and t.dtype in _DTYPES, f"rows are f32, f16 or bf16 tensors [..., cols]: {t.dtype} {tuple(t.shape)}"
-    cols = t.shape[-1]
-    assert cols > 0, "rows without columns"
-    return t.numel() // cols, cols, _DTYPES[t.dtype]
+    """(shape, rows, cols, vs_dtype, device index) of the tensor that a call's others go by."""
+    shape, device, dtype = t.shape, t.get_device(), _DTYPES.get(t.dtype)
+    assert device >= 0 and dtype is not None and len(shape) and shape[-1] > 0, \
+        f"rows are CUDA f32, f16 or bf16 tensors [..., cols]: {t.device} {t.dtype} {tuple(shape)}"
+    cols = shape[-1]
+    return shape, t.numel() // cols, cols, dtype, device
 
 
-def _row_output(t: torch.Tensor, shape, dtype, like: torch.Tensor) -> int:
-    assert t.device == like.device and t.shape == shape and t.dtype == dtype and t.is_contiguous(), \
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride of an input; 0 stands for contiguous rows."""
+    if t.is_contiguous():
+        return 0
+    assert t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1], \
+        f"row inputs are contiguous or 2-D with unit column stride: strides {t.stride()}"
+    return t.stride(0)
+
+
+def _like(t: torch.Tensor, shape, dtype, device: int) -> bool:
+    return t.shape == shape and t.dtype is dtype and t.get_device() == device
+
+
+def _weight(w: torch.Tensor | None, wdtype, cols: int, device: int):
+    if w is None:
+        return None
+    assert w.dtype is wdtype and w.numel() == cols and w.dim() == 1 and w.get_device() == device and w.is_contiguous(), \
+        f"weights are contiguous [cols], of one type (f32 or the rows'): {w.dtype} {tuple(w.shape)}"
+    return w.data_ptr()
+
+
+def _weight_dtype(weight, bias, x):
+    w = weight if weight is not None else bias
+    if w is None:
+        return _F32
+    assert w.dtype is _F32 or w.dtype is x.dtype, f"weights are f32 or of the rows' type: {w.dtype}"
+    return w.dtype
+
+
+def _stat(t: torch.Tensor, rows: int, device: int) -> int:
+    assert t.dtype is _F32 and t.numel() == rows and t.get_device() == device and t.is_contiguous(), \
+        f"row statistics are contiguous f32 [rows]: {t.dtype} {tuple(t.shape)}"
+    return t.data_ptr()
+
+
+def _output(t: torch.Tensor, shape, dtype, device: int) -> int:
+    assert _like(t, shape, dtype, device) and t.is_contiguous(), \
         f"`out` holds contiguous {dtype} {tuple(shape)}: got {t.dtype} {tuple(t.shape)}"
     return t.data_ptr()
 
 
-def _weight(w: torch.Tensor | None, x: torch.Tensor):
-    if w is None:
-        return None
-    assert w.shape == x.shape[-1:] and w.device == x.device and w.is_contiguous() and w.dtype in (torch.float32, x.dtype), \
-        f"layer-norm weights are contiguous [cols] in f32 or the rows' type: {w.dtype} {tuple(w.shape)}"
-    return w.data_ptr()
-
-
-def _weight_dtype(weight, bias, x) -> torch.dtype:
-    assert weight is None or bias is None or weight.dtype == bias.dtype, "weight and bias are of one type"
-    w = weight if weight is not None else bias
-    return torch.float32 if w is None else w.dtype
+def _refuse_input(name, t, x):
+    raise AssertionError(f"{name} shares the rows' device, type and shape: {t.device} {t.dtype} {tuple(t.shape)} "
+                         f"beside {x.device} {x.dtype} {tuple(x.shape)}")
 
 
 def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
     """Zeroes each value with probability ``p`` and scales the others so that the expectation stays.  The mask is
     a function of (seed, offset, the value's index in x) and is never stored (vs_dropout in the header defines it);
     give every call of a step its own ``offset``.  Any contiguous shape; ``out`` may be ``x``."""
-    assert x.is_cuda and x.is_contiguous() and x.dtype in _DTYPES, "dropout takes contiguous CUDA f32, f16 or bf16"
+    dtype, device = _DTYPES.get(x.dtype), x.get_device()
+    assert device >= 0 and dtype is not None and x.is_contiguous(), "dropout takes contiguous CUDA f32, f16 or bf16"
     if out is None:
         out = torch.empty_like(x)
-    y = _row_output(out, x.shape, x.dtype, x)
-    ctx = context(x.device)
-    ctx.check(ctx.lib.vs_dropout(ctx.h, x.numel(), _DTYPES[x.dtype], x.data_ptr(), p, seed & _U64, offset & _U64, y))
+    y = _output(out, x.shape, x.dtype, device)
+    ctx = _row_context(device)
+    st = ctx.lib.vs_dropout(ctx.h, x.numel(), dtype, x.data_ptr(), p, seed & _U64, offset & _U64, y)
+    if st:
+        ctx.check(st)
     return out
 
 
@@ -471,18 +499,18 @@ class LayerNormOutput:
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5, out: LayerNormOutput | None = None) -> LayerNormOutput:
     """y = (x - mean) rstd weight + bias over each row, with the row statistics its backward reads."""
-    rows, cols, dtype = _row_shape(x)
+    shape, rows, cols, dtype, device = _row_shape(x)
     wdtype = _weight_dtype(weight, bias, x)
     if out is None:
-        out = LayerNormOutput(torch.empty(x.shape, dtype=x.dtype, device=x.device),
-                              torch.empty(rows, dtype=torch.float32, device=x.device),
-                              torch.empty(rows, dtype=torch.float32, device=x.device))
-    px, sx = _row_input(x, x)
-    y = _row_output(out.y, x.shape, x.dtype, x)
-    mean, rstd = (_row_output(t, (rows,), torch.float32, x) for t in (out.mean, out.rstd))
-    ctx = context(x.device)
-    ctx.check(ctx.lib.vs_layer_norm(ctx.h, rows, cols, dtype, _DTYPES[wdtype], px, sx, _weight(weight, x),
-                                    _weight(bias, x), eps, y, mean, rstd))
+        out = LayerNormOutput(torch.empty(shape, dtype=x.dtype, device=x.device),
+                              *torch.empty(2, rows, dtype=_F32, device=x.device).unbind())
+    args = (rows, cols, dtype, _DTYPES[wdtype], x.data_ptr(), _row_stride(x), _weight(weight, wdtype, cols, device),
+            _weight(bias, wdtype, cols, device), eps, _output(out.y, shape, x.dtype, device),
+            _stat(out.mean, rows, device), _stat(out.rstd, rows, device))
+    ctx = _row_context(device)
+    st = ctx.lib.vs_layer_norm(ctx.h, *args)
+    if st:
+        ctx.check(st)
     return out
 
 
@@ -491,12 +519,6 @@ class LayerNormGrads:
     dx: torch.Tensor  # [..., cols]
     dweight: torch.Tensor | None  # [cols], of the weight's type
     dbias: torch.Tensor | None
-
-
-def _stat(t: torch.Tensor, rows: int, x: torch.Tensor) -> int:
-    assert t.device == x.device and t.dtype == torch.float32 and t.numel() == rows and t.is_contiguous(), \
-        f"row statistics are contiguous f32 [rows]: {t.dtype} {tuple(t.shape)}"
-    return t.data_ptr()
 
 
 def _weight_grads(cols: int, wdtype: torch.dtype, weight, with_bias, x):
@@ -510,18 +532,21 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | Non
                    out: LayerNormGrads | None = None) -> LayerNormGrads:
     """Gradients of ``layer_norm``'s input, weight and bias; the sums over the rows are taken in a fixed order.
     ``with_bias`` asks for dbias (by default where there is a weight); ``out.dx`` may be ``dy``."""
-    rows, cols, dtype = _row_shape(x)
+    shape, rows, cols, dtype, device = _row_shape(x)
+    if not _like(dy, shape, x.dtype, device):
+        _refuse_input("dy", dy, x)
     wdtype = _weight_dtype(weight, None, x)
     if out is None:
-        out = LayerNormGrads(torch.empty(x.shape, dtype=x.dtype, device=x.device),
+        out = LayerNormGrads(torch.empty(shape, dtype=x.dtype, device=x.device),
                              *_weight_grads(cols, wdtype, weight, with_bias, x))
-    (pdy, sdy), (px, sx) = _row_input(dy, x), _row_input(x, x)
-    dx = _row_output(out.dx, x.shape, x.dtype, x)
-    dw, db = (None if t is None else _row_output(t, (cols,), wdtype, x) for t in (out.dweight, out.dbias))
-    ctx = context(x.device)
-    ctx.check(ctx.lib.vs_layer_norm_backward(ctx.h, rows, cols, dtype, _DTYPES[wdtype], pdy, sdy, px, sx,
-                                             _weight(weight, x), _stat(mean, rows, x), _stat(rstd, rows, x), dx, dw,
-                                             db))
+    args = (rows, cols, dtype, _DTYPES[wdtype], dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x),
+            _weight(weight, wdtype, cols, device), _stat(mean, rows, device), _stat(rstd, rows, device),
+            _output(out.dx, shape, x.dtype, device), _weight(out.dweight, wdtype, cols, device),
+            _weight(out.dbias, wdtype, cols, device))
+    ctx = _row_context(device)
+    st = ctx.lib.vs_layer_norm_backward(ctx.h, *args)
+    if st:
+        ctx.check(st)
     return out
 
 
@@ -538,20 +563,22 @@ def dropout_add_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
                      out: DropoutAddNormOutput | None = None) -> DropoutAddNormOutput:
     """z = residual + dropout(x) and y = layer_norm(z) in one pass (what stands between two residual blocks);
     the mask is that of ``dropout`` on a contiguous x.  ``out.z`` may be ``residual``, ``out.y`` may be ``x``."""
-    rows, cols, dtype = _row_shape(x)
+    shape, rows, cols, dtype, device = _row_shape(x)
+    if not _like(residual, shape, x.dtype, device):
+        _refuse_input("residual", residual, x)
     wdtype = _weight_dtype(weight, bias, x)
     if out is None:
-        out = DropoutAddNormOutput(torch.empty(x.shape, dtype=x.dtype, device=x.device),
-                                   torch.empty(x.shape, dtype=x.dtype, device=x.device),
-                                   torch.empty(rows, dtype=torch.float32, device=x.device),
-                                   torch.empty(rows, dtype=torch.float32, device=x.device))
-    (px, sx), (pr, sr) = _row_input(x, x), _row_input(residual, x)
-    y, z = (_row_output(t, x.shape, x.dtype, x) for t in (out.y, out.z))
-    mean, rstd = (_row_output(t, (rows,), torch.float32, x) for t in (out.mean, out.rstd))
-    ctx = context(x.device)
-    ctx.check(ctx.lib.vs_dropout_add_norm(ctx.h, rows, cols, dtype, _DTYPES[wdtype], px, sx, pr, sr,
-                                          _weight(weight, x), _weight(bias, x), p, seed & _U64, offset & _U64, eps, y,
-                                          z, mean, rstd))
+        out = DropoutAddNormOutput(torch.empty(shape, dtype=x.dtype, device=x.device),
+                                   torch.empty(shape, dtype=x.dtype, device=x.device),
+                                   *torch.empty(2, rows, dtype=_F32, device=x.device).unbind())
+    args = (rows, cols, dtype, _DTYPES[wdtype], x.data_ptr(), _row_stride(x), residual.data_ptr(),
+            _row_stride(residual), _weight(weight, wdtype, cols, device), _weight(bias, wdtype, cols, device), p,
+            seed & _U64, offset & _U64, eps, _output(out.y, shape, x.dtype, device),
+            _output(out.z, shape, x.dtype, device), _stat(out.mean, rows, device), _stat(out.rstd, rows, device))
+    ctx = _row_context(device)
+    st = ctx.lib.vs_dropout_add_norm(ctx.h, *args)
+    if st:
+        ctx.check(st)
     return out
 
 
@@ -569,21 +596,25 @@ def dropout_add_norm_bwd(dy: torch.Tensor, dz: torch.Tensor | None, z: torch.Ten
                          out: DropoutAddNormGrads | None = None) -> DropoutAddNormGrads:
     """Gradients of ``dropout_add_norm``: dresidual = dz + the norm's gradient, dx = dropout_bwd of it.  ``dz`` is
     what reaches z past the norm (None: nothing does); ``out.dx`` may be ``dy``, ``out.dresidual`` may be ``dz``."""
-    rows, cols, dtype = _row_shape(z)
+    shape, rows, cols, dtype, device = _row_shape(z)
+    if not _like(dy, shape, z.dtype, device):
+        _refuse_input("dy", dy, z)
+    if dz is not None and not _like(dz, shape, z.dtype, device):
+        _refuse_input("dz", dz, z)
     wdtype = _weight_dtype(weight, None, z)
     if out is None:
-        out = DropoutAddNormGrads(torch.empty(z.shape, dtype=z.dtype, device=z.device),
-                                  torch.empty(z.shape, dtype=z.dtype, device=z.device),
+        out = DropoutAddNormGrads(torch.empty(shape, dtype=z.dtype, device=z.device),
+                                  torch.empty(shape, dtype=z.dtype, device=z.device),
                                   *_weight_grads(cols, wdtype, weight, with_bias, z))
-    (pdy, sdy), (pz, sz) = _row_input(dy, z), _row_input(z, z)
-    pdz, sdz = (None, 0) if dz is None else _row_input(dz, z)
-    dx, dres = (_row_output(t, z.shape, z.dtype, z) for t in (out.dx, out.dresidual))
-    dw, db = (None if t is None else _row_output(t, (cols,), wdtype, z) for t in (out.dweight, out.dbias))
-    ctx = context(z.device)
-    ctx.check(ctx.lib.vs_dropout_add_norm_backward(ctx.h, rows, cols, dtype, _DTYPES[wdtype], pdy, sdy, pdz, sdz, pz,
-                                                   sz, _weight(weight, z), _stat(mean, rows, z),
-                                                   _stat(rstd, rows, z), p, seed & _U64, offset & _U64, dx, dres, dw,
-                                                   db))
+    args = (rows, cols, dtype, _DTYPES[wdtype], dy.data_ptr(), _row_stride(dy), None if dz is None else dz.data_ptr(),
+            0 if dz is None else _row_stride(dz), z.data_ptr(), _row_stride(z), _weight(weight, wdtype, cols, device),
+            _stat(mean, rows, device), _stat(rstd, rows, device), p, seed & _U64, offset & _U64,
+            _output(out.dx, shape, z.dtype, device), _output(out.dresidual, shape, z.dtype, device),
+            _weight(out.dweight, wdtype, cols, device), _weight(out.dbias, wdtype, cols, device))
+    ctx = _row_context(device)
+    st = ctx.lib.vs_dropout_add_norm_backward(ctx.h, *args)
+    if st:
+        ctx.check(st)
     return out
 
 
