@@ -128,27 +128,28 @@ __global__ void __launch_bounds__(256) norm_cols_kernel(Shape s, Mat<const T> dy
 }
 
 // dw and db from `strips` partial sums [strips][2][cols]: a CTA takes 32 columns
-// of one of the two, 128 groups of 8 threads take every 128th strip's 16-byte
-// pieces of them (8 loads of 16 bytes in flight for 1024 strips), and the groups'
-// sums are added in a fixed order.
-__global__ void __launch_bounds__(1024) norm_join_kernel(uint32_t cols, uint32_t strips, const float* partial,
+// of one of the two, GROUPS groups of 8 threads take every GROUPS-th strip's
+// 16-byte pieces of them, and the groups' sums are added in a fixed order.
+template <uint32_t GROUPS>
+__global__ void __launch_bounds__(GROUPS * 8) norm_join_kernel(uint32_t cols, uint32_t strips, const float* partial,
                                                          int32_t dtype, void* dweight, void* dbias) {
-  __shared__ float4 part[128][9];
+  __shared__ float4 part[GROUPS][9];
   const uint32_t piece = threadIdx.x & 7u, group = threadIdx.x >> 3;
   const uint32_t c = blockIdx.x * 32 + piece * 4;
   const float* from = partial + (uint64_t)blockIdx.y * cols + c;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the sums' kernel has ended and its writes are visible
   float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (cols % 4 == 0) {
     if (c < cols) {
 #pragma unroll 4
-      for (uint32_t k = group; k < strips; k += 128) {
+      for (uint32_t k = group; k < strips; k += GROUPS) {
         const float4 v = *reinterpret_cast<const float4*>(from + (uint64_t)k * 2 * cols);
         s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
       }
     }
   } else {
 #pragma unroll 2
-    for (uint32_t k = group; k < strips; k += 128) {
+    for (uint32_t k = group; k < strips; k += GROUPS) {
       const float* p = from + (uint64_t)k * 2 * cols;
       if (c < cols) s.x += p[0];
       if (c + 1 < cols) s.y += p[1];
@@ -158,14 +159,16 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(uint32_t cols, uint32_t
   }
   part[group][piece] = s;
   __syncthreads();
-  // 32 columns x 32 threads, four groups each
-  const uint32_t col = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  float v = 0.0f;
-#pragma unroll
-  for (uint32_t k = 0; k < 4; ++k) v += reinterpret_cast<const float*>(&part[lane + 32 * k][col >> 2])[col & 3u];
-  v = warp_sum(v);
+  // a warp per column
+  const uint32_t lane = threadIdx.x & 31u;
   void* out = blockIdx.y ? dbias : dweight;
-  if (lane == 0 && blockIdx.x * 32 + col < cols && out) store_as(out, dtype, blockIdx.x * 32 + col, v);
+  for (uint32_t col = threadIdx.x >> 5; col < 32; col += GROUPS / 4) {
+    float v = 0.0f;
+#pragma unroll
+    for (uint32_t k = lane; k < GROUPS; k += 32) v += reinterpret_cast<const float*>(&part[k][col >> 2])[col & 3u];
+    v = warp_sum(v);
+    if (lane == 0 && blockIdx.x * 32 + col < cols && out) store_as(out, dtype, blockIdx.x * 32 + col, v);
+  }
 }
 
 // What every entry point checks of its shape.
@@ -307,14 +310,27 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, c
 
 vs_status norm_join_partials(vs_ctx* ctx, uint32_t cols, uint32_t strips, const float* partial, int32_t dtype,
                              void* dweight, void* dbias) {
-  norm_join_kernel<<<dim3((cols + 31) / 32, 2), 1024, 0, ctx->stream>>>(cols, strips, partial, dtype, dweight, dbias);
+  // launched beside the kernel that writes the sums, which it waits for: its
+  // launch is over by then
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((cols + 31) / 32, 2);
+  const bool few = strips <= 128;
+  config.blockDim = dim3(few ? 256 : 1024);
+  config.stream = ctx->stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  VS_CUDA(ctx, cudaLaunchKernelEx(&config, few ? norm_join_kernel<32> : norm_join_kernel<128>, cols, strips, partial,
+                                  dtype, dweight, dbias));
   ++ctx->launches;
-  return vs_cuda(ctx, cudaGetLastError(), "norm weight gradient launch");
+  return VS_OK;
 }
 
-// The ctx's buffer serves one call after another: a call on another stream than
-// the last one's first waits for that one.  A call being captured into a graph
-// gets memory of the graph's own, since the graph may run beside other calls.
+// Calls on one stream follow one another, so each stream has one buffer.  A call
+// being captured into a graph gets memory of the graph's own, since the graph may
+// run beside other calls.
 vs_status norm_scratch_begin(vs_ctx* ctx, size_t floats, NormScratch* out) {
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   VS_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
@@ -322,16 +338,25 @@ vs_status norm_scratch_begin(vs_ctx* ctx, size_t floats, NormScratch* out) {
   if (out->pooled) return vs_cuda(ctx, cudaMallocAsync((void**)&out->p, floats * 4, ctx->stream), "norm scratch");
   unsigned long long id = 0;
   VS_CUDA(ctx, cudaStreamGetId(ctx->stream, &id));
-  if (!ctx->norm_done) VS_CUDA(ctx, cudaEventCreateWithFlags(&ctx->norm_done, cudaEventDisableTiming));
-  else if (id != ctx->norm_stream) VS_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->norm_done, 0));
-  ctx->norm_stream = id;
-  VS_TRY(vs_ensure(ctx, ctx->norm_sums, floats * 4));
-  out->p = static_cast<float*>(ctx->norm_sums.ptr);
+  const uint32_t seen = ctx->norm_streams < vs_ctx::NORM_STREAMS ? ctx->norm_streams : vs_ctx::NORM_STREAMS;
+  uint32_t k = 0;
+  while (k < seen && ctx->norm_stream[k] != id) ++k;
+  if (k == seen) {
+    k = ctx->norm_streams % vs_ctx::NORM_STREAMS;
+    DevBuf& b = ctx->norm_sums[k];
+    if (b.ptr) {  // another stream's: wait for whatever still uses it
+      VS_CUDA(ctx, cudaDeviceSynchronize());
+      vs_release(ctx, b);
+    }
+    ctx->norm_stream[k] = id;
+    ++ctx->norm_streams;
+  }
+  VS_TRY(vs_ensure(ctx, ctx->norm_sums[k], floats * 4));
+  out->p = static_cast<float*>(ctx->norm_sums[k].ptr);
   return VS_OK;
 }
 vs_status norm_scratch_end(vs_ctx* ctx, const NormScratch& scratch) {
-  if (scratch.pooled) return vs_cuda(ctx, cudaFreeAsync(scratch.p, ctx->stream), "norm scratch");
-  return vs_cuda(ctx, cudaEventRecord(ctx->norm_done, ctx->stream), "norm scratch");
+  return scratch.pooled ? vs_cuda(ctx, cudaFreeAsync(scratch.p, ctx->stream), "norm scratch") : VS_OK;
 }
 
 extern "C" {

@@ -318,6 +318,9 @@ template <typename T, int VEC, int K, bool kSpread = VEC * sizeof(T) == 16> stru
   }
 };
 
+// Lets the kernel that joins the column sums be launched; it waits by itself.
+VSD void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // The sum over groups of `lanes` (a power of two) neighbouring lanes.
 VSD float lanes_sum(float v, uint32_t lanes) {
 #pragma unroll

@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
     for (uint32_t k = id; k < 4 * NORM_MAX_WARPS; k += members) (&red[0][0][0])[k] = 0.0f;
   if (kCta) __syncthreads(); else __syncwarp();
 
+  launch_next();
   uint32_t slot = 0, parity = 0, half = 0;
   bool ok = true;
   uint64_t row0 = first * a.tile_rows;

@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
   float2 w[PAIRS], dw[PAIRS], db[PAIRS];
 #pragma unroll
   for (int i = 0; i < PAIRS; ++i) dw[i] = db[i] = both(0.0f);
+  launch_next();
   bool ready = false;
   uint32_t half = 0;
   if (kCta) {
