@@ -240,9 +240,10 @@ vs_status norm_forward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, co
   const bool stream = vector_rows(s, {mx.stride, kJoin ? mr.stride : mx.stride}, {x, residual, y, z});
   const bool small = is_small(s, sizeof(T) * (kJoin ? 4 : 2));
   bool taken = false;
-  if (stream && !small) VS_TRY(norm_stream_forward(ctx, dtype, kJoin, f, &taken));
+  if (stream && !small) VS_TRY(norm_tile_forward(ctx, dtype, kJoin, f, &taken));
+  if (stream && !small && !taken) VS_TRY(norm_row_forward(ctx, dtype, kJoin, f, &taken));
   if (!taken) VS_TRY(norm_direct_forward(ctx, dtype, kJoin, f, &taken));
-  if (!taken && stream && small) VS_TRY(norm_stream_forward(ctx, dtype, kJoin, f, &taken));
+  if (!taken && stream && small) VS_TRY(norm_row_forward(ctx, dtype, kJoin, f, &taken));
   if (taken) return VS_OK;
   norm_fwd_rows_kernel<T, kJoin><<<row_grid(s.rows), 256, 0, ctx->stream>>>(s, mx, mr, wt, eps, d, (T*)y, (T*)z, mean,
                                                                             rstd);
@@ -278,9 +279,10 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, c
   // by the plain kernel's traffic, so that the joined one's weight gradients are the same sums
   const bool small = is_small(s, sizeof(T) * 3);
   bool taken = false;
-  if (stream && !small) VS_TRY(norm_stream_backward(ctx, dtype, kJoin, f, &taken));
+  if (stream && !small) VS_TRY(norm_tile_backward(ctx, dtype, kJoin, f, &taken));
+  if (stream && !small && !taken) VS_TRY(norm_row_backward(ctx, dtype, kJoin, f, &taken));
   if (!taken) VS_TRY(norm_direct_backward(ctx, dtype, kJoin, f, &taken));
-  if (!taken && stream && small) VS_TRY(norm_stream_backward(ctx, dtype, kJoin, f, &taken));
+  if (!taken && stream && small) VS_TRY(norm_row_backward(ctx, dtype, kJoin, f, &taken));
   if (taken) return VS_OK;
   // the column sums read dy, which dx may overwrite, so they come first
   if (dweight || dbias) {

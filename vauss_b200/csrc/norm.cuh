@@ -435,8 +435,19 @@ constexpr uint32_t NORM_MAX_SMEM = 226 * 1024;
 // Threads of an SM that the CTA-per-row kernels' registers leave room for.  The
 // grids follow from this and the shape alone, never from an occupancy query, so
 // the order of the weight gradients' sums does too.
-constexpr uint32_t NORM_FWD_THREADS = 512;
-constexpr uint32_t NORM_BWD_THREADS = 384;
+#ifndef VAR_FK
+#define VAR_FK 4
+#endif
+#ifndef VAR_BK
+#define VAR_BK 4
+#endif
+#ifndef VAR_RF
+#define VAR_RF 512
+#endif
+#ifndef VAR_RB
+#define VAR_RB 384
+#endif
+constexpr uint32_t NORM_ROW_FWD = VAR_RF, NORM_ROW_BWD = VAR_RB;
 
 // The sums of a and b over a warp in one chain: lanes 0 to 15 get a's, the others b's.
 VSD float warp_sum2(float a, float b) {
@@ -489,10 +500,13 @@ inline int norm_runs(uint32_t chunks, int most) {
   return best;
 }
 
-// The streaming kernels take contiguous rows on 16-byte aligned buffers;
-// *taken tells whether the shape is one of theirs.
-vs_status norm_stream_forward(vs_ctx* ctx, int32_t dtype, bool join, const NormFwd& a, bool* taken);
-vs_status norm_stream_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBwd& a, bool* taken);
+// The streaming kernels take contiguous rows on 16-byte aligned buffers: tiles of
+// short rows per warp, or a CTA per long row; *taken tells whether the shape is
+// one of theirs.
+vs_status norm_row_forward(vs_ctx* ctx, int32_t dtype, bool join, const NormFwd& a, bool* taken);
+vs_status norm_row_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBwd& a, bool* taken);
+vs_status norm_tile_forward(vs_ctx* ctx, int32_t dtype, bool join, const NormFwd& a, bool* taken);
+vs_status norm_tile_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBwd& a, bool* taken);
 // The direct kernels take rows of any stride and alignment, up to a width.
 vs_status norm_direct_forward(vs_ctx* ctx, int32_t dtype, bool join, const NormFwd& a, bool* taken);
 vs_status norm_direct_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBwd& a, bool* taken);

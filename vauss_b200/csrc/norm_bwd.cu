@@ -1,9 +1,9 @@
 // Streaming backward layer norm, alone or joined with the residual sum and the
-// dropout, for contiguous rows; the workers and their rings are those of the
+// dropout, for contiguous rows; the warps and their rings are those of the
 // forward (norm_fwd.cu).
 //
-// A thread's columns are the same for every row, so the weight's and the bias's
-// gradients grow in registers over all rows of a worker; a CTA then leaves one
+// A lane's columns are the same for every row, so the weight's and the bias's
+// gradients grow in registers over all rows of a warp; a CTA then leaves one
 // partial sum per column and a second kernel adds the CTAs' in a fixed order.
 #include <atomic>
 
@@ -36,31 +36,25 @@ struct BwdArgs {
 
 // Whole-vector rows are written from registers, others through their slots, as
 // in the forward.
-template <typename T, int VEC, int K, bool kJoin, bool kCta>
-__global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCta ? 1 : warp_ctas<T, VEC, K>())
+template <typename T, int VEC, int K, bool kJoin>
+__global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
     norm_bwd_kernel(const BwdArgs a, const __grid_constant__ Dropout d) {
   using P = Part<T, VEC, K>;
   using R = typename P::R;
   constexpr int PAIRS = P::PAIRS;
   constexpr bool kDirect = P::kVector;
   constexpr bool kBits = kJoin && VEC != 8;
-  constexpr uint32_t WORKERS = kCta ? 1 : NORM_WARPS;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t bars[WORKERS][NORM_STAGES];
-  __shared__ __align__(16) float red[2][2][kCta ? NORM_MAX_WARPS : 4];
-  __shared__ uint32_t late[2];
-  const uint32_t worker = kCta ? 0 : threadIdx.x >> 5;
-  const uint32_t id = kCta ? threadIdx.x : threadIdx.x & 31u, members = kCta ? blockDim.x : 32;
-  const uint32_t warps = blockDim.x >> 5;
-  const uint32_t lanes = kCta ? members : 1u << a.log_lanes;
-  const uint32_t sub = kCta ? 0 : id >> a.log_lanes, per_pass = kCta ? 1 : 32u >> a.log_lanes;
-  const P part(kCta ? id : id & (lanes - 1), lanes, sub, a.cols);
+  __shared__ __align__(8) uint64_t bars[NORM_WARPS][NORM_STAGES];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t lanes = 1u << a.log_lanes, sub = lane >> a.log_lanes, per_pass = 32u >> a.log_lanes;
+  const P part(lane & (lanes - 1), lanes, sub, a.cols);
   const uint32_t stage = a.inputs * a.slot + 2 * a.stat_slot;  // dy, z, (dz), mean, rstd
-  unsigned char* ring = smem + (size_t)worker * (a.stages * stage + a.bits);
-  unsigned char* bits = ring + a.stages * stage;  // two rows' for a CTA
-  uint64_t* full = bars[worker];
+  unsigned char* ring = smem + (size_t)warp * (a.stages * stage + a.bits);
+  uint32_t* bits = reinterpret_cast<uint32_t*>(ring + a.stages * stage);
+  uint64_t* full = bars[warp];
 
-  const uint64_t first = (uint64_t)blockIdx.x * WORKERS + worker, step = (uint64_t)gridDim.x * WORKERS;
+  const uint64_t first = (uint64_t)blockIdx.x * NORM_WARPS + warp, step = (uint64_t)gridDim.x * NORM_WARPS;
   const uint32_t tile_bytes = a.tile_rows * a.cols * (uint32_t)sizeof(T);
   const uint64_t total = a.rows * a.cols * sizeof(T), step_bytes = step * tile_bytes;
   const uint64_t step_rows = step * a.tile_rows;
@@ -88,67 +82,53 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
     load_at += step_bytes;
     load_row += step_rows;
   };
-  if (id == 0) {
-    if (kCta) late[0] = late[1] = 0;
+  if (lane == 0) {
     for (uint32_t k = 0; k < a.stages; ++k) mbar_init(&full[k], 1);
     mbar_init_fence();
     for (uint32_t k = 0; k < a.stages; ++k) refill(k);
   }
-  // the weights: a lane's in registers, a CTA's threads' in shared memory, each
-  // thread's own at places of its own
   float2 w[PAIRS], dw[PAIRS], db[PAIRS];
-  float2* ws = reinterpret_cast<float2*>(ring + a.stages * stage + a.bits) + id;
   part.weights(a.w.weight, a.w.dtype, 1.0f, w);
 #pragma unroll
-  for (int i = 0; i < PAIRS; ++i) {
-    if (kCta) ws[i * members] = w[i];
-    dw[i] = db[i] = both(0.0f);
-  }
+  for (int i = 0; i < PAIRS; ++i) dw[i] = db[i] = both(0.0f);
   const float n = (float)a.cols, inv = 1.0f / n;
-  if (kCta)
-    for (uint32_t k = id; k < 4 * NORM_MAX_WARPS; k += members) (&red[0][0][0])[k] = 0.0f;
-  if (kCta) __syncthreads(); else __syncwarp();
+  __syncwarp();
 
   launch_next();
-  uint32_t slot = 0, parity = 0, half = 0;
+  uint32_t slot = 0, parity = 0;
   bool ok = true;
   uint64_t row0 = first * a.tile_rows;
   for (; row0 < a.rows; row0 += step_rows, begin += step_bytes) {
-    ok = mbar_wait(&full[slot], parity);
-    if (kCta) {
-      if (!ok) late[half] = 1;
-    } else if (!(ok = __all_sync(0xffffffffu, ok))) {
-      break;
-    }
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], parity));
+    if (!ok) break;
     unsigned char* gbuf = ring + slot * stage;
     unsigned char* zbuf = gbuf + a.slot;
     unsigned char* rbuf = zbuf + a.slot;  // dz, where there is one
     unsigned char* mbuf = gbuf + a.inputs * a.slot;
-    uint32_t* kept = reinterpret_cast<uint32_t*>(bits + (kCta ? half * (a.bits / 2) : 0));
-    const uint32_t rows = kCta ? 1 : a.rows - row0 < a.tile_rows ? (uint32_t)(a.rows - row0) : a.tile_rows;
+    const uint32_t rows = a.rows - row0 < a.tile_rows ? (uint32_t)(a.rows - row0) : a.tile_rows;
     const uint64_t i0 = begin / sizeof(T);
     const uint32_t shift = kDirect ? 0 : (uint32_t)begin & 15u;
     // the buffers' last 16-byte pieces, where they are not whole
     if (a.rows - row0 < a.tile_rows + 4u || (!kDirect && total - begin < tile_bytes + 16u)) {
       const Span s = span_at(begin), st = stat_at(row0);
-      span_tail<T>(s, gbuf, a.dy, id, members);
-      span_tail<T>(s, zbuf, a.z, id, members);
-      if (kJoin && a.inputs == 3) span_tail<T>(s, rbuf, a.dz, id, members);
-      span_tail<float>(st, mbuf, a.mean, id, members);
-      span_tail<float>(st, mbuf + a.stat_slot, a.rstd, id, members);
-      if (kCta) __syncthreads(); else __syncwarp();
+      span_tail<T>(s, gbuf, a.dy, lane, 32);
+      span_tail<T>(s, zbuf, a.z, lane, 32);
+      if (kJoin && a.inputs == 3) span_tail<T>(s, rbuf, a.dz, lane, 32);
+      span_tail<float>(st, mbuf, a.mean, lane, 32);
+      span_tail<float>(st, mbuf + a.stat_slot, a.rstd, lane, 32);
+      __syncwarp();
     }
     const uint32_t stat_shift = (uint32_t)row0 * 4 & 15u;
     const float* ms = reinterpret_cast<const float*>(mbuf + stat_shift);
     const float* qs = reinterpret_cast<const float*>(mbuf + a.stat_slot + stat_shift);
-    if (kBits && d.threshold) {  // a CTA's are read after the sums' barrier
-      fill_bits(d, i0, rows * a.cols, kept, id, members);
-      if (!kCta) __syncwarp();
+    if (kBits && d.threshold) {
+      fill_bits(d, i0, rows * a.cols, bits, lane, 32);
+      __syncwarp();
     }
     for (uint32_t p = 0; p < rows; p += per_pass) {
       // a lane beyond the tile's rows computes its last row and leaves nothing
-      const bool live = kCta || p + sub < rows;
-      const uint32_t r = kCta ? 0 : live ? p + sub : rows - 1, r_at = r * a.cols;
+      const bool live = p + sub < rows;
+      const uint32_t r = live ? p + sub : rows - 1, r_at = r * a.cols;
       T* gr = reinterpret_cast<T*>(gbuf + shift) + r_at;
       T* zr = reinterpret_cast<T*>(zbuf + shift) + r_at;
       const T* dr = reinterpret_cast<const T*>(rbuf + shift) + r_at;
@@ -157,7 +137,7 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
       R t[PAIRS], res[PAIRS];
       part.load(gr, t);
       part.clear(t);
-      if (!kCta && p + per_pass > rows && !live) {  // the first test is the same for all
+      if (p + per_pass > rows && !live) {  // the first test is the same for all
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) t[i] = R{};
       }
@@ -176,28 +156,17 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
       }
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        g[i] = mul2(g[i], kCta ? ws[i * members] : w[i]);
+        g[i] = mul2(g[i], w[i]);
         s1 = add2(s1, g[i]);
         s2 = fma2(g[i], h[i], s2);
       }
       float m1 = s1.x + s1.y, m2 = s2.x + s2.y;
-      if (kCta) {
-        m1 = warp_sum2(m1, m2);
-        if ((id & 15u) == 0) red[half][id >> 4 & 1u][id >> 5] = m1;
-        // `red`, `late` and the keep bits alternate between two rows, so one
-        // barrier per row is enough
-        __syncthreads();
-        ok = !late[half];
-        m1 = parts_sum(red[half][0], warps);
-        m2 = parts_sum(red[half][1], warps);
-      } else {
-        m1 = lanes_sum(m1, lanes);
-        m2 = lanes_sum(m2, lanes);
-      }
+      m1 = lanes_sum(m1, lanes);
+      m2 = lanes_sum(m2, lanes);
       m1 = quotient(m1, n, inv);
       m2 = quotient(m2, n, inv);
-      if (!kCta && !kDirect) __syncwarp();  // the last row is read by all before it is written
-      if (live && ok) {
+      if (!kDirect) __syncwarp();  // the last row is read by all before it is written
+      if (live) {
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) g[i] = mul2(fma2(h[i], both(-m2), add2(g[i], both(-m1))), both(q));
         if (kJoin) {
@@ -208,40 +177,38 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
 #pragma unroll
           for (int i = 0; i < PAIRS; ++i) part.set(t, i, g[i]);
           part.store(kDirect ? static_cast<T*>(a.dresidual) + i0 + r_at : zr, t);
-          if (d.threshold) drop_part(part, g, i0 + r_at, d, kept, ((uint32_t)i0 & 7u) + r_at);
+          if (d.threshold) drop_part(part, g, i0 + r_at, d, bits, ((uint32_t)i0 & 7u) + r_at);
         }
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) part.set(t, i, g[i]);
         part.store(kDirect ? static_cast<T*>(a.dx) + i0 + r_at : gr, t);
       }
     }
-    if (kCta && !ok) break;
-    half ^= 1;
     if (kDirect) {
-      // every thread has its part of the tile in registers (a CTA's by the sums' barrier)
-      if (!kCta) __syncwarp();
-      if (id == 0) refill(slot);
+      // every lane has its part of the tile in registers
+      __syncwarp();
+      if (lane == 0) refill(slot);
     } else {
       proxy_fence();
-      if (kCta) __syncthreads(); else __syncwarp();
-      if (id < 32) {
+      __syncwarp();
+      {
         const Span s = span_at(begin);
-        span_store<T>(s, gbuf, a.dx, id);
-        if (kJoin) span_store<T>(s, zbuf, a.dresidual, id);
+        span_store<T>(s, gbuf, a.dx, lane);
+        if (kJoin) span_store<T>(s, zbuf, a.dresidual, lane);
       }
-      if (id == 0) {
+      if (lane == 0) {
         bulk_commit();
         bulk_wait_read<1>();
         if (row0 != first * a.tile_rows) refill(slot == 0 ? a.stages - 1 : slot - 1);
       }
-      if (!kCta) __syncwarp();
+      __syncwarp();
     }
     if (++slot == a.stages) {
       slot = 0;
       parity ^= 1;
     }
   }
-  if (!ok && id == 0) {  // a copy did not land in time: report, and let those in flight end
+  if (!ok && lane == 0) {  // a copy did not land in time: report, and let those in flight end
     atomicOr(a.err, VS_DERR_WAIT);
     for (uint32_t k = 0; k < a.stages && row0 < a.rows; ++k, row0 += step_rows) {
       mbar_wait(&full[slot], parity);
@@ -251,26 +218,15 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
       }
     }
   }
-  if (!kDirect && id == 0) bulk_wait<0>();
+  if (!kDirect && lane == 0) bulk_wait<0>();
   if (!a.partial) return;
 
   float* out = a.partial + (uint64_t)blockIdx.x * 2 * a.cols;
-  if (kCta) {
-#pragma unroll
-    for (int e = 0; e < P::E; ++e) {
-      const uint32_t c = part.col(e / VEC) + e % VEC;
-      if (part.has(e / VEC)) {
-        out[c] = (&dw[e / 2].x)[e % 2];
-        out[a.cols + c] = (&db[e / 2].x)[e % 2];
-      }
-    }
-    return;
-  }
   // lanes with the same columns (their runs turned differently), then the
   // warps, each in order, through the rings' memory
   __syncthreads();
   float* sums = reinterpret_cast<float*>(smem);  // [warp][2][cols]
-  float* mine = sums + worker * 2 * a.cols;
+  float* mine = sums + warp * 2 * a.cols;
   for (uint32_t k = 0; k < per_pass; ++k) {
     if (sub == k) {
 #pragma unroll
@@ -294,10 +250,9 @@ __global__ void __launch_bounds__(kCta ? NORM_BWD_THREADS : NORM_WARPS * 32, kCt
 }
 
 // Leaves *taken as it is where the slots do not fit.
-template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kernel(vs_ctx* ctx, const NormBwd& f, bool* taken) {
+template <typename T, int VEC, int K, bool kJoin> vs_status run_kernel(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   static std::atomic<uint64_t> ready{0};
-  constexpr uint32_t WORKERS = kCta ? 1 : NORM_WARPS;
-  auto kernel = norm_bwd_kernel<T, VEC, K, kJoin, kCta>;
+  auto kernel = norm_bwd_kernel<T, VEC, K, kJoin>;
   const uint64_t bit = 1ull << (ctx->device & 63);
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
     VS_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)NORM_MAX_SMEM));
@@ -308,34 +263,26 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   a.cols = f.s.cols;
   a.inputs = f.dz ? 3 : 2;
   const uint32_t chunks = (a.cols + VEC - 1) / VEC, row_bytes = a.cols * (uint32_t)sizeof(T);
-  uint32_t threads = NORM_WARPS * 32, per_sm = warp_ctas<T, VEC, K>();
-  a.tile_rows = 1;
-  if (kCta) {
-    threads = ((chunks + K - 1) / K + 31) & ~31u;
-    per_sm = NORM_BWD_THREADS / threads;
-  } else {
-    while ((1u << a.log_lanes) * K < chunks) ++a.log_lanes;
-    // As in the forward, and the same for the plain and the joined kernel, so
-    // that their weight gradients are the same sums in the same order.
-    const uint32_t per_pass = 32u >> a.log_lanes;
-    uint32_t passes = warp_slot<T, VEC>() / (row_bytes * per_pass);
-    const uint64_t share = (uint64_t)B200_SMS * per_sm * WORKERS * per_pass;
-    const uint64_t even = (a.rows + share - 1) / share;
-    if (passes > even) passes = (uint32_t)even;
-    a.tile_rows = (passes < 1 ? 1 : passes) * per_pass;
-  }
+  uint32_t per_sm = warp_ctas<T, VEC, K>();
+  while ((1u << a.log_lanes) * K < chunks) ++a.log_lanes;
+  // As in the forward, and the same for the plain and the joined kernel, so
+  // that their weight gradients are the same sums in the same order.
+  const uint32_t per_pass = 32u >> a.log_lanes;
+  uint32_t passes = warp_slot<T, VEC>() / (row_bytes * per_pass);
+  const uint64_t share = (uint64_t)B200_SMS * per_sm * NORM_WARPS * per_pass;
+  const uint64_t even = (a.rows + share - 1) / share;
+  if (passes > even) passes = (uint32_t)even;
+  a.tile_rows = (passes < 1 ? 1 : passes) * per_pass;
   a.slot = (a.tile_rows * row_bytes + 30u) & ~15u;
   a.stat_slot = (a.tile_rows * 4 + 30u) & ~15u;
-  a.bits = VEC != 8 ? ((a.tile_rows * a.cols / 8 + 2 + 15) & ~15u) * (kCta ? 2 : 1) : 0;
+  a.bits = VEC != 8 ? ((a.tile_rows * a.cols / 8 + 2 + 15) & ~15u) : 0;
   // Slots and CTAs as in the forward, the CTAs as for the joined kernel's three
-  // inputs; the rings' memory also takes the warps' column sums, and a CTA's
-  // threads keep their weights behind theirs.
+  // inputs; the rings' memory also takes the warps' column sums.
   constexpr uint32_t least = Part<T, VEC, K>::kVector ? 1 : 2;
-  const uint32_t sums = kCta ? 0 : WORKERS * 2 * a.cols * 4;
-  const uint32_t ws = kCta ? threads * Part<T, VEC, K>::PAIRS * 8 : 0;
+  const uint32_t sums = NORM_WARPS * 2 * a.cols * 4;
   auto bytes = [&](uint32_t inputs, uint32_t stages) {
-    const uint32_t rings = WORKERS * (stages * (inputs * a.slot + 2 * a.stat_slot) + a.bits);
-    return (!kCta && rings < sums ? sums : rings) + ws + NORM_PADDING;
+    const uint32_t rings = NORM_WARPS * (stages * (inputs * a.slot + 2 * a.stat_slot) + a.bits);
+    return (rings < sums ? sums : rings) + NORM_PADDING;
   };
   auto room = [&] { return NORM_MAX_SMEM / per_sm - 1024; };
   while (per_sm > 1 && bytes(3, 2) > room()) --per_sm;
@@ -346,14 +293,14 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   a.dy = f.dy; a.z = f.z; a.dz = f.dz; a.w = f.w; a.mean = f.mean; a.rstd = f.rstd;
   a.dx = f.dx; a.dresidual = f.dresidual;
   a.err = ctx->d_err;
-  const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + WORKERS - 1) / WORKERS;
+  const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + NORM_WARPS - 1) / NORM_WARPS;
   const uint64_t all = (uint64_t)per_sm * B200_SMS;
   const uint32_t grid = (uint32_t)(all < most ? all : most);
   const bool want = f.dweight || f.dbias;
   NormScratch scratch;
   if (want) VS_TRY(norm_scratch_begin(ctx, (size_t)grid * 2 * a.cols, &scratch));
   a.partial = scratch.p;
-  kernel<<<grid, threads, bytes(a.inputs, a.stages), ctx->stream>>>(a, f.d);
+  kernel<<<grid, NORM_WARPS * 32, bytes(a.inputs, a.stages), ctx->stream>>>(a, f.d);
   ++ctx->launches;
   vs_status st = vs_cuda(ctx, cudaGetLastError(), "norm backward launch");
   if (want) {
@@ -364,32 +311,24 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   return st;
 }
 
-// As in the forward, with up to 3 runs of 8 or 4 of 4 values per lane; a CTA's
-// threads hold up to 32 values.
+// As in the forward, with up to 3 runs of 8 or 4 of 4 values per lane.
 template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   constexpr int V = 16 / sizeof(T);
   const uint32_t chunks = f.s.cols / V;
   switch (norm_runs(chunks, sizeof(T) == 4 ? 4 : 3)) {
-    case 1: return run_kernel<T, V, 1, kJoin, false>(ctx, f, taken);
-    case 2: return run_kernel<T, V, 2, kJoin, false>(ctx, f, taken);
-    case 3: return run_kernel<T, V, 3, kJoin, false>(ctx, f, taken);
+    case 1: return run_kernel<T, V, 1, kJoin>(ctx, f, taken);
+    case 2: return run_kernel<T, V, 2, kJoin>(ctx, f, taken);
+    case 3: return run_kernel<T, V, 3, kJoin>(ctx, f, taken);
     case 4:
-      if constexpr (sizeof(T) == 4) return run_kernel<T, V, 4, kJoin, false>(ctx, f, taken);
-  }
-  if (sizeof(T) == 2 || chunks <= 128 * 4) {
-    if (chunks <= NORM_BWD_THREADS * 4) return run_kernel<T, V, 4, kJoin, true>(ctx, f, taken);
-  } else if (chunks <= NORM_BWD_THREADS * 8) {
-    return run_kernel<float, 4, 8, kJoin, true>(ctx, f, taken);
+      if constexpr (sizeof(T) == 4) return run_kernel<T, V, 4, kJoin>(ctx, f, taken);
   }
   return VS_OK;
 }
 
 template <typename T, int VEC, int KS, int KL, bool kJoin>
 vs_status run_blocks(vs_ctx* ctx, const NormBwd& f, bool* taken) {
-  if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin, false>(ctx, f, taken);
-  if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin, false>(ctx, f, taken);
-  if (f.s.cols <= NORM_BWD_THREADS * VEC * KL) return run_kernel<T, VEC, KL, kJoin, true>(ctx, f, taken);
-  if (f.s.cols <= NORM_BWD_THREADS * VEC * (2 * KL + 1)) return run_kernel<T, VEC, 2 * KL + 1, kJoin, true>(ctx, f, taken);
+  if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin>(ctx, f, taken);
+  if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin>(ctx, f, taken);
   return VS_OK;
 }
 
@@ -402,7 +341,7 @@ template <typename T, bool kJoin> vs_status run(vs_ctx* ctx, const NormBwd& f, b
 
 }  // namespace
 
-vs_status norm_stream_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBwd& f, bool* taken) {
+vs_status norm_tile_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBwd& f, bool* taken) {
   *taken = false;
   return vs_with_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);

@@ -1,12 +1,11 @@
 // Streaming forward layer norm, alone or joined with the dropout and residual
-// sum before it, for contiguous rows.
+// sum before it, for short contiguous rows.
 //
 // The work is one read and one write of the rows, so the kernels keep bulk
-// copies in flight all the time: each worker (a warp with a tile of rows, or a
-// CTA with one row of more than about 500 values) owns a ring of shared-memory
-// slots that one thread refills with cp.async.bulk, and holds its row in
-// registers for the two sums (mean, then squares about it).  A thread's columns
-// are the same for every row, so the weights stay in registers too.
+// copies in flight all the time: each warp owns a ring of shared-memory slots, a
+// tile of rows each, that one lane refills with cp.async.bulk, and its lanes hold
+// rows in registers for the two sums (mean, then squares about it).  A lane's
+// columns are the same for every row, so the weights stay in registers too.
 #include <atomic>
 
 #include "norm.cuh"
@@ -15,7 +14,7 @@ namespace {
 
 using namespace vs;
 
-// CTAs of the warp workers on an SM, and the bytes of one slot and input.  Two
+// CTAs of the warp warps on an SM, and the bytes of one slot and input.  Two
 // things meet here.  Every byte in flight beyond what hides the latency only
 // queues in front of the DRAM and costs throughput (f32 rows of 256, two slots
 // of 2 KB a warp: 12 warps 97 % of the copy rate, 16 warps 86 %; joined, two
@@ -44,30 +43,25 @@ struct FwdArgs {
 // Rows of whole 16-byte vectors are written from registers; others go back into
 // their slot and out by a bulk store, so that no access is narrower than its
 // run of bytes.
-template <typename T, int VEC, int K, bool kJoin, bool kCta>
-__global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCta ? 1 : warp_ctas<T, VEC, K, kJoin>())
+template <typename T, int VEC, int K, bool kJoin>
+__global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K, kJoin>())
     norm_fwd_kernel(const FwdArgs a, const __grid_constant__ Dropout d) {
   using P = Part<T, VEC, K>;
   using R = typename P::R;
   constexpr int PAIRS = P::PAIRS;
   constexpr bool kDirect = P::kVector;
   constexpr bool kBits = kJoin && VEC != 8;
-  constexpr uint32_t NIN = kJoin ? 2 : 1, WORKERS = kCta ? 1 : NORM_WARPS;
+  constexpr uint32_t NIN = kJoin ? 2 : 1;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t bars[WORKERS][NORM_STAGES];
-  __shared__ __align__(16) float red[2][kCta ? NORM_MAX_WARPS : 4];
-  __shared__ uint32_t late;
-  const uint32_t worker = kCta ? 0 : threadIdx.x >> 5;
-  const uint32_t id = kCta ? threadIdx.x : threadIdx.x & 31u, members = kCta ? blockDim.x : 32;
-  const uint32_t warps = blockDim.x >> 5;
-  const uint32_t lanes = kCta ? members : 1u << a.log_lanes;
-  const uint32_t sub = kCta ? 0 : id >> a.log_lanes, per_pass = kCta ? 1 : 32u >> a.log_lanes;
-  const P part(kCta ? id : id & (lanes - 1), lanes, sub, a.cols);
-  unsigned char* ring = smem + (size_t)worker * (a.stages * NIN * a.slot + a.bits);
+  __shared__ __align__(8) uint64_t bars[NORM_WARPS][NORM_STAGES];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t lanes = 1u << a.log_lanes, sub = lane >> a.log_lanes, per_pass = 32u >> a.log_lanes;
+  const P part(lane & (lanes - 1), lanes, sub, a.cols);
+  unsigned char* ring = smem + (size_t)warp * (a.stages * NIN * a.slot + a.bits);
   uint32_t* bits = reinterpret_cast<uint32_t*>(ring + a.stages * NIN * a.slot);
-  uint64_t* full = bars[worker];
+  uint64_t* full = bars[warp];
 
-  const uint64_t first = (uint64_t)blockIdx.x * WORKERS + worker, step = (uint64_t)gridDim.x * WORKERS;
+  const uint64_t first = (uint64_t)blockIdx.x * NORM_WARPS + warp, step = (uint64_t)gridDim.x * NORM_WARPS;
   const uint32_t tile_bytes = a.tile_rows * a.cols * (uint32_t)sizeof(T);
   const uint64_t total = a.rows * a.cols * sizeof(T), step_bytes = step * tile_bytes;
   uint64_t begin = first * tile_bytes;  // of the tile at hand
@@ -86,8 +80,7 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
     }
     load_at += step_bytes;
   };
-  if (id == 0) {
-    if (kCta) late = 0;
+  if (lane == 0) {
     for (uint32_t k = 0; k < a.stages; ++k) mbar_init(&full[k], 1);
     mbar_init_fence();
     for (uint32_t k = 0; k < a.stages; ++k) refill(k);
@@ -96,39 +89,33 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
   part.weights(a.w.weight, a.w.dtype, 1.0f, w);
   part.weights(a.w.bias, a.w.dtype, 0.0f, b);
   const float n = (float)a.cols, inv = 1.0f / n;
-  if (kCta)
-    for (uint32_t k = id; k < 2 * NORM_MAX_WARPS; k += members) (&red[0][0])[k] = 0.0f;
-  if (kCta) __syncthreads(); else __syncwarp();
+  __syncwarp();
 
   uint32_t slot = 0, parity = 0;
   bool ok = true;
   uint64_t row0 = first * a.tile_rows;
   for (; row0 < a.rows; row0 += step * a.tile_rows, begin += step_bytes) {
-    ok = mbar_wait(&full[slot], parity);
-    if (kCta) {
-      if (!ok) late = 1;
-    } else if (!(ok = __all_sync(0xffffffffu, ok))) {
-      break;
-    }
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], parity));
+    if (!ok) break;
     unsigned char* in = ring + slot * NIN * a.slot;
     unsigned char* res = in + a.slot;
-    const uint32_t rows = kCta ? 1 : a.rows - row0 < a.tile_rows ? (uint32_t)(a.rows - row0) : a.tile_rows;
+    const uint32_t rows = a.rows - row0 < a.tile_rows ? (uint32_t)(a.rows - row0) : a.tile_rows;
     const uint64_t i0 = begin / sizeof(T);
     const uint32_t shift = kDirect ? 0 : (uint32_t)begin & 15u;
     if (!kDirect && total - begin < tile_bytes + 16u) {  // the last 16-byte piece, where it is not whole
       const Span s = span_at(begin);
-      span_tail<T>(s, in, a.x, id, members);
-      if (kJoin) span_tail<T>(s, res, a.residual, id, members);
-      if (kCta) __syncthreads(); else __syncwarp();
+      span_tail<T>(s, in, a.x, lane, 32);
+      if (kJoin) span_tail<T>(s, res, a.residual, lane, 32);
+      __syncwarp();
     }
     if (kBits && d.threshold) {
-      fill_bits(d, i0, rows * a.cols, bits, id, members);
-      if (kCta) __syncthreads(); else __syncwarp();
+      fill_bits(d, i0, rows * a.cols, bits, lane, 32);
+      __syncwarp();
     }
     for (uint32_t p = 0; p < rows; p += per_pass) {
       // a lane beyond the tile's rows computes its last row and writes nothing
-      const bool live = kCta || p + sub < rows;
-      const uint32_t r = kCta ? 0 : live ? p + sub : rows - 1, r_at = r * a.cols;
+      const bool live = p + sub < rows;
+      const uint32_t r = live ? p + sub : rows - 1, r_at = r * a.cols;
       T* xr = reinterpret_cast<T*>(in + shift) + r_at;
       T* rr = reinterpret_cast<T*>(res + shift) + r_at;
       float2 v[PAIRS];
@@ -151,16 +138,15 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) s = add2(v[i], s);
       float m = s.x + s.y;
-      m = quotient(kCta ? cta_sum(m, red[0], warps) : lanes_sum(m, lanes), n, inv);
-      if (kCta) ok = !late;  // between two barriers: the same for all
+      m = quotient(lanes_sum(m, lanes), n, inv);
       part.subtract(v, m);
       s = both(0.0f);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) s = fma2(v[i], v[i], s);
       float q = s.x + s.y;
-      q = rsqrtf(fmaf(kCta ? cta_sum(q, red[1], warps) : lanes_sum(q, lanes), inv, a.eps));
-      if (!kCta && !kDirect) __syncwarp();  // the last row is read by all before it is written
-      if (live && ok) {
+      q = rsqrtf(fmaf(lanes_sum(q, lanes), inv, a.eps));
+      if (!kDirect) __syncwarp();  // the last row is read by all before it is written
+      if (live) {
         if (kJoin) part.store(kDirect ? static_cast<T*>(a.z) + i0 + r_at : rr, t);
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) part.set(t, i, fma2(mul2(v[i], both(q)), w[i], b[i]));
@@ -171,33 +157,32 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
         }
       }
     }
-    if (kCta && !ok) break;
     if (kDirect) {
-      // every thread has its part of the tile in registers (the sums' barriers tell)
-      if (!kCta) __syncwarp();
-      if (id == 0) refill(slot);
+      // every lane has its part of the tile in registers
+      __syncwarp();
+      if (lane == 0) refill(slot);
     } else {
       proxy_fence();
-      if (kCta) __syncthreads(); else __syncwarp();
-      if (id < 32) {
+      __syncwarp();
+      {
         const Span s = span_at(begin);
-        span_store<T>(s, in, a.y, id);
-        if (kJoin) span_store<T>(s, res, a.z, id);
+        span_store<T>(s, in, a.y, lane);
+        if (kJoin) span_store<T>(s, res, a.z, lane);
       }
-      if (id == 0) {
+      if (lane == 0) {
         bulk_commit();
         // the slot before this one has been read out by now: it is filled again
         bulk_wait_read<1>();
         if (row0 != first * a.tile_rows) refill(slot == 0 ? a.stages - 1 : slot - 1);
       }
-      if (!kCta) __syncwarp();
+      __syncwarp();
     }
     if (++slot == a.stages) {
       slot = 0;
       parity ^= 1;
     }
   }
-  if (!ok && id == 0) {  // a copy did not land in time: report, and let those in flight end
+  if (!ok && lane == 0) {  // a copy did not land in time: report, and let those in flight end
     atomicOr(a.err, VS_DERR_WAIT);
     for (uint32_t k = 0; k < a.stages && row0 < a.rows; ++k, row0 += step * a.tile_rows) {
       mbar_wait(&full[slot], parity);
@@ -207,14 +192,14 @@ __global__ void __launch_bounds__(kCta ? NORM_FWD_THREADS : NORM_WARPS * 32, kCt
       }
     }
   }
-  if (!kDirect && id == 0) bulk_wait<0>();
+  if (!kDirect && lane == 0) bulk_wait<0>();
 }
 
 // Leaves *taken as it is where the slots do not fit.
-template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kernel(vs_ctx* ctx, const NormFwd& f, bool* taken) {
+template <typename T, int VEC, int K, bool kJoin> vs_status run_kernel(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   static std::atomic<uint64_t> ready{0};
-  constexpr uint32_t NIN = kJoin ? 2 : 1, WORKERS = kCta ? 1 : NORM_WARPS;
-  auto kernel = norm_fwd_kernel<T, VEC, K, kJoin, kCta>;
+  constexpr uint32_t NIN = kJoin ? 2 : 1;
+  auto kernel = norm_fwd_kernel<T, VEC, K, kJoin>;
   const uint64_t bit = 1ull << (ctx->device & 63);
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
     VS_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)NORM_MAX_SMEM));
@@ -224,21 +209,15 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   a.rows = f.s.rows;
   a.cols = f.s.cols;
   const uint32_t chunks = (a.cols + VEC - 1) / VEC, row_bytes = a.cols * (uint32_t)sizeof(T);
-  uint32_t threads = NORM_WARPS * 32, per_sm = warp_ctas<T, VEC, K, kJoin>();
-  a.tile_rows = 1;
-  if (kCta) {
-    threads = ((chunks + K - 1) / K + 31) & ~31u;
-    per_sm = NORM_FWD_THREADS / threads;
-  } else {
-    while ((1u << a.log_lanes) * K < chunks) ++a.log_lanes;
-    // whole passes per slot; fewer where that would leave warps without rows
-    const uint32_t per_pass = 32u >> a.log_lanes;
-    uint32_t passes = warp_slot<T, VEC>() / (row_bytes * per_pass);
-    const uint64_t share = (uint64_t)B200_SMS * per_sm * WORKERS * per_pass;
-    const uint64_t even = (a.rows + share - 1) / share;
-    if (passes > even) passes = (uint32_t)even;
-    a.tile_rows = (passes < 1 ? 1 : passes) * per_pass;
-  }
+  uint32_t per_sm = warp_ctas<T, VEC, K, kJoin>();
+  while ((1u << a.log_lanes) * K < chunks) ++a.log_lanes;
+  // whole passes per slot; fewer where that would leave warps without rows
+  const uint32_t per_pass = 32u >> a.log_lanes;
+  uint32_t passes = warp_slot<T, VEC>() / (row_bytes * per_pass);
+  const uint64_t share = (uint64_t)B200_SMS * per_sm * NORM_WARPS * per_pass;
+  const uint64_t even = (a.rows + share - 1) / share;
+  if (passes > even) passes = (uint32_t)even;
+  a.tile_rows = (passes < 1 ? 1 : passes) * per_pass;
   a.slot = (a.tile_rows * row_bytes + 30u) & ~15u;
   a.bits = kJoin && VEC != 8 ? (a.tile_rows * a.cols / 8 + 2 + 15) & ~15u : 0;
   // Two slots: one being worked on, one on its way (a third one costs rows of
@@ -246,7 +225,7 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   // CTAs where the SM's shared memory does not hold theirs.  A slot that is
   // written back needs at least another beside it.
   constexpr uint32_t least = Part<T, VEC, K>::kVector ? 1 : 2;
-  auto bytes = [&](uint32_t stages) { return WORKERS * (stages * NIN * a.slot + a.bits) + NORM_PADDING; };
+  auto bytes = [&](uint32_t stages) { return NORM_WARPS * (stages * NIN * a.slot + a.bits) + NORM_PADDING; };
   auto room = [&] { return NORM_MAX_SMEM / per_sm - 1024; };
   while (per_sm > 1 && bytes(2) > room()) --per_sm;
   a.stages = Part<T, VEC, K>::kVector ? 2 : 3;
@@ -255,36 +234,32 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status run_kerne
   *taken = true;
   a.x = f.x; a.residual = f.residual; a.w = f.w; a.eps = f.eps; a.y = f.y; a.z = f.z; a.mean = f.mean; a.rstd = f.rstd;
   a.err = ctx->d_err;
-  const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + WORKERS - 1) / WORKERS;
+  const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + NORM_WARPS - 1) / NORM_WARPS;
   const uint64_t grid = (uint64_t)per_sm * B200_SMS;
-  kernel<<<(uint32_t)(grid < most ? grid : most), threads, bytes(a.stages), ctx->stream>>>(a, f.d);
+  kernel<<<(uint32_t)(grid < most ? grid : most), NORM_WARPS * 32, bytes(a.stages), ctx->stream>>>(a, f.d);
   ++ctx->launches;
   return vs_cuda(ctx, cudaGetLastError(), "norm launch");
 }
 
 // The runs per lane, of 1 to 4, with the fewest idle places on a warp's lanes
-// (then the most, for the fewest shuffles); rows over a warp's 4 runs take a CTA.
+// (then the most, for the fewest shuffles).
 template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   constexpr int V = 16 / sizeof(T);
   const uint32_t chunks = f.s.cols / V;
   switch (norm_runs(chunks, 4)) {
-    case 1: return run_kernel<T, V, 1, kJoin, false>(ctx, f, taken);
-    case 2: return run_kernel<T, V, 2, kJoin, false>(ctx, f, taken);
-    case 3: return run_kernel<T, V, 3, kJoin, false>(ctx, f, taken);
-    case 4: return run_kernel<T, V, 4, kJoin, false>(ctx, f, taken);
+    case 1: return run_kernel<T, V, 1, kJoin>(ctx, f, taken);
+    case 2: return run_kernel<T, V, 2, kJoin>(ctx, f, taken);
+    case 3: return run_kernel<T, V, 3, kJoin>(ctx, f, taken);
+    case 4: return run_kernel<T, V, 4, kJoin>(ctx, f, taken);
   }
-  if (chunks <= NORM_FWD_THREADS * 4) return run_kernel<T, V, 4, kJoin, true>(ctx, f, taken);
-  if (sizeof(T) == 4 && chunks <= NORM_FWD_THREADS * 8) return run_kernel<float, 4, 8, kJoin, true>(ctx, f, taken);
   return VS_OK;
 }
 
 // KS runs in a block where they hold the row, KL otherwise.
 template <typename T, int VEC, int KS, int KL, bool kJoin>
 vs_status run_blocks(vs_ctx* ctx, const NormFwd& f, bool* taken) {
-  if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin, false>(ctx, f, taken);
-  if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin, false>(ctx, f, taken);
-  if (f.s.cols <= NORM_FWD_THREADS * VEC * KL) return run_kernel<T, VEC, KL, kJoin, true>(ctx, f, taken);
-  if (f.s.cols <= NORM_FWD_THREADS * VEC * (2 * KL + 1)) return run_kernel<T, VEC, 2 * KL + 1, kJoin, true>(ctx, f, taken);
+  if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin>(ctx, f, taken);
+  if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin>(ctx, f, taken);
   return VS_OK;
 }
 
@@ -297,7 +272,7 @@ template <typename T, bool kJoin> vs_status run(vs_ctx* ctx, const NormFwd& f, b
 
 }  // namespace
 
-vs_status norm_stream_forward(vs_ctx* ctx, int32_t dtype, bool join, const NormFwd& f, bool* taken) {
+vs_status norm_tile_forward(vs_ctx* ctx, int32_t dtype, bool join, const NormFwd& f, bool* taken) {
   *taken = false;
   return vs_with_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
