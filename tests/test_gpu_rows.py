@@ -246,6 +246,66 @@ def test_dropout_add_norm_bwd(cuda, dtype, rows, cols):
             assert torch.equal(v.dx, want[0]) and torch.equal(v.dresidual, want[1])
 
 
+# Calls large enough for the streaming backward kernels (over 16 MB of traffic) in every type, with tiles and rows
+# that end inside 16-byte pieces.  The sums over the rows are strips of at most a few hundred rows each.
+LARGE = [(250_001, 12), (900_000, 5), (60_001, 59), (50_003, 64), (30_001, 100), (10_001, 384), (7_001, 520),
+         (3_701, 1030), (1_901, 2049), (1_001, 4096), (801, 5003), (331, 12_000)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", LARGE)
+def test_large_backward(cuda, dtype, rows, cols):
+    z, z64 = rows_of(cuda, rows, cols, dtype, rows + cols)
+    dy, dy64 = rows_of(cuda, rows, cols, dtype, rows + cols + 1)
+    dz, dz64 = rows_of(cuda, rows, cols, dtype, rows + cols + 2)
+    w, _, w64, _ = weights_of(cuda, cols, F32, cols)
+    o = ops.layer_norm(z, w, None, EPS)
+    y64, m64, q64 = norm_ref(z64, w64, 0.0)
+    close(o.y, y64, "y", terms=max(1.0, float(q64.max())))
+    m, q = o.mean.cpu().double()[:, None], o.rstd.cpu().double()[:, None]
+    t64, dw64, db64 = norm_bwd_ref(dy64, z64, w64, m, q)
+    scale = float(q.max() * dy64.abs().max() * w64.abs().max())
+    g = ops.layer_norm_bwd(dy, z, w, o.mean, o.rstd)
+    close(g.dx, t64, "dx", terms=max(1.0, scale / float(t64.abs().max())))
+    h = ((z64 - m) * q).abs()
+    close(g.dweight, dw64, "dweight", terms=max(1.0, float((dy64.abs() * h).sum(0).max()) / float(dw64.abs().max())))
+    close(g.dbias, db64, "dbias", terms=max(1.0, float(dy64.abs().sum(0).max()) / float(db64.abs().max())))
+    for d, d64 in ((dz, dz64), (None, 0.0)):
+        j = ops.dropout_add_norm_bwd(dy, d, z, w, o.mean, o.rstd, 0.25, 11, 2**33 + 5)
+        want = t64 + d64
+        close(j.dresidual, want, "dresidual", terms=max(1.0, scale / float(want.abs().max())))
+        dx64 = dropout_ref(want, 0.25, 11, 2**33 + 5)
+        close(j.dx, dx64, "joined dx", terms=max(1.0, 2 * scale / float(dx64.abs().max())))
+        assert torch.equal(j.dweight, g.dweight) and torch.equal(j.dbias, g.dbias)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(60_001, 59), (3_701, 1030), (1_001, 4096)])
+def test_large_in_place_and_strided(cuda, dtype, rows, cols):
+    """In place, and from columns of a wider buffer, the same bits as out of place from contiguous rows (the column
+    sums of strided rows are taken by another kernel and only agree within rounding)."""
+    z, _ = rows_of(cuda, rows, cols, dtype, 1)
+    dy, _ = rows_of(cuda, rows, cols, dtype, 2)
+    dz, _ = rows_of(cuda, rows, cols, dtype, 3)
+    w, b, _, _ = weights_of(cuda, cols, F32, 4)
+    o = ops.dropout_add_norm(dy, z, w, b, 0.25, 1, 2)
+    g = ops.dropout_add_norm_bwd(dy, dz, z, w, o.mean, o.rstd, 0.25, 1, 2)
+    wide = [torch.zeros(rows, cols + 3, dtype=dtype, device=cuda) for _ in range(3)]
+    for k, t in zip(wide, (dy, dz, z)):
+        k[:, 1:1 + cols] = t
+    sdy, sdz, sz = (k[:, 1:1 + cols] for k in wide)
+    s = ops.dropout_add_norm_bwd(sdy, sdz, sz, w, o.mean, o.rstd, 0.25, 1, 2)
+    tol = 4 * UNIT[dtype] * float(g.dx.float().abs().max())
+    assert float((s.dx.float() - g.dx.float()).abs().max()) <= tol
+    assert float((s.dweight - g.dweight).abs().max()) <= F32_ERR * rows
+    f = ops.dropout_add_norm(sdy, sz, w, b, 0.25, 1, 2)
+    assert float((f.y.float() - o.y.float()).abs().max()) <= 4 * UNIT[dtype] * float(o.y.float().abs().max())
+    assert torch.equal(f.z, o.z)
+    v = ops.dropout_add_norm_bwd(dy, dz, z, w, o.mean, o.rstd, 0.25, 1, 2,
+                                 out=ops.DropoutAddNormGrads(dy, dz, torch.empty_like(w), torch.empty_like(w)))
+    assert torch.equal(v.dx, g.dx) and torch.equal(v.dresidual, g.dresidual) and torch.equal(v.dweight, g.dweight)
+
+
 def test_no_weights_and_single_gradients(cuda):
     x, x64 = rows_of(cuda, 50, 72, F32, 1)
     dy, dy64 = rows_of(cuda, 50, 72, F32, 2)

@@ -6,7 +6,6 @@
 //   backward  h = (z - m) q, g = dy w,
 //             t = q (g - mean g - h mean(g h)) (+ dz),
 //             dresidual = t, dx = dropout(t), dw = sum_rows dy h, db = sum_rows dy
-#include <stdlib.h>
 #include <initializer_list>
 
 #include "norm.cuh"
@@ -212,12 +211,6 @@ bool vector_rows(Shape s, std::initializer_list<uint64_t> strides, std::initiali
   return true;
 }
 
-// Calls whose traffic the direct kernels finish before rings would be full.
-bool is_small(Shape s, size_t bytes_per_value) {
-  static const double lim = getenv("VS_SMALL") ? atof(getenv("VS_SMALL")) : 8e6;
-  return (double)s.rows * s.cols * bytes_per_value < lim;
-}
-
 uint32_t row_grid(uint64_t rows) { return (uint32_t)(rows < 0x7fffffffull ? rows : 0x7fffffffull); }
 
 template <typename T, bool kJoin>
@@ -238,12 +231,10 @@ vs_status norm_forward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, co
   VS_CUDA(ctx, cudaSetDevice(ctx->device));
   const NormFwd f{s, x, residual, mx.stride, mr.stride, wt, eps, d, y, z, mean, rstd};
   const bool stream = vector_rows(s, {mx.stride, kJoin ? mr.stride : mx.stride}, {x, residual, y, z});
-  const bool small = is_small(s, sizeof(T) * (kJoin ? 4 : 2));
   bool taken = false;
-  if (stream && !small) VS_TRY(norm_tile_forward(ctx, dtype, kJoin, f, &taken));
-  if (stream && !small && !taken) VS_TRY(norm_row_forward(ctx, dtype, kJoin, f, &taken));
+  if (stream) VS_TRY(norm_tile_forward(ctx, dtype, kJoin, f, &taken));
+  if (stream && !taken) VS_TRY(norm_row_forward(ctx, dtype, kJoin, f, &taken));
   if (!taken) VS_TRY(norm_direct_forward(ctx, dtype, kJoin, f, &taken));
-  if (!taken && stream && small) VS_TRY(norm_row_forward(ctx, dtype, kJoin, f, &taken));
   if (taken) return VS_OK;
   norm_fwd_rows_kernel<T, kJoin><<<row_grid(s.rows), 256, 0, ctx->stream>>>(s, mx, mr, wt, eps, d, (T*)y, (T*)z, mean,
                                                                             rstd);
@@ -276,8 +267,11 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, c
                   wt.dtype, dweight, dbias};
   const bool stream = vector_rows(s, {mdy.stride, mz.stride, kJoin && dz ? mdz.stride : mz.stride},
                                   {dy, dz, z, dx, dresidual, mean, rstd});
-  // by the plain kernel's traffic, so that the joined one's weight gradients are the same sums
-  const bool small = is_small(s, sizeof(T) * 3);
+  // Small calls leave fewer CTAs' sums to join when they run direct: 20k x 64 f16
+  // (8 MB of the plain kernel's traffic, which decides for the joined one too, so
+  // that both add up the same sums) 17 and 25 us, 1000 x 4096 bf16 (25 MB) 23 and
+  // 25 us, 2000 x 4096 35 and 29 us.
+  const bool small = (double)s.rows * s.cols * sizeof(T) * 3 < 16e6;
   bool taken = false;
   if (stream && !small) VS_TRY(norm_tile_backward(ctx, dtype, kJoin, f, &taken));
   if (stream && !small && !taken) VS_TRY(norm_row_backward(ctx, dtype, kJoin, f, &taken));

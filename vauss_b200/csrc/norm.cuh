@@ -435,20 +435,6 @@ constexpr uint32_t NORM_MAX_SMEM = 226 * 1024;
 // Threads of an SM that the CTA-per-row kernels' registers leave room for.  The
 // grids follow from this and the shape alone, never from an occupancy query, so
 // the order of the weight gradients' sums does too.
-#ifndef VAR_FK
-#define VAR_FK 4
-#endif
-#ifndef VAR_BK
-#define VAR_BK 4
-#endif
-#ifndef VAR_RF
-#define VAR_RF 512
-#endif
-#ifndef VAR_RB
-#define VAR_RB 384
-#endif
-constexpr uint32_t NORM_ROW_FWD = VAR_RF, NORM_ROW_BWD = VAR_RB;
-
 // The sums of a and b over a warp in one chain: lanes 0 to 15 get a's, the others b's.
 VSD float warp_sum2(float a, float b) {
   const bool low = (threadIdx.x & 16u) == 0;

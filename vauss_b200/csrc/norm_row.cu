@@ -16,6 +16,13 @@ namespace {
 
 using namespace vs;
 
+// Threads that an SM holds of the forward and of the backward by the values each
+// one holds: their registers fix it.
+template <typename T, int K, bool kJoin> constexpr uint32_t row_fwd() {
+  return K * (16 / sizeof(T)) <= 16 ? 768 : kJoin ? 384 : 512;
+}
+template <typename T, int K> constexpr uint32_t row_bwd() { return K * (16 / sizeof(T)) <= 16 ? 512 : 384; }
+
 struct RowArgs {
   uint64_t rows;
   uint32_t cols, slot, stages, inputs, ragged;  // ragged: 1 where the last warp takes the rows' ends
@@ -186,7 +193,7 @@ template <typename T> VSD bool end_column(const RowPlace<T>& place, uint32_t col
 }
 
 template <typename T, int K, bool kJoin>
-__global__ void __launch_bounds__(NORM_ROW_FWD) norm_row_fwd_kernel(const RowArgs a, const __grid_constant__ Dropout d) {
+__global__ void __launch_bounds__(row_fwd<T, K, kJoin>()) norm_row_fwd_kernel(const RowArgs a, const __grid_constant__ Dropout d) {
   using P = RowPart<T, K>;
   constexpr int PAIRS = P::PAIRS;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -294,7 +301,7 @@ __global__ void __launch_bounds__(NORM_ROW_FWD) norm_row_fwd_kernel(const RowArg
 }
 
 template <typename T, int K, bool kJoin>
-__global__ void __launch_bounds__(NORM_ROW_BWD) norm_row_bwd_kernel(const RowArgs a, const __grid_constant__ Dropout d) {
+__global__ void __launch_bounds__(row_bwd<T, K>()) norm_row_bwd_kernel(const RowArgs a, const __grid_constant__ Dropout d) {
   using P = RowPart<T, K>;
   constexpr int PAIRS = P::PAIRS;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -446,23 +453,32 @@ __global__ void __launch_bounds__(NORM_ROW_BWD) norm_row_bwd_kernel(const RowArg
   }
 }
 
-// Threads, grid and slots of a shape; `held` bytes per thread stand beside the
-// ring.  The grid follows from the largest number of inputs, so that the plain and
-// the joined backward add up the same sums.  False where the slots do not fit.
-template <typename T, int K>
-bool lay_out(RowArgs* a, uint32_t sm_threads, uint32_t most_inputs, uint32_t held, uint32_t* threads, uint32_t* grid,
-             size_t* smem) {
+// Threads of a CTA.
+template <typename T, int K> uint32_t row_threads(uint32_t cols) {
   constexpr uint32_t V = 16 / sizeof(T);
-  a->ragged = a->cols % V != 0;  // rows of whole vectors all start on one
-  *threads = ((a->cols / V + K - 1) / K + 31) & ~31u;
-  if (a->ragged) *threads += 32;
-  if (*threads > sm_threads) return false;
+  return ((cols / V + K - 1) / K + 31) / 32 * 32 + (cols % V ? 32 : 0);
+}
+
+// Grid and slots of a shape; `held` bytes per thread stand beside the ring, and
+// the grid is that of CTAs of `grid_threads` threads of `sm_threads` with `inputs`
+// inputs.  CTAs beyond what keeps `flight` bytes on their way only queue at the
+// DRAM: one input, f32 rows of 1024, 6 CTAs 95 % of the copy rate, 8 CTAs 85 %; two
+// inputs, bf16 rows of 4096, 3 CTAs 96 %, 4 CTAs 76 %.  False where the slots do not
+// fit.
+template <typename T>
+bool lay_out(RowArgs* a, uint32_t threads, uint32_t grid_threads, uint32_t sm_threads, uint32_t inputs, uint32_t held,
+             uint32_t* grid, size_t* smem) {
+  constexpr uint32_t V = 16 / sizeof(T);
+  if (threads > sm_threads || grid_threads > sm_threads) return false;
+  a->ragged = a->cols % V != 0;
   a->slot = (a->cols * (uint32_t)sizeof(T) + 30u) & ~15u;
-  uint32_t per_sm = sm_threads / *threads;
-  auto bytes = [&](uint32_t inputs, uint32_t stages) { return stages * inputs * a->slot + *threads * held; };
+  const uint32_t flight = (inputs > 1 ? 96 : sizeof(T) == 4 ? 48 : 64) * 1024, each = 2 * inputs * a->slot;
+  uint32_t per_sm = sm_threads / grid_threads;
+  if (per_sm > (flight + each - 1) / each) per_sm = (flight + each - 1) / each;
+  auto bytes = [&](uint32_t in, uint32_t stages) { return stages * in * a->slot + threads * held; };
   auto room = [&] { return NORM_MAX_SMEM / per_sm - 1024; };
-  while (per_sm > 1 && bytes(most_inputs, 2) > room()) --per_sm;
-  if (bytes(most_inputs, 1) > room()) return false;
+  while (per_sm > 1 && bytes(inputs, 2) > room()) --per_sm;
+  if (bytes(inputs, 1) > room()) return false;
   a->stages = bytes(a->inputs, 2) <= room() ? 2 : 1;
   *smem = bytes(a->inputs, a->stages);
   const uint64_t full = (uint64_t)per_sm * B200_SMS / V * V;
@@ -487,9 +503,10 @@ template <typename T, int K, bool kJoin> vs_status run(vs_ctx* ctx, const NormFw
   a.inputs = kJoin ? 2 : 1;
   a.in[0] = f.x; a.in[1] = f.residual; a.w = f.w; a.eps = f.eps; a.out0 = f.y; a.out1 = f.z;
   a.mean = f.mean; a.rstd = f.rstd; a.err = ctx->d_err;
-  uint32_t threads, grid;
+  const uint32_t threads = row_threads<T, K>(a.cols);
+  uint32_t grid;
   size_t smem;
-  if (!lay_out<T, K>(&a, NORM_ROW_FWD, a.inputs, 0, &threads, &grid, &smem)) return VS_OK;
+  if (!lay_out<T>(&a, threads, threads, row_fwd<T, K, kJoin>(), a.inputs, 0, &grid, &smem)) return VS_OK;
   auto kernel = norm_row_fwd_kernel<T, K, kJoin>;
   VS_TRY(allow_smem(ctx, kernel, ready));
   *taken = true;
@@ -498,7 +515,7 @@ template <typename T, int K, bool kJoin> vs_status run(vs_ctx* ctx, const NormFw
   return vs_cuda(ctx, cudaGetLastError(), "norm launch");
 }
 
-template <typename T, int K, bool kJoin> vs_status run(vs_ctx* ctx, const NormBwd& f, bool* taken) {
+template <typename T, int K, int KG, bool kJoin> vs_status run(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   static std::atomic<uint64_t> ready{0};
   RowArgs a{};
   a.rows = f.s.rows;
@@ -506,9 +523,11 @@ template <typename T, int K, bool kJoin> vs_status run(vs_ctx* ctx, const NormBw
   a.inputs = f.dz ? 3 : 2;
   a.in[0] = f.dy; a.in[1] = f.z; a.in[2] = f.dz; a.w = f.w; a.out0 = f.dx; a.out1 = f.dresidual;
   a.mean = const_cast<float*>(f.mean); a.rstd = const_cast<float*>(f.rstd); a.err = ctx->d_err;
-  uint32_t threads, grid;
+  // the grid is the joined kernel's for both, so that they add up the same sums
+  const uint32_t threads = row_threads<T, K>(a.cols);
+  uint32_t grid;
   size_t smem;
-  if (!lay_out<T, K>(&a, NORM_ROW_BWD, 3, RowPart<T, K>::E * 4, &threads, &grid, &smem)) return VS_OK;
+  if (!lay_out<T>(&a, threads, row_threads<T, KG>(a.cols), row_bwd<T, K>(), 3, RowPart<T, K>::E * 4, &grid, &smem)) return VS_OK;
   auto kernel = norm_row_bwd_kernel<T, K, kJoin>;
   VS_TRY(allow_smem(ctx, kernel, ready));
   *taken = true;
@@ -527,11 +546,24 @@ template <typename T, int K, bool kJoin> vs_status run(vs_ctx* ctx, const NormBw
   return st;
 }
 
-// 16 values per thread up to 1024 (16-bit) or 2048 (f32) columns, 32 beyond.
-template <typename T, bool kJoin, typename F> vs_status pick(vs_ctx* ctx, const F& f, bool* taken) {
-  constexpr uint32_t V = 16 / sizeof(T), S = 16 / V, L = std::is_same<F, NormFwd>::value ? VAR_FK * 8 / V : VAR_BK * 8 / V;
-  if (f.s.cols <= (sizeof(T) == 2 ? 1024u : 2048u)) return run<T, S, kJoin>(ctx, f, taken);
-  return run<T, L, kJoin>(ctx, f, taken);
+// Values per thread: 32 make fewer instructions per value, 16 more warps.  Forward,
+// bf16 rows of 4096: 32 values 94 %, 16 values 76 % of the copy rate; f16 rows of
+// 1030, whose ends take a warp, 47 and 61 %; joined f32 rows of 4096 42 and 68 %.
+template <typename T, bool kJoin> vs_status pick(vs_ctx* ctx, const NormFwd& f, bool* taken) {
+  constexpr int V = 16 / sizeof(T);
+  const uint32_t most = sizeof(T) == 2 ? 2047 : kJoin ? ~0u : 2048;  // columns for 16 values
+  if (f.s.cols <= most) VS_TRY((run<T, 16 / V, kJoin>(ctx, f, taken)));
+  if (!*taken) VS_TRY((run<T, 32 / V, kJoin>(ctx, f, taken)));
+  return VS_OK;
+}
+// Backward: bf16 rows of 4096, joined, 16 values 77 %, 32 values 62 %; the joined
+// f32 kernel, whose vectors need a generator call each, holds 8 where it can.
+template <typename T, bool kJoin> vs_status pick(vs_ctx* ctx, const NormBwd& f, bool* taken) {
+  constexpr int V = 16 / sizeof(T), S = 16 / V, L = 32 / V;
+  if constexpr (sizeof(T) == 4) VS_TRY((run<T, kJoin ? 2 : S, 2, kJoin>(ctx, f, taken)));
+  if (!*taken) VS_TRY((run<T, S, S, kJoin>(ctx, f, taken)));
+  if (!*taken) VS_TRY((run<T, L, L, kJoin>(ctx, f, taken)));
+  return VS_OK;
 }
 
 }  // namespace
