@@ -25,9 +25,13 @@ EPS = 1e-5
 
 
 def keep_mask(n, p, seed, offset):
-    """The definition in the header, with Python integers' exact products (numpy uint64)."""
+    return keep_mask_at(0, n, p, seed, offset)
+
+
+def keep_mask_at(first, n, p, seed, offset):
+    """The definition in the header for indices [first, first + n), first a multiple of 8, in numpy's uint64."""
     t = 65536 if p == 1 else min(65535, int(p * 65536 + 0.5))
-    g = np.arange((n + 7) // 8, dtype=np.uint64)
+    g = np.arange(first // 8, first // 8 + (n + 7) // 8, dtype=np.uint64)
     m32 = np.uint64(0xFFFFFFFF)
     s32 = np.uint64(32)
     c = [g & m32, g >> s32, np.full_like(g, offset & 0xFFFFFFFF), np.full_like(g, offset >> 32)]
@@ -376,6 +380,31 @@ def test_large_offset_rows(cuda):
     y64, m64, q64 = norm_ref(x64, 1.0, 0.0)
     o = ops.layer_norm(x, eps=EPS)
     assert float((o.y.cpu().double() - y64).abs().max()) <= 32 * 1000 * 2.0**-24 * float(q64.max()) + 1e-5
+
+
+def test_indices_past_32_bits(cuda):
+    """The last values of buffers of over 2^32 values: the mask's index and the rows' addresses are 64-bit."""
+    rows, cols = (1 << 21) + 5, 2048
+    n = rows * cols
+    x = torch.ones(rows, cols, dtype=F16, device=cuda)
+    x[-3:] = torch.linspace(-1, 1, 3 * cols, device=cuda, dtype=F16).view(3, cols)
+    first = n - 3 * cols
+    # the words of the groups that hold the last three rows, from counters over 2^29
+    keep, scale = keep_mask_at(first, 3 * cols, 0.5, 7, 9)
+    want = torch.where(keep.view(3, cols), x[-3:].cpu().double() * scale, 0.0)
+    y = ops.dropout(x, 0.5, 7, 9)
+    close(y[-3:], want, "dropout")
+    del y
+    o = ops.dropout_add_norm(x, x, None, None, 0.5, 7, 9)
+    close(o.z[-3:], want + x[-3:].cpu().double(), "z")
+    y64, m64, q64 = norm_ref(o.z[-3:].cpu().double(), 1.0, 0.0)
+    close(o.y[-3:], y64, "y")
+    close(o.mean[-3:], m64[:, 0], "mean", terms=64.0)
+    g = ops.layer_norm_bwd(o.y, o.z, None, o.mean, o.rstd)
+    assert bool(torch.isfinite(g.dx[-3:]).all())
+    t64, _, _ = norm_bwd_ref(o.y[-3:].cpu().double(), o.z[-3:].cpu().double(), 1.0, o.mean[-3:].cpu().double()[:, None],
+                             o.rstd[-3:].cpu().double()[:, None])
+    close(g.dx[-3:], t64, "dx", terms=max(1.0, float(q64.max() * y64.abs().max()) / float(t64.abs().max())))
 
 
 def test_no_rows(cuda):
