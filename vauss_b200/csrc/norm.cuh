@@ -63,6 +63,27 @@ template <int N> VSD void bulk_wait_read() { asm volatile("cp.async.bulk.wait_gr
 template <int N> VSD void bulk_wait() { asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory"); }
 VSD void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Loads and stores by shared-memory address.
+VSD uint4 lds16(uint32_t at) {
+  uint4 q;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(at));
+  return q;
+}
+VSD void sts16(uint32_t at, uint4 q) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
+}
+template <typename T> VSD float lds_value(uint32_t at) {
+  if constexpr (sizeof(T) == 4) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+  } else {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+    return to_f32(reinterpret_cast<const T&>(v));
+  }
+}
+
 // A run [begin, end) of bytes of a 16-byte aligned buffer of `total` bytes, as
 // bulk copies see it: they move the aligned pieces that cover the run, [lo, hi);
 // where the buffer's last piece is not whole, its bytes [hi, end) are copied by

@@ -67,11 +67,12 @@ template <typename T, int K> struct RowPart {
 
   VSD bool has(int k) const { return at + k * threads < vectors; }
   VSD uint32_t col(int k) const { return lead + (at + k * threads) * V; }
-  // the vectors of a row whose first value is at `row`, 16 zero bytes for those beyond it
-  VSD void load(const T* row, const void* zeros, R* t) const {
+  // the vectors of a row whose first value lies at `row` in shared memory, the 16
+  // zero bytes at `zeros` for those beyond it
+  VSD void load(uint32_t row, uint32_t zeros, R* t) const {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const uint4 q = *(has(k) ? reinterpret_cast<const uint4*>(row + col(k)) : static_cast<const uint4*>(zeros));
+      const uint4 q = lds16(has(k) ? row + col(k) * (uint32_t)sizeof(T) : zeros);
       if constexpr (WORDS == 4) {
         t[k * 4] = q.x; t[k * 4 + 1] = q.y; t[k * 4 + 2] = q.z; t[k * 4 + 3] = q.w;
       } else {
@@ -142,22 +143,20 @@ template <typename T> struct RowRing {
   const RowArgs& a;
   unsigned char* slots;
   uint64_t* full;
-  uint32_t shift;
+  uint32_t base;  // the first slot's row in shared memory, `shift` values into the slot
   uint64_t total, row_bytes, load_at;  // load_at: where the next row to be copied begins (thread 0's)
-  VSD RowRing(const RowArgs& a_, unsigned char* s, uint64_t* f, uint32_t shift_)
-      : a(a_), slots(s), full(f), shift(shift_) {
+  VSD RowRing(const RowArgs& a_, unsigned char* s, uint64_t* f, uint32_t shift)
+      : a(a_), slots(s), full(f), base(smem_u32(s) + shift * (uint32_t)sizeof(T)) {
     row_bytes = (uint64_t)a.cols * sizeof(T);
     total = a.rows * row_bytes;
     load_at = blockIdx.x * row_bytes;
   }
-  VSD T* row(uint32_t slot, uint32_t input) const {
-    return reinterpret_cast<T*>(slots + (slot * a.inputs + input) * a.slot) + shift;
-  }
+  VSD uint32_t row(uint32_t slot, uint32_t input) const { return base + (slot * a.inputs + input) * a.slot; }
   VSD void refill(uint32_t slot) {
     if (load_at < total) {
       const Span s = span_of(load_at, load_at + row_bytes, total);
       mbar_expect(&full[slot], s.bytes * a.inputs);
-      for (uint32_t k = 0; k < a.inputs; ++k) span_load(s, row(slot, k) - shift, a.in[k], &full[slot]);
+      for (uint32_t k = 0; k < a.inputs; ++k) span_load(s, slots + (slot * a.inputs + k) * a.slot, a.in[k], &full[slot]);
     }
     load_at += gridDim.x * row_bytes;
   }
@@ -170,7 +169,8 @@ template <typename T> struct RowRing {
   // unwhole 16 bytes are not copied.
   VSD float single(uint32_t slot, uint32_t input, uint64_t begin, uint32_t c) const {
     const uint64_t at = begin + c * sizeof(T);
-    return to_f32(at < (total & ~15ull) ? row(slot, input)[c] : static_cast<const T*>(a.in[input])[at / sizeof(T)]);
+    if (at >= (total & ~15ull)) return to_f32(static_cast<const T*>(a.in[input])[at / sizeof(T)]);
+    return lds_value<T>(row(slot, input) + c * (uint32_t)sizeof(T));
   }
   // After a copy that did not land in time: report it and let the others end.
   VSD void give_up(uint32_t slot, uint32_t parity, uint64_t row) const {
@@ -260,12 +260,12 @@ __global__ void __launch_bounds__(row_fwd<T, K, kJoin>()) norm_row_fwd_kernel(co
     const uint64_t i0 = begin / sizeof(T);
     float2 v[PAIRS];
     typename P::R t[PAIRS];
-    part.load(ring.row(slot, 0), &zeros, t);
+    part.load(ring.row(slot, 0), smem_u32(&zeros), t);
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) v[i] = part.value(t, i);
     if (kJoin) {
       if (d.threshold) part.drop(v, i0, d);
-      part.load(ring.row(slot, 1), &zeros, t);
+      part.load(ring.row(slot, 1), smem_u32(&zeros), t);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
         part.set(t, i, add2(v[i], part.value(t, i)));  // z, rounded as it is stored
@@ -383,11 +383,13 @@ __global__ void __launch_bounds__(row_bwd<T, K>()) norm_row_bwd_kernel(const Row
 
   const P part{tid, blockDim.x - 32 * a.ragged, place.lead, place.vectors};
   // the weights, each thread's own at places of its own
-  float4* ws = reinterpret_cast<float4*>(smem + a.stages * a.inputs * a.slot) + tid;
+  const uint32_t ws = smem_u32(smem) + a.stages * a.inputs * a.slot + tid * 16, ws_step = blockDim.x * 16;
   float2 dw[PAIRS], db[PAIRS];
   part.weights(a.w.weight, a.w.dtype, 1.0f, dw);
 #pragma unroll
-  for (int i = 0; i < PAIRS; i += 2) ws[i / 2 * blockDim.x] = make_float4(dw[i].x, dw[i].y, dw[i + 1].x, dw[i + 1].y);
+  for (int i = 0; i < PAIRS; i += 2)
+    sts16(ws + i / 2 * ws_step, make_uint4(__float_as_uint(dw[i].x), __float_as_uint(dw[i].y),
+                                           __float_as_uint(dw[i + 1].x), __float_as_uint(dw[i + 1].y)));
 #pragma unroll
   for (int i = 0; i < PAIRS; ++i) dw[i] = db[i] = both(0.0f);
   bool ok = true;
@@ -398,23 +400,24 @@ __global__ void __launch_bounds__(row_bwd<T, K>()) norm_row_bwd_kernel(const Row
     const uint64_t i0 = begin / sizeof(T);
     typename P::R t[PAIRS], res[kJoin ? PAIRS : 1];
     float2 g[PAIRS], h[PAIRS];
-    part.load(ring.row(slot, 0), &zeros, t);
+    part.load(ring.row(slot, 0), smem_u32(&zeros), t);
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) g[i] = part.value(t, i);
-    part.load(ring.row(slot, 1), &zeros, t);
+    part.load(ring.row(slot, 1), smem_u32(&zeros), t);
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) h[i] = mul2(add2(part.value(t, i), both(-m)), both(q));
     if constexpr (kJoin)
-      if (a.inputs == 3) part.load(ring.row(slot, 2), &zeros, res);
+      if (a.inputs == 3) part.load(ring.row(slot, 2), smem_u32(&zeros), res);
     float2 s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
     for (int i = 0; i < PAIRS; i += 2) {  // g is zero for values that are not the row's
-      const float4 w = ws[i / 2 * blockDim.x];
+      const uint4 w = lds16(ws + i / 2 * ws_step);
 #pragma unroll
       for (int j = i; j < i + 2; ++j) {
         dw[j] = fma2(g[j], h[j], dw[j]);
         db[j] = add2(db[j], g[j]);
-        g[j] = mul2(g[j], j > i ? make_float2(w.z, w.w) : make_float2(w.x, w.y));
+        g[j] = mul2(g[j], j > i ? make_float2(__uint_as_float(w.z), __uint_as_float(w.w))
+                                     : make_float2(__uint_as_float(w.x), __uint_as_float(w.y)));
         s1 = add2(s1, g[j]);
         s2 = fma2(g[j], h[j], s2);
       }
