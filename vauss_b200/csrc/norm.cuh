@@ -365,6 +365,17 @@ VSD uint32_t keep_bits(const Words& w, uint32_t limit) {
   return bits;
 }
 
+// The numbers of a run of four or eight values from index e, a multiple of the
+// run: the first words, where a run of four is a group's second half.
+template <int VEC> VSD Words run_words(const Dropout& d, uint64_t e) {
+  Words w = philox(d, e >> 3);
+  if (VEC == 4 && (e & 4u)) {
+    w.w[0] = w.w[2];
+    w.w[1] = w.w[3];
+  }
+  return w;
+}
+
 // Dropout of a thread's values, decided one run at a time.
 template <typename P> VSD void drop_runs(const P& part, float2* v, uint64_t i0, const Dropout& d) {
   constexpr int VEC = P::E / P::RUNS;
@@ -377,12 +388,9 @@ template <typename P> VSD void drop_runs(const P& part, float2* v, uint64_t i0, 
     if constexpr (VEC == 1) {
       f[k] = keep_at(d, e) ? f[k] : 0.0f;
     } else {
-      const Words words = philox(d, e >> 3);
+      const Words words = run_words<VEC>(d, e);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const bool kept = VEC == 8 ? keeps(words, j, d.limit) : e & 4u ? keeps(words, j + 4, d.limit) : keeps(words, j, d.limit);
-        f[k * VEC + j] = kept ? f[k * VEC + j] : 0.0f;
-      }
+      for (int j = 0; j < VEC; ++j) f[k * VEC + j] = keeps(words, j, d.limit) ? f[k * VEC + j] : 0.0f;
     }
   }
 }

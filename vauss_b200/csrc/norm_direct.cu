@@ -87,6 +87,8 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
 template <typename T, int VEC, int K, bool kJoin, bool kCta>
 __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS * 32)
     norm_direct_bwd_kernel(const NormBwd a, uint32_t log_lanes, const __grid_constant__ Dropout d, float* partial) {
+  // One CTA's column sums are the weight gradients; several leave theirs in `partial`.
+  const bool alone = gridDim.x == 1;
   using P = Part<T, VEC, K, true>;
   constexpr int PAIRS = P::PAIRS;
   __shared__ __align__(16) float red[2][2][kCta ? NORM_MAX_WARPS : 4];
@@ -100,7 +102,7 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
   float2 w[PAIRS], dw[PAIRS], db[PAIRS];
 #pragma unroll
   for (int i = 0; i < PAIRS; ++i) dw[i] = db[i] = both(0.0f);
-  launch_next();
+  if (!alone) launch_next();
   bool ready = false;
   uint32_t half = 0;
   if (kCta) {
@@ -170,15 +172,33 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
       part.store(static_cast<T*>(a.dx) + r * a.s.cols, t);
     }
   }
-  if (!partial) return;
+  if (!partial && !(alone && (a.dweight || a.dbias))) return;
   float* out = partial + (uint64_t)blockIdx.x * 2 * a.s.cols;
+  auto leave = [&](uint32_t which, uint32_t c, float v) {
+    if (!alone) out[which * a.s.cols + c] = v;
+    else if (void* to = which ? a.dbias : a.dweight) store_as(to, a.wdtype, c, v);
+  };
   if (kCta) {
+    // whole 16-byte pieces where they fit
+    float* to0 = alone ? static_cast<float*>(a.dweight) : out;
+    float* to1 = alone ? static_cast<float*>(a.dbias) : out + a.s.cols;
+    if (VEC % 4 == 0 && (!alone || (a.wdtype == VS_F32 && (((uintptr_t)to0 | (uintptr_t)to1) & 15u) == 0))) {
+#pragma unroll
+      for (int i = 0; i + 1 < PAIRS; i += 2) {
+        const int k = 2 * i / VEC;
+        if (!part.has(k)) continue;
+        const uint32_t c = part.col(k) + 2 * i % VEC;
+        if (to0) *reinterpret_cast<float4*>(to0 + c) = make_float4(dw[i].x, dw[i].y, dw[i + 1].x, dw[i + 1].y);
+        if (to1) *reinterpret_cast<float4*>(to1 + c) = make_float4(db[i].x, db[i].y, db[i + 1].x, db[i + 1].y);
+      }
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < P::E; ++e) {
       if (!part.has(e / VEC)) continue;
       const uint32_t c = part.col(e / VEC) + e % VEC;
-      out[c] = (&dw[e / 2].x)[e % 2];
-      out[a.s.cols + c] = (&db[e / 2].x)[e % 2];
+      leave(0, c, (&dw[e / 2].x)[e % 2]);
+      leave(1, c, (&db[e / 2].x)[e % 2]);
     }
     return;
   }
@@ -201,7 +221,7 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
   for (uint32_t c = threadIdx.x; c < 2 * a.s.cols; c += DIRECT_WARPS * 32) {
     float v = sums[c];
     for (uint32_t k = 1; k < DIRECT_WARPS; ++k) v += sums[k * 2 * a.s.cols + c];
-    out[c] = v;
+    leave(c >= a.s.cols, c >= a.s.cols ? c - a.s.cols : c, v);
   }
 }
 
@@ -209,7 +229,9 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
 struct Shape {
   uint32_t grid, threads, log_lanes;
 };
-template <int VEC, int K, bool kCta> Shape shape_of(const NormShape& s) {
+// `alone`: up to this many rounds of rows stay on one CTA (a second launch costs
+// about 3 us of the host and of the GPU, a round about 1 us).
+template <int VEC, int K, bool kCta> Shape shape_of(const NormShape& s, uint32_t alone) {
   const uint32_t chunks = (s.cols + VEC - 1) / VEC;
   Shape l{0, DIRECT_WARPS * 32, 0};
   uint64_t most = s.rows;
@@ -221,19 +243,19 @@ template <int VEC, int K, bool kCta> Shape shape_of(const NormShape& s) {
     most = (s.rows + rows - 1) / rows;
   }
   const uint64_t room = (uint64_t)B200_SMS * (l.threads >= 512 ? 1 : 512 / l.threads);
-  l.grid = (uint32_t)(room < most ? room : most);
+  l.grid = most <= alone ? 1 : (uint32_t)(room < most ? room : most);
   return l;
 }
 
 template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status launch(vs_ctx* ctx, const NormFwd& f) {
-  const Shape l = shape_of<VEC, K, kCta>(f.s);
+  const Shape l = shape_of<VEC, K, kCta>(f.s, 1);
   norm_direct_fwd_kernel<T, VEC, K, kJoin, kCta><<<l.grid, l.threads, 0, ctx->stream>>>(f, l.log_lanes, f.d);
   ++ctx->launches;
   return vs_cuda(ctx, cudaGetLastError(), "norm launch");
 }
 template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status launch(vs_ctx* ctx, const NormBwd& f) {
-  const Shape l = shape_of<VEC, K, kCta>(f.s);
-  const bool want = f.dweight || f.dbias;
+  const Shape l = shape_of<VEC, K, kCta>(f.s, 4);
+  const bool want = (f.dweight || f.dbias) && l.grid > 1;
   NormScratch scratch;
   if (want) VS_TRY(norm_scratch_begin(ctx, (size_t)l.grid * 2 * f.s.cols, &scratch));
   const size_t smem = kCta ? 0 : DIRECT_WARPS * 2 * f.s.cols * 4;

@@ -128,12 +128,9 @@ template <typename T, int K> struct RowPart {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const uint64_t e = i0 + col(k);
-      const Words words = philox(d, e >> 3);
+      const Words words = run_words<V>(d, e);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const bool kept = V == 8 ? keeps(words, j, d.limit) : e & 4u ? keeps(words, j + 4, d.limit) : keeps(words, j, d.limit);
-        f[k * V + j] = kept ? f[k * V + j] : 0.0f;
-      }
+      for (int j = 0; j < V; ++j) f[k * V + j] = keeps(words, j, d.limit) ? f[k * V + j] : 0.0f;
     }
   }
 };
@@ -447,6 +444,17 @@ __global__ void __launch_bounds__(row_bwd<T, K>()) norm_row_bwd_kernel(const Row
   }
   if (!ok && tid == 0) ring.give_up(slot, parity, row);
   if (!out) return;
+  if (a.cols % 4 == 0 && place.lead % 4 == 0) {  // whole 16-byte pieces: single values would cost the L2 a write each
+#pragma unroll
+    for (int i = 0; i < PAIRS; i += 2) {
+      const int k = 2 * i / P::V;
+      if (!part.has(k)) continue;
+      float* to = out + part.col(k) + 2 * i % P::V;
+      *reinterpret_cast<float4*>(to) = make_float4(dw[i].x, dw[i].y, dw[i + 1].x, dw[i + 1].y);
+      *reinterpret_cast<float4*>(to + a.cols) = make_float4(db[i].x, db[i].y, db[i + 1].x, db[i + 1].y);
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < P::E; ++e) {
     if (!part.has(e / P::V)) continue;
