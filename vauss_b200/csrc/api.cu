@@ -137,6 +137,7 @@ VS_API void vs_ctx_destroy(vs_ctx* ctx) {
   vs_release(ctx, ctx->misc);
   vs_release(ctx, ctx->io_stage);
   vs_release(ctx, ctx->vjp_rows);
+  if (ctx->norm_streams > 1) cudaDeviceSynchronize();  // other streams' buffers
   for (DevBuf& b : ctx->norm_sums) vs_release(ctx, b);
   cudaStreamSynchronize(ctx->stream);
   if (ctx->d_err) cudaFree(ctx->d_err);

@@ -324,9 +324,9 @@ vs_status norm_join_partials(vs_ctx* ctx, uint32_t cols, uint32_t strips, const 
   return VS_OK;
 }
 
-// Calls on one stream follow one another, so each stream has one buffer.  A call
-// being captured into a graph gets memory of the graph's own, since the graph may
-// run beside other calls.
+// Calls on one stream follow one another, so each stream has one buffer (the
+// first NORM_STREAMS that call).  A call being captured into a graph gets memory of
+// the graph's own, since the graph may run beside other calls.
 vs_status norm_scratch_begin(vs_ctx* ctx, size_t floats, NormScratch* out) {
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   VS_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
@@ -334,19 +334,13 @@ vs_status norm_scratch_begin(vs_ctx* ctx, size_t floats, NormScratch* out) {
   if (out->pooled) return vs_cuda(ctx, cudaMallocAsync((void**)&out->p, floats * 4, ctx->stream), "norm scratch");
   unsigned long long id = 0;
   VS_CUDA(ctx, cudaStreamGetId(ctx->stream, &id));
-  const uint32_t seen = ctx->norm_streams < vs_ctx::NORM_STREAMS ? ctx->norm_streams : vs_ctx::NORM_STREAMS;
   uint32_t k = 0;
-  while (k < seen && ctx->norm_stream[k] != id) ++k;
-  if (k == seen) {
-    k = ctx->norm_streams % vs_ctx::NORM_STREAMS;
-    DevBuf& b = ctx->norm_sums[k];
-    if (b.ptr) {  // another stream's: wait for whatever still uses it
-      VS_CUDA(ctx, cudaDeviceSynchronize());
-      vs_release(ctx, b);
-    }
-    ctx->norm_stream[k] = id;
-    ++ctx->norm_streams;
+  while (k < ctx->norm_streams && ctx->norm_stream[k] != id) ++k;
+  if (k == vs_ctx::NORM_STREAMS) {  // more streams than buffers: memory of the call's own
+    out->pooled = true;
+    return vs_cuda(ctx, cudaMallocAsync((void**)&out->p, floats * 4, ctx->stream), "norm scratch");
   }
+  if (k == ctx->norm_streams) ctx->norm_stream[ctx->norm_streams++] = id;
   VS_TRY(vs_ensure(ctx, ctx->norm_sums[k], floats * 4));
   out->p = static_cast<float*>(ctx->norm_sums[k].ptr);
   return VS_OK;

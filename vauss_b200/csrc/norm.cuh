@@ -38,10 +38,18 @@ VSD bool mbar_try(uint64_t* b, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Waits for a copy to land; false after about a second without it.
-constexpr uint32_t COPY_SPIN_LIMIT = 1u << 22;
+// Waits for a copy to land; false after a second without it.
+constexpr uint64_t COPY_WAIT_NS = 1000000000ull;
+constexpr uint32_t COPY_SPIN_LIMIT = 1u << 26;  // backstop on the iteration count
+VSD uint64_t copy_clock_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
 VSD bool mbar_wait(uint64_t* b, uint32_t parity) {
-  for (uint32_t spins = 0; spins < COPY_SPIN_LIMIT; ++spins)
+  if (mbar_try(b, parity)) return true;
+  const uint64_t t0 = copy_clock_ns();
+  for (uint32_t spins = 0; spins < COPY_SPIN_LIMIT && copy_clock_ns() - t0 < COPY_WAIT_NS; ++spins)
     if (mbar_try(b, parity)) return true;
   return false;
 }

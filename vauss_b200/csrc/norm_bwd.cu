@@ -1,5 +1,5 @@
 // Streaming backward layer norm, alone or joined with the residual sum and the
-// dropout, for contiguous rows; the warps and their rings are those of the
+// dropout, for short contiguous rows; the warps and their rings are those of the
 // forward (norm_fwd.cu).
 //
 // A lane's columns are the same for every row, so the weight's and the bias's
@@ -195,11 +195,9 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
     } else {
       proxy_fence();
       __syncwarp();
-      {
-        const Span s = span_at(begin);
-        span_store<T>(s, gbuf, a.dx, lane);
-        if (kJoin) span_store<T>(s, zbuf, a.dresidual, lane);
-      }
+      const Span s = span_at(begin);
+      span_store<T>(s, gbuf, a.dx, lane);
+      if (kJoin) span_store<T>(s, zbuf, a.dresidual, lane);
       if (lane == 0) {
         bulk_commit();
         bulk_wait_read<1>();

@@ -14,7 +14,7 @@ namespace {
 
 using namespace vs;
 
-// CTAs of the warp warps on an SM, and the bytes of one slot and input.  Two
+// CTAs on an SM, and the bytes of one slot and input.  Two
 // things meet here.  Every byte in flight beyond what hides the latency only
 // queues in front of the DRAM and costs throughput (f32 rows of 256, two slots
 // of 2 KB a warp: 12 warps 97 % of the copy rate, 16 warps 86 %; joined, two
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K, kJoin>()
   const uint32_t tile_bytes = a.tile_rows * a.cols * (uint32_t)sizeof(T);
   const uint64_t total = a.rows * a.cols * sizeof(T), step_bytes = step * tile_bytes;
   uint64_t begin = first * tile_bytes;  // of the tile at hand
-  uint64_t load_at = begin;             // of the tile to be copied next (thread 0's)
+  uint64_t load_at = begin;             // of the tile to be copied next (lane 0's)
   auto span_at = [&](uint64_t b) {
     const uint64_t end = total - b < tile_bytes ? total : b + tile_bytes;
     return kDirect ? Span{b, end, b, (uint32_t)(end - b), 0} : span_of(b, end, total);
@@ -164,11 +164,9 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K, kJoin>()
     } else {
       proxy_fence();
       __syncwarp();
-      {
-        const Span s = span_at(begin);
-        span_store<T>(s, in, a.y, lane);
-        if (kJoin) span_store<T>(s, res, a.z, lane);
-      }
+      const Span s = span_at(begin);
+      span_store<T>(s, in, a.y, lane);
+      if (kJoin) span_store<T>(s, res, a.z, lane);
       if (lane == 0) {
         bulk_commit();
         // the slot before this one has been read out by now: it is filled again
@@ -220,10 +218,10 @@ template <typename T, int VEC, int K, bool kJoin> vs_status run_kernel(vs_ctx* c
   a.tile_rows = (passes < 1 ? 1 : passes) * per_pass;
   a.slot = (a.tile_rows * row_bytes + 30u) & ~15u;
   a.bits = kJoin && VEC != 8 ? (a.tile_rows * a.cols / 8 + 2 + 15) & ~15u : 0;
-  // Two slots: one being worked on, one on its way (a third one costs rows of
-  // 4096 bf16 13 %, see above), and a third for slots that are written back; fewer
-  // CTAs where the SM's shared memory does not hold theirs.  A slot that is
-  // written back needs at least another beside it.
+  // Two slots: one being worked on, one on its way, and a third where slots are
+  // written back (59 f32 columns: two 69 %, three 89 %); fewer CTAs where the SM's
+  // shared memory does not hold theirs.  A slot that is written back needs at
+  // least another beside it.
   constexpr uint32_t least = Part<T, VEC, K>::kVector ? 1 : 2;
   auto bytes = [&](uint32_t stages) { return NORM_WARPS * (stages * NIN * a.slot + a.bits) + NORM_PADDING; };
   auto room = [&] { return NORM_MAX_SMEM / per_sm - 1024; };

@@ -27,12 +27,12 @@ struct vs_ctx {
   DevBuf sort_keys, sort_vals, sort_hist, scan_sums, misc;
   DevBuf io_stage;  // checkpoint I/O chunks (two halves)
   DevBuf vjp_rows;  // per-visible-splat VJP rows of the single-view Q8 step
-  // layer norm's column sums per CTA, for each stream that called (by the ids
-  // that cudaStreamGetId gives, which are never used twice)
+  // layer norm's column sums per CTA, for each of the first streams that called (by
+  // the ids that cudaStreamGetId gives, which are never used twice)
   static constexpr uint32_t NORM_STREAMS = 16;
   DevBuf norm_sums[NORM_STREAMS];
   unsigned long long norm_stream[NORM_STREAMS] = {};
-  uint32_t norm_streams = 0;  // streams seen; the buffer of the 17th replaces the first one's, and so on
+  uint32_t norm_streams = 0;
 };
 
 struct vs_frame {

@@ -503,7 +503,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     wdtype = _weight_dtype(weight, bias, x)
     if out is None:
         out = LayerNormOutput(torch.empty(shape, dtype=x.dtype, device=x.device),
-                              *torch.empty(2, rows, dtype=_F32, device=x.device).unbind())
+                              torch.empty(rows, dtype=_F32, device=x.device),
+                              torch.empty(rows, dtype=_F32, device=x.device))
     args = (rows, cols, dtype, _DTYPES[wdtype], x.data_ptr(), _row_stride(x), _weight(weight, wdtype, cols, device),
             _weight(bias, wdtype, cols, device), eps, _output(out.y, shape, x.dtype, device),
             _stat(out.mean, rows, device), _stat(out.rstd, rows, device))
@@ -570,7 +571,8 @@ def dropout_add_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
     if out is None:
         out = DropoutAddNormOutput(torch.empty(shape, dtype=x.dtype, device=x.device),
                                    torch.empty(shape, dtype=x.dtype, device=x.device),
-                                   *torch.empty(2, rows, dtype=_F32, device=x.device).unbind())
+                                   torch.empty(rows, dtype=_F32, device=x.device),
+                                   torch.empty(rows, dtype=_F32, device=x.device))
     args = (rows, cols, dtype, _DTYPES[wdtype], x.data_ptr(), _row_stride(x), residual.data_ptr(),
             _row_stride(residual), _weight(weight, wdtype, cols, device), _weight(bias, wdtype, cols, device), p,
             seed & _U64, offset & _U64, eps, _output(out.y, shape, x.dtype, device),
