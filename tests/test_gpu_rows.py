@@ -445,6 +445,43 @@ def test_on_another_stream(cuda):
         assert torch.equal(g.dx, ref.dx) and torch.equal(g.dweight, ref.dweight) and torch.equal(g.dbias, ref.dbias)
 
 
+def test_many_streams(cuda):
+    """More streams than the ctx keeps buffers for, each with calls of growing size, all in flight at once."""
+    dy, _ = rows_of(cuda, 3000, 40, BF16, 1)
+    x, _ = rows_of(cuda, 3000, 40, BF16, 2)
+    w, _, _, _ = weights_of(cuda, 40, F32, 3)
+    o = ops.layer_norm(x, w)
+    sizes = (5, 200, 1000, 3000)
+    want = [ops.layer_norm_bwd(dy[:n], x[:n], w, o.mean[:n], o.rstd[:n]) for n in sizes]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(20)]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append([ops.layer_norm_bwd(dy[:n], x[:n], w, o.mean[:n], o.rstd[:n]) for n in sizes])
+    torch.cuda.synchronize()
+    for per_stream in got:
+        for g, ref in zip(per_stream, want):
+            assert torch.equal(g.dweight, ref.dweight) and torch.equal(g.dbias, ref.dbias) and torch.equal(g.dx, ref.dx)
+
+
+def test_statistics_at_any_address(cuda):
+    """mean and rstd one element past a 16-byte boundary: another kernel, the same values within rounding."""
+    rows, cols = 60_000, 64
+    dy, _ = rows_of(cuda, rows, cols, F32, 1)
+    x, _ = rows_of(cuda, rows, cols, F32, 2)
+    w, _, _, _ = weights_of(cuda, cols, F32, 3)
+    o = ops.layer_norm(x, w)
+    want = ops.layer_norm_bwd(dy, x, w, o.mean, o.rstd)
+    off = torch.empty(2, rows + 1, device=cuda)
+    off[0, 1:], off[1, 1:] = o.mean, o.rstd
+    got = ops.layer_norm_bwd(dy, x, w, off[0, 1:], off[1, 1:])
+    # the row sums are taken in another order: 2 * 64 * 2^-24 of values of order one, times rstd
+    tol = 2 * 64 * 2.0**-24 * float(o.rstd.max()) * 8
+    assert float((got.dx - want.dx).abs().max()) <= tol
+    assert float((got.dweight - want.dweight).abs().max()) <= F32_ERR * float((dy.abs() * 4).sum(0).max())
+
+
 def test_in_a_graph(cuda):
     x, _ = rows_of(cuda, 512, 80, BF16, 1)
     r, _ = rows_of(cuda, 512, 80, BF16, 2)

@@ -328,25 +328,34 @@ vs_status norm_join_partials(vs_ctx* ctx, uint32_t cols, uint32_t strips, const 
 // first NORM_STREAMS that call).  A call being captured into a graph gets memory of
 // the graph's own, since the graph may run beside other calls.
 vs_status norm_scratch_begin(vs_ctx* ctx, size_t floats, NormScratch* out) {
+  const size_t bytes = 16 + floats * 4;  // the ticket, then the floats
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  VS_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
-  out->pooled = capture != cudaStreamCaptureStatusNone;
-  if (out->pooled) return vs_cuda(ctx, cudaMallocAsync((void**)&out->p, floats * 4, ctx->stream), "norm scratch");
   unsigned long long id = 0;
-  VS_CUDA(ctx, cudaStreamGetId(ctx->stream, &id));
+  VS_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &capture));
   uint32_t k = 0;
-  while (k < ctx->norm_streams && ctx->norm_stream[k] != id) ++k;
-  if (k == vs_ctx::NORM_STREAMS) {  // more streams than buffers: memory of the call's own
-    out->pooled = true;
-    return vs_cuda(ctx, cudaMallocAsync((void**)&out->p, floats * 4, ctx->stream), "norm scratch");
+  out->pooled = capture != cudaStreamCaptureStatusNone;
+  if (!out->pooled) {
+    VS_CUDA(ctx, cudaStreamGetId(ctx->stream, &id));  // not while capturing: it ends the capture
+    while (k < ctx->norm_streams && ctx->norm_stream[k] != id) ++k;
+    out->pooled = k == vs_ctx::NORM_STREAMS;
   }
-  if (k == ctx->norm_streams) ctx->norm_stream[ctx->norm_streams++] = id;
-  VS_TRY(vs_ensure(ctx, ctx->norm_sums[k], floats * 4));
-  out->p = static_cast<float*>(ctx->norm_sums[k].ptr);
-  return VS_OK;
+  void* at = nullptr;
+  bool fresh = true;
+  if (out->pooled) {
+    VS_CUDA(ctx, cudaMallocAsync(&at, bytes, ctx->stream));
+  } else {
+    if (k == ctx->norm_streams) ctx->norm_stream[ctx->norm_streams++] = id;
+    const size_t before = ctx->norm_sums[k].bytes;
+    VS_TRY(vs_ensure(ctx, ctx->norm_sums[k], bytes));
+    at = ctx->norm_sums[k].ptr;
+    fresh = ctx->norm_sums[k].bytes != before;
+  }
+  out->ticket = static_cast<uint32_t*>(at);
+  out->p = static_cast<float*>(at) + 4;
+  return fresh ? vs_cuda(ctx, cudaMemsetAsync(at, 0, 16, ctx->stream), "norm scratch") : VS_OK;
 }
 vs_status norm_scratch_end(vs_ctx* ctx, const NormScratch& scratch) {
-  return scratch.pooled ? vs_cuda(ctx, cudaFreeAsync(scratch.p, ctx->stream), "norm scratch") : VS_OK;
+  return scratch.pooled ? vs_cuda(ctx, cudaFreeAsync(scratch.ticket, ctx->stream), "norm scratch") : VS_OK;
 }
 
 extern "C" {

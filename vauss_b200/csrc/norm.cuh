@@ -533,10 +533,12 @@ vs_status norm_tile_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBw
 // The direct kernels take rows of any stride and alignment, up to a width.
 vs_status norm_direct_forward(vs_ctx* ctx, int32_t dtype, bool join, const NormFwd& a, bool* taken);
 vs_status norm_direct_backward(vs_ctx* ctx, int32_t dtype, bool join, const NormBwd& a, bool* taken);
-// `floats` floats of scratch for one call, on the ctx stream; end it after the
-// call's last launch.
+// `floats` floats of scratch for one call, 16-byte aligned, on the ctx stream; end
+// it after the call's last launch.  The word at `ticket` is zero before the call and
+// has to be zero after it.
 struct NormScratch {
   float* p = nullptr;
+  uint32_t* ticket = nullptr;
   bool pooled = false;
 };
 vs_status norm_scratch_begin(vs_ctx* ctx, size_t floats, NormScratch* out);

@@ -11,12 +11,17 @@ namespace {
 
 using namespace vs;
 
-constexpr uint32_t DIRECT_WARPS = 4;
+// Warps of a CTA whose warps work on their own.  The backward's leave their sums
+// together, so that few CTAs' sums are left to be added.
+constexpr uint32_t FWD_WARPS = 4, BWD_WARPS = 16;
 // threads of a CTA by the values each one holds
 constexpr uint32_t direct_threads(int elems) { return elems > 8 ? 512 : 1024; }
+// Sums of up to this many floats are added by the last CTA to leave its own, which
+// saves the launch of another kernel (20k x 64 f16: 3.4 us of the host's time).
+constexpr uint32_t FOLD_FLOATS = 65536, FOLD_GROUPS = 32;
 
 template <typename T, int VEC, int K, bool kJoin, bool kCta>
-__global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS * 32)
+__global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : FWD_WARPS * 32)
     norm_direct_fwd_kernel(const NormFwd a, uint32_t log_lanes, const __grid_constant__ Dropout d) {
   using P = Part<T, VEC, K, true>;
   constexpr int PAIRS = P::PAIRS;
@@ -25,7 +30,7 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
   const uint32_t lanes = kCta ? blockDim.x : 1u << log_lanes;
   const uint32_t sub = kCta ? 0 : id >> log_lanes, per_pass = kCta ? 1 : 32u >> log_lanes;
   const P part(kCta ? id : id & (lanes - 1), lanes, sub, a.s.cols);
-  const uint64_t step = (uint64_t)gridDim.x * (kCta ? 1 : DIRECT_WARPS) * per_pass;
+  const uint64_t step = (uint64_t)gridDim.x * (kCta ? 1 : FWD_WARPS) * per_pass;
   const float n = (float)a.s.cols, inv = 1.0f / n;
   float2 w[PAIRS], b[PAIRS];
   bool ready = false;
@@ -33,7 +38,7 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
     for (uint32_t k = id; k < 2 * NORM_MAX_WARPS; k += blockDim.x) (&red[0][0])[k] = 0.0f;
     __syncthreads();
   }
-  for (uint64_t r0 = ((uint64_t)blockIdx.x * (kCta ? 1 : DIRECT_WARPS) + (kCta ? 0 : threadIdx.x >> 5)) * per_pass;
+  for (uint64_t r0 = ((uint64_t)blockIdx.x * (kCta ? 1 : FWD_WARPS) + (kCta ? 0 : threadIdx.x >> 5)) * per_pass;
        r0 < a.s.rows; r0 += step) {
     // a lane beyond the last row computes that row and writes nothing
     const bool live = r0 + sub < a.s.rows;
@@ -85,9 +90,11 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
 }
 
 template <typename T, int VEC, int K, bool kJoin, bool kCta>
-__global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS * 32)
-    norm_direct_bwd_kernel(const NormBwd a, uint32_t log_lanes, const __grid_constant__ Dropout d, float* partial) {
-  // One CTA's column sums are the weight gradients; several leave theirs in `partial`.
+__global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : BWD_WARPS * 32)
+    norm_direct_bwd_kernel(const NormBwd a, uint32_t log_lanes, const __grid_constant__ Dropout d, float* partial,
+                           uint32_t* ticket) {
+  // One CTA's column sums are the weight gradients; several leave theirs in
+  // `partial`, and with a `ticket` the last one adds them up.
   const bool alone = gridDim.x == 1;
   using P = Part<T, VEC, K, true>;
   constexpr int PAIRS = P::PAIRS;
@@ -97,19 +104,19 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
   const uint32_t lanes = kCta ? blockDim.x : 1u << log_lanes;
   const uint32_t sub = kCta ? 0 : id >> log_lanes, per_pass = kCta ? 1 : 32u >> log_lanes;
   const P part(kCta ? id : id & (lanes - 1), lanes, sub, a.s.cols);
-  const uint64_t step = (uint64_t)gridDim.x * (kCta ? 1 : DIRECT_WARPS) * per_pass;
+  const uint64_t step = (uint64_t)gridDim.x * (kCta ? 1 : BWD_WARPS) * per_pass;
   const float n = (float)a.s.cols, inv = 1.0f / n;
   float2 w[PAIRS], dw[PAIRS], db[PAIRS];
 #pragma unroll
   for (int i = 0; i < PAIRS; ++i) dw[i] = db[i] = both(0.0f);
-  if (!alone) launch_next();
+  if (!alone && !ticket) launch_next();
   bool ready = false;
   uint32_t half = 0;
   if (kCta) {
     for (uint32_t k = id; k < 4 * NORM_MAX_WARPS; k += blockDim.x) (&red[0][0][0])[k] = 0.0f;
     __syncthreads();
   }
-  for (uint64_t r0 = ((uint64_t)blockIdx.x * (kCta ? 1 : DIRECT_WARPS) + (kCta ? 0 : threadIdx.x >> 5)) * per_pass;
+  for (uint64_t r0 = ((uint64_t)blockIdx.x * (kCta ? 1 : BWD_WARPS) + (kCta ? 0 : threadIdx.x >> 5)) * per_pass;
        r0 < a.s.rows; r0 += step) {
     const bool live = r0 + sub < a.s.rows;
     const uint64_t r = live ? r0 + sub : a.s.rows - 1;
@@ -218,11 +225,44 @@ __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : DIRECT_WARPS 
     __syncwarp();
   }
   __syncthreads();
-  for (uint32_t c = threadIdx.x; c < 2 * a.s.cols; c += DIRECT_WARPS * 32) {
+  const uint32_t pieces = (2 * a.s.cols + 3) / 4;  // of 16 bytes, in which the last CTA reads
+  if (ticket) out = partial + (uint64_t)blockIdx.x * 4 * pieces;
+  for (uint32_t c = threadIdx.x; c < 2 * a.s.cols; c += BWD_WARPS * 32) {
     float v = sums[c];
-    for (uint32_t k = 1; k < DIRECT_WARPS; ++k) v += sums[k * 2 * a.s.cols + c];
-    leave(c >= a.s.cols, c >= a.s.cols ? c - a.s.cols : c, v);
+    for (uint32_t k = 1; k < BWD_WARPS; ++k) v += sums[k * 2 * a.s.cols + c];
+    if (ticket) out[c] = v;
+    else leave(c >= a.s.cols, c >= a.s.cols ? c - a.s.cols : c, v);
   }
+  if (!ticket) return;
+  __shared__ bool last;
+  __threadfence();  // the sums are written before the ticket is drawn
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  // groups of threads take every groups-th CTA's sums, 16 bytes a thread; then the
+  // groups' sums are added in order
+  const uint32_t fit = BWD_WARPS * 32 / pieces, groups = fit < FOLD_GROUPS ? fit : FOLD_GROUPS;
+  const uint32_t group = threadIdx.x / pieces, piece = threadIdx.x % pieces;
+  if (group < groups) {
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float4* from = reinterpret_cast<const float4*>(partial) + piece;
+#pragma unroll 4
+    for (uint32_t k = group; k < gridDim.x; k += groups) {
+      const float4 v = __ldcg(from + (uint64_t)k * pieces);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    reinterpret_cast<float4*>(sums)[group * pieces + piece] = s;
+  }
+  __syncthreads();
+  for (uint32_t c = threadIdx.x; c < 2 * a.s.cols; c += BWD_WARPS * 32) {
+    float v = sums[c];
+    for (uint32_t k = 1; k < groups; ++k) v += sums[k * 4 * pieces + c];
+    const uint32_t which = c >= a.s.cols;
+    if (void* to = which ? a.dbias : a.dweight) store_as(to, a.wdtype, which ? c - a.s.cols : c, v);
+  }
+  if (threadIdx.x == 0) *ticket = 0;  // for the next call
 }
 
 // The launch of one shape: a CTA per row of `threads`, or warps.
@@ -231,15 +271,15 @@ struct Shape {
 };
 // `alone`: up to this many rounds of rows stay on one CTA (a second launch costs
 // about 3 us of the host and of the GPU, a round about 1 us).
-template <int VEC, int K, bool kCta> Shape shape_of(const NormShape& s, uint32_t alone) {
+template <int VEC, int K, bool kCta> Shape shape_of(const NormShape& s, uint32_t warps, uint32_t alone) {
   const uint32_t chunks = (s.cols + VEC - 1) / VEC;
-  Shape l{0, DIRECT_WARPS * 32, 0};
+  Shape l{0, warps * 32, 0};
   uint64_t most = s.rows;
   if (kCta) {
     l.threads = ((chunks + K - 1) / K + 31) & ~31u;
   } else {
     while ((1u << l.log_lanes) * K < chunks) ++l.log_lanes;
-    const uint32_t rows = DIRECT_WARPS * (32u >> l.log_lanes);
+    const uint32_t rows = warps * (32u >> l.log_lanes);
     most = (s.rows + rows - 1) / rows;
   }
   const uint64_t room = (uint64_t)B200_SMS * (l.threads >= 512 ? 1 : 512 / l.threads);
@@ -248,23 +288,25 @@ template <int VEC, int K, bool kCta> Shape shape_of(const NormShape& s, uint32_t
 }
 
 template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status launch(vs_ctx* ctx, const NormFwd& f) {
-  const Shape l = shape_of<VEC, K, kCta>(f.s, 1);
+  const Shape l = shape_of<VEC, K, kCta>(f.s, FWD_WARPS, 1);
   norm_direct_fwd_kernel<T, VEC, K, kJoin, kCta><<<l.grid, l.threads, 0, ctx->stream>>>(f, l.log_lanes, f.d);
   ++ctx->launches;
   return vs_cuda(ctx, cudaGetLastError(), "norm launch");
 }
 template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status launch(vs_ctx* ctx, const NormBwd& f) {
-  const Shape l = shape_of<VEC, K, kCta>(f.s, 4);
+  const Shape l = shape_of<VEC, K, kCta>(f.s, BWD_WARPS, 4);
   const bool want = (f.dweight || f.dbias) && l.grid > 1;
   NormScratch scratch;
-  if (want) VS_TRY(norm_scratch_begin(ctx, (size_t)l.grid * 2 * f.s.cols, &scratch));
-  const size_t smem = kCta ? 0 : DIRECT_WARPS * 2 * f.s.cols * 4;
-  norm_direct_bwd_kernel<T, VEC, K, kJoin, kCta><<<l.grid, l.threads, smem, ctx->stream>>>(f, l.log_lanes, f.d,
-                                                                                         scratch.p);
+  if (want) VS_TRY(norm_scratch_begin(ctx, (size_t)l.grid * (2 * f.s.cols + 3), &scratch));
+  const bool fold = want && !kCta && l.grid * 2 * f.s.cols <= FOLD_FLOATS;
+  size_t smem = kCta ? 0 : BWD_WARPS * 2 * f.s.cols * 4;
+  if (fold && smem < BWD_WARPS * 32 * 16) smem = BWD_WARPS * 32 * 16;
+  norm_direct_bwd_kernel<T, VEC, K, kJoin, kCta><<<l.grid, l.threads, smem, ctx->stream>>>(
+      f, l.log_lanes, f.d, scratch.p, fold ? scratch.ticket : nullptr);
   ++ctx->launches;
   vs_status st = vs_cuda(ctx, cudaGetLastError(), "norm backward launch");
   if (want) {
-    if (st == VS_OK) st = norm_join_partials(ctx, f.s.cols, l.grid, scratch.p, f.wdtype, f.dweight, f.dbias);
+    if (st == VS_OK && !fold) st = norm_join_partials(ctx, f.s.cols, l.grid, scratch.p, f.wdtype, f.dweight, f.dbias);
     const vs_status end = norm_scratch_end(ctx, scratch);
     if (st == VS_OK) st = end;
   }
