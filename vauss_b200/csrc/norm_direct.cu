@@ -16,9 +16,11 @@ using namespace vs;
 constexpr uint32_t FWD_WARPS = 4, BWD_WARPS = 16;
 // threads of a CTA by the values each one holds
 constexpr uint32_t direct_threads(int elems) { return elems > 8 ? 512 : 1024; }
-// Sums of up to this many floats are added by the last CTA to leave its own, which
-// saves the launch of another kernel (20k x 64 f16: 3.4 us of the host's time).
-constexpr uint32_t FOLD_FLOATS = 65536, FOLD_GROUPS = 32;
+// The sums of up to this many CTAs are added by the last one to leave its own,
+// which saves the launch of another kernel: a call of 500 x 64 bf16 (8 CTAs) takes
+// 9.0 us instead of 11.6; with 148 CTAs the one CTA's reads take longer than the
+// launch (20k x 64 f16 12.3 us instead of 10.9).
+constexpr uint32_t FOLD_CTAS = 64, FOLD_GROUPS = 32;
 
 template <typename T, int VEC, int K, bool kJoin, bool kCta>
 __global__ void __launch_bounds__(kCta ? direct_threads(VEC * K) : FWD_WARPS * 32)
@@ -298,7 +300,7 @@ template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status launch(vs
   const bool want = (f.dweight || f.dbias) && l.grid > 1;
   NormScratch scratch;
   if (want) VS_TRY(norm_scratch_begin(ctx, (size_t)l.grid * (2 * f.s.cols + 3), &scratch));
-  const bool fold = want && !kCta && l.grid * 2 * f.s.cols <= FOLD_FLOATS;
+  const bool fold = want && !kCta && l.grid <= FOLD_CTAS;
   size_t smem = kCta ? 0 : BWD_WARPS * 2 * f.s.cols * 4;
   if (fold && smem < BWD_WARPS * 32 * 16) smem = BWD_WARPS * 32 * 16;
   norm_direct_bwd_kernel<T, VEC, K, kJoin, kCta><<<l.grid, l.threads, smem, ctx->stream>>>(
