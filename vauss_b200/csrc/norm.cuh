@@ -2,6 +2,8 @@
 // the streaming kernels, and the launchers norm.cu chooses between.
 #pragma once
 
+#include <initializer_list>
+
 #include "rows.cuh"
 
 namespace vs {
@@ -191,7 +193,7 @@ VSD void pack(const __nv_bfloat16*, float2 v, uint32_t& u) {
 template <typename T> VSD void pack(const T* t, float2 v, uint2& u) {
   uint32_t both_values;
   pack(t, v, both_values);
-  u = make_uint2(both_values & 0xffffu, both_values >> 16);
+  u = make_uint2(both_values, both_values >> 16);  // the first value is read and stored by its lower half
 }
 VSD float keep_if(float v, uint32_t mask) { return __uint_as_float(__float_as_uint(v) & mask); }
 
@@ -506,18 +508,20 @@ struct NormBwd {
   void *dweight, *dbias;
 };
 
-// The runs a lane holds of a row of `chunks` runs, 1 to `most`, with the fewest
-// idle places on the row's lanes (a power of two of them), then the most runs; 0
-// where a warp cannot hold the row.
-inline int norm_runs(uint32_t chunks, int most) {
+// Of `choices`, the runs of `width` values per lane (on a power of two of lanes) that
+// cost a row of `runs` runs the fewest instructions, at about 11 for a value's place,
+// used or idle, and 100 for a lane's share of a row; 0 where a warp cannot hold the
+// row.
+inline int norm_fit(uint32_t runs, int width, std::initializer_list<int> choices) {
   int best = 0;
-  uint32_t places = ~0u;
-  for (int k = 1; k <= most; ++k) {
+  uint32_t least = ~0u;
+  for (int k : choices) {
     uint32_t lanes = 1;
-    while (lanes * k < chunks) lanes *= 2;
-    if (lanes <= 32 && lanes * k <= places) {
+    while (lanes * k < runs) lanes *= 2;
+    const uint32_t cost = lanes * (uint32_t)(11 * k * width + 100);
+    if (lanes <= 32 && cost < least) {
       best = k;
-      places = lanes * k;
+      least = cost;
     }
   }
   return best;

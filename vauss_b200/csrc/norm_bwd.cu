@@ -18,7 +18,7 @@ using namespace vs;
 // slots of 3 KB, 80 % with 8 warps of 32 values.
 template <typename T, int VEC, int K> constexpr int warp_ctas() {
   if (VEC * K <= 8) return 5;
-  if (VEC * K > 16) return 2;
+  if (VEC * K > 18) return 2;
   return VEC * sizeof(T) == 16 && sizeof(T) == 4 ? 2 : 3;
 }
 // Bytes of a slot and input: f32 rows 2 KB, 16-bit rows of 128 bytes 2 KB (89 % of
@@ -313,11 +313,11 @@ template <typename T, int VEC, int K, bool kJoin> vs_status run_kernel(vs_ctx* c
   return st;
 }
 
-// As in the forward, with up to 3 runs of 8 or 4 of 4 values per lane.
+// As in the forward, with up to 3 vectors of 8 or 4 of 4 values per lane.
 template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   constexpr int V = 16 / sizeof(T);
   const uint32_t chunks = f.s.cols / V;
-  switch (norm_runs(chunks, sizeof(T) == 4 ? 4 : 3)) {
+  switch (sizeof(T) == 4 ? norm_fit(chunks, V, {1, 2, 3, 4}) : norm_fit(chunks, V, {1, 2, 3})) {
     case 1: return run_kernel<T, V, 1, kJoin>(ctx, f, taken);
     case 2: return run_kernel<T, V, 2, kJoin>(ctx, f, taken);
     case 3: return run_kernel<T, V, 3, kJoin>(ctx, f, taken);
@@ -327,18 +327,30 @@ template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormB
   return VS_OK;
 }
 
-template <typename T, int VEC, int KS, int KL, bool kJoin>
-vs_status run_blocks(vs_ctx* ctx, const NormBwd& f, bool* taken) {
-  if (f.s.cols <= VEC * KS) return run_kernel<T, VEC, KS, kJoin>(ctx, f, taken);
-  if (f.s.cols <= 32 * VEC * KL) return run_kernel<T, VEC, KL, kJoin>(ctx, f, taken);
+template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormBwd& f, bool* taken) {
+  if constexpr (sizeof(T) == 2) {
+    if (f.s.cols % 2 == 0) {
+      switch (norm_fit(f.s.cols / 2, 2, {3, 5, 7, 9})) {
+        case 3: return run_kernel<T, 2, 3, kJoin>(ctx, f, taken);
+        case 5: return run_kernel<T, 2, 5, kJoin>(ctx, f, taken);
+        case 7: return run_kernel<T, 2, 7, kJoin>(ctx, f, taken);
+        case 9: return run_kernel<T, 2, 9, kJoin>(ctx, f, taken);
+      }
+      return VS_OK;
+    }
+  }
+  switch (norm_fit(f.s.cols, 1, {5, 9, 11, 15})) {
+    case 5: return run_kernel<T, 1, 5, kJoin>(ctx, f, taken);
+    case 9: return run_kernel<T, 1, 9, kJoin>(ctx, f, taken);
+    case 11: return run_kernel<T, 1, 11, kJoin>(ctx, f, taken);
+    case 15: return run_kernel<T, 1, 15, kJoin>(ctx, f, taken);
+  }
   return VS_OK;
 }
 
 template <typename T, bool kJoin> vs_status run(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   if (f.s.cols % (16 / sizeof(T)) == 0) return run_vectors<T, kJoin>(ctx, f, taken);
-  if constexpr (sizeof(T) == 2)
-    if (f.s.cols % 2 == 0) return run_blocks<T, 2, 3, 7, kJoin>(ctx, f, taken);
-  return run_blocks<T, 1, 5, 15, kJoin>(ctx, f, taken);
+  return run_blocks<T, kJoin>(ctx, f, taken);
 }
 
 }  // namespace
