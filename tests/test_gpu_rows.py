@@ -283,6 +283,24 @@ def test_large_backward(cuda, dtype, rows, cols):
         assert torch.equal(j.dweight, g.dweight) and torch.equal(j.dbias, g.dbias)
 
 
+# A width for each number of values that a lane holds, in runs of four, two and one.
+WIDTHS = [2, 3, 6, 10, 17, 18, 20, 23, 28, 33, 36, 60, 76, 130, 170, 201, 250, 300, 401, 420, 700]
+
+
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_large_widths(cuda, cols):
+    rows = 3_000_001 // cols
+    test_large_backward(cuda, BF16, rows, cols)
+    x, x64 = rows_of(cuda, rows, cols, BF16, cols + 3)
+    r, r64 = rows_of(cuda, rows, cols, BF16, cols + 4)
+    w, b, w64, b64 = weights_of(cuda, cols, F32, cols + 5)
+    o = ops.dropout_add_norm(x, r, w, b, 0.25, 7, 9, EPS)
+    z64 = r64 + dropout_ref(x64, 0.25, 7, 9)
+    close(o.z, z64, "z")
+    y64, _, q64 = norm_ref(o.z.cpu().double(), w64, b64)
+    close(o.y, y64, "y", terms=max(1.0, float(q64.max())))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols", [(60_001, 59), (3_701, 1030), (1_001, 4096)])
 def test_large_in_place_and_strided(cuda, dtype, rows, cols):

@@ -261,6 +261,13 @@ template <typename T, int VEC, int K, bool kSpread = VEC * sizeof(T) == 16> stru
           t[k * W + 1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
         }
       }
+    } else if constexpr (VEC == 4 && sizeof(T) == 2) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const uint2 q = *reinterpret_cast<const uint2*>(row + from(k));
+        t[2 * k] = q.x;
+        t[2 * k + 1] = q.y;
+      }
     } else if constexpr (VEC == 2 && sizeof(T) == 2) {
 #pragma unroll
       for (int k = 0; k < K; ++k) t[k] = *reinterpret_cast<const uint32_t*>(row + from(k));
@@ -284,6 +291,8 @@ template <typename T, int VEC, int K, bool kSpread = VEC * sizeof(T) == 16> stru
         else q = make_uint4(__float_as_uint(t[k * W].x), __float_as_uint(t[k * W].y), __float_as_uint(t[k * W + 1].x),
                             __float_as_uint(t[k * W + 1].y));
         *reinterpret_cast<uint4*>(row + from(k)) = q;
+      } else if constexpr (VEC == 4 && sizeof(T) == 2) {
+        *reinterpret_cast<uint2*>(row + from(k)) = make_uint2(t[2 * k], t[2 * k + 1]);
       } else if constexpr (VEC == 2 && sizeof(T) == 2) {
         *reinterpret_cast<uint32_t*>(row + from(k)) = t[k];
       } else if constexpr (sizeof(T) == 2) {
@@ -295,7 +304,7 @@ template <typename T, int VEC, int K, bool kSpread = VEC * sizeof(T) == 16> stru
   }
   // A [cols] vector of weights, `other` where there is none.
   VSD void weights(const void* p, int32_t dtype, float other, float2* w) const {
-    if constexpr (VEC % 4 == 0) {
+    if constexpr (kSpread && VEC % 4 == 0) {
       if (p && dtype == VS_F32 && ((uintptr_t)p & 15u) == 0) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -471,9 +480,6 @@ VSD float cta_sum(float v, float* part, uint32_t warps) {
 constexpr uint32_t NORM_WARPS = 4;   // warps of a CTA whose warps work on their own
 constexpr uint32_t NORM_STAGES = 4;  // ring slots at most
 constexpr uint32_t NORM_MAX_SMEM = 226 * 1024;
-// Threads of an SM that the CTA-per-row kernels' registers leave room for.  The
-// grids follow from this and the shape alone, never from an occupancy query, so
-// the order of the weight gradients' sums does too.
 // The sums of a and b over a warp in one chain: lanes 0 to 15 get a's, the others b's.
 VSD float warp_sum2(float a, float b) {
   const bool low = (threadIdx.x & 16u) == 0;
@@ -510,19 +516,19 @@ struct NormBwd {
 
 // Of `choices`, the runs of `width` values per lane (on a power of two of lanes) that
 // cost a row of `runs` runs the fewest instructions, at about 11 for a value's place,
-// used or idle, and 100 for a lane's share of a row; 0 where a warp cannot hold the
-// row.
-inline int norm_fit(uint32_t runs, int width, std::initializer_list<int> choices) {
-  int best = 0;
-  uint32_t least = ~0u;
+// used or idle, and 100 for a lane's share of a row; none (k = 0) where a warp cannot
+// hold the row.
+struct NormFit {
+  int k;
+  uint32_t cost;
+};
+inline NormFit norm_fit(uint32_t runs, int width, std::initializer_list<int> choices) {
+  NormFit best{0, ~0u};
   for (int k : choices) {
     uint32_t lanes = 1;
     while (lanes * k < runs) lanes *= 2;
     const uint32_t cost = lanes * (uint32_t)(11 * k * width + 100);
-    if (lanes <= 32 && cost < least) {
-      best = k;
-      least = cost;
-    }
+    if (lanes <= 32 && cost < best.cost) best = {k, cost};
   }
   return best;
 }

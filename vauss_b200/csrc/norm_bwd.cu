@@ -18,7 +18,7 @@ using namespace vs;
 // slots of 3 KB, 80 % with 8 warps of 32 values.
 template <typename T, int VEC, int K> constexpr int warp_ctas() {
   if (VEC * K <= 8) return 5;
-  if (VEC * K > 18) return 2;
+  if (VEC * K > 20) return 2;
   return VEC * sizeof(T) == 16 && sizeof(T) == 4 ? 2 : 3;
 }
 // Bytes of a slot and input: f32 rows 2 KB, 16-bit rows of 128 bytes 2 KB (89 % of
@@ -317,7 +317,7 @@ template <typename T, int VEC, int K, bool kJoin> vs_status run_kernel(vs_ctx* c
 template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   constexpr int V = 16 / sizeof(T);
   const uint32_t chunks = f.s.cols / V;
-  switch (sizeof(T) == 4 ? norm_fit(chunks, V, {1, 2, 3, 4}) : norm_fit(chunks, V, {1, 2, 3})) {
+  switch ((sizeof(T) == 4 ? norm_fit(chunks, V, {1, 2, 3, 4}) : norm_fit(chunks, V, {1, 2, 3})).k) {
     case 1: return run_kernel<T, V, 1, kJoin>(ctx, f, taken);
     case 2: return run_kernel<T, V, 2, kJoin>(ctx, f, taken);
     case 3: return run_kernel<T, V, 3, kJoin>(ctx, f, taken);
@@ -327,10 +327,22 @@ template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormB
   return VS_OK;
 }
 
+// Runs of four where they cost less than runs of two (300 bf16 columns 78 %, in runs of
+// two 60 %; 100 columns in runs of two 62 %, of four 52 %).  28 values a lane leave
+// registers for two CTAs only, so they are for rows that nothing else holds (700
+// columns 63 %, a CTA per row 43 %; 28 columns 57 %, 14 values on two lanes 77 %).
 template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   if constexpr (sizeof(T) == 2) {
-    if (f.s.cols % 2 == 0) {
-      switch (norm_fit(f.s.cols / 2, 2, {3, 5, 7, 9})) {
+    const uint32_t cols = f.s.cols;
+    const NormFit two = cols % 2 == 0 ? norm_fit(cols / 2, 2, {3, 5, 7, 9}) : NormFit{0, ~0u};
+    if (cols % 4 == 0) {
+      const NormFit four = norm_fit(cols / 4, 4, {3, 5});
+      if (four.k == 0 && two.k == 0 && norm_fit(cols / 4, 4, {7}).k) return run_kernel<T, 4, 7, kJoin>(ctx, f, taken);
+      if (four.cost < two.cost)
+        return four.k == 3 ? run_kernel<T, 4, 3, kJoin>(ctx, f, taken) : run_kernel<T, 4, 5, kJoin>(ctx, f, taken);
+    }
+    if (cols % 2 == 0) {
+      switch (two.k) {
         case 3: return run_kernel<T, 2, 3, kJoin>(ctx, f, taken);
         case 5: return run_kernel<T, 2, 5, kJoin>(ctx, f, taken);
         case 7: return run_kernel<T, 2, 7, kJoin>(ctx, f, taken);
@@ -339,7 +351,7 @@ template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormBw
       return VS_OK;
     }
   }
-  switch (norm_fit(f.s.cols, 1, {5, 9, 11, 15})) {
+  switch (norm_fit(f.s.cols, 1, {5, 9, 11, 15}).k) {
     case 5: return run_kernel<T, 1, 5, kJoin>(ctx, f, taken);
     case 9: return run_kernel<T, 1, 9, kJoin>(ctx, f, taken);
     case 11: return run_kernel<T, 1, 11, kJoin>(ctx, f, taken);
