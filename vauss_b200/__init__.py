@@ -5,4 +5,6 @@ Kernels live in ``csrc/`` behind the C ABI of ``include/vauss_b200.h``
 point for torch tensors, ``trainer`` and ``view_parallel`` are the training
 step on one and on several GPUs, ``refine``, ``dataset`` and ``checkpoint``
 are densification, the staged ground-truth feed and PLY / moment I/O.
+``feature_head`` is a learned colour head over the row operators (dropout,
+layer norm and the two joined) that ``ops`` wraps.
 """
