@@ -302,6 +302,26 @@ def test_large_widths(cuda, cols):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(67, 16_001), (70, 20_000), (43, 33_333), (2, 140_003)])
+def test_longest_rows(cuda, dtype, rows, cols):
+    """Rows that no kernel holds whole, from contiguous buffers and from columns of a wider one."""
+    test_large_backward(cuda, dtype, rows, cols)
+    x, x64 = rows_of(cuda, rows, cols, dtype, cols + 3)
+    r, r64 = rows_of(cuda, rows, cols, dtype, cols + 4)
+    w, b, w64, b64 = weights_of(cuda, cols, F32, cols + 5)
+    o = ops.dropout_add_norm(x, r, w, b, 0.25, 7, 9, EPS)
+    z64 = r64 + dropout_ref(x64, 0.25, 7, 9)
+    close(o.z, z64, "z")
+    y64, _, q64 = norm_ref(o.z.cpu().double(), w64, b64)
+    close(o.y, y64, "y", terms=max(1.0, float(q64.max())))
+    wide = torch.zeros(rows, cols + 3, dtype=dtype, device=cuda)
+    wide[:, 1:1 + cols] = x
+    v = ops.dropout_add_norm(wide[:, 1:1 + cols], r, w, b, 0.25, 7, 9, EPS)
+    assert torch.equal(v.z, o.z)
+    close(v.y, y64, "y of strided rows", terms=max(1.0, float(q64.max())))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols", [(60_001, 59), (3_701, 1030), (1_001, 4096)])
 def test_large_in_place_and_strided(cuda, dtype, rows, cols):
     """In place, and from columns of a wider buffer, the same bits as out of place from contiguous rows (the column

@@ -7,6 +7,7 @@
 //             t = q (g - mean g - h mean(g h)) (+ dz),
 //             dresidual = t, dx = dropout(t), dw = sum_rows dy h, db = sum_rows dy
 #include <initializer_list>
+#include <type_traits>
 
 #include "norm.cuh"
 
@@ -19,41 +20,117 @@ using Shape = NormShape;
 // One CTA per row, three passes over it: any width, stride and alignment.  The
 // mean is a quotient, not a product with 1 / cols, so that a constant row whose
 // sum is exact has a variance of exactly zero.
+// A row goes in 16-byte vectors where all its buffers begin alike within 16 bytes, its
+// ends and other rows value by value; each pass deals the same values to the same
+// thread, so that a pass may read what the thread wrote or overwrite what it read.
+constexpr uint32_t ROW_THREADS = 512;
+template <typename T> struct RowSplit {
+  static constexpr uint32_t V = 16 / sizeof(T);
+  uint32_t lead, end, cols;  // whole vectors of [lead, end)
+  VSD RowSplit(uint32_t cols_, const void* p, uint32_t differ) : cols(cols_) {
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15u);
+    lead = (16 - off) % 16 / sizeof(T);
+    if (lead > cols || (differ & 15u)) lead = cols;
+    end = lead + (cols - lead) / V * V;
+  }
+  // fn(c, number of values from c on)
+  template <typename F> VSD void each(F fn) const {
+#pragma unroll 2
+    for (uint32_t c = lead + threadIdx.x * V; c < end; c += ROW_THREADS * V) fn(c, std::integral_constant<uint32_t, V>());
+    for (uint32_t k = threadIdx.x; k < lead + (cols - end); k += ROW_THREADS)
+      fn(k < lead ? k : end + (k - lead), std::integral_constant<uint32_t, 1>());
+  }
+};
+VSD uint32_t differ(const void* a, const void* b) {
+  return (uint32_t)(reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b));
+}
+template <uint32_t N, typename T> VSD void row_load(const T* p, float* v) {
+  alignas(16) T t[N];
+  if constexpr (N > 1) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
+  else t[0] = p[0];
+#pragma unroll
+  for (uint32_t j = 0; j < N; ++j) v[j] = to_f32(t[j]);
+}
+template <uint32_t N, typename T> VSD void row_store(T* p, const float* v) {
+  alignas(16) T t[N];
+#pragma unroll
+  for (uint32_t j = 0; j < N; ++j) t[j] = from_f32<T>(v[j]);
+  if constexpr (N > 1) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
+  else p[0] = t[0];
+}
+template <uint32_t N> VSD void row_weights(const void* p, int32_t dtype, uint32_t c, float other, float* v) {
+  const float* f = static_cast<const float*>(p) + c;
+  if (N > 1 && p && dtype == VS_F32 && (reinterpret_cast<uintptr_t>(f) & 15u) == 0) {
+#pragma unroll
+    for (uint32_t j = 0; j < N; j += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(f + j);
+      v[j] = q.x; v[j + 1] = q.y; v[j + 2] = q.z; v[j + 3] = q.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < N; ++j) v[j] = p ? load_as(p, dtype, c + j) : other;
+}
+template <uint32_t N> VSD void row_drop(const Dropout& d, uint64_t i, float* v) {
+  if (!d.threshold) return;
+  if (N > 1 && i % N == 0) {
+    const Words words = run_words<N>(d, i);
+#pragma unroll
+    for (uint32_t j = 0; j < N; ++j) v[j] = dropped(v[j], keeps(words, j, d.limit), d.scale);
+    return;
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < N; ++j) v[j] = dropped(v[j], keep_at(d, i + j), d.scale);
+}
+
 template <typename T, bool kJoin>
-__global__ void __launch_bounds__(256) norm_fwd_rows_kernel(Shape s, Mat<const T> x, Mat<const T> residual, Weights wt,
-                                                            float eps, const Dropout d, T* y, T* z, float* mean,
-                                                            float* rstd) {
+__global__ void __launch_bounds__(ROW_THREADS) norm_fwd_rows_kernel(Shape s, Mat<const T> x, Mat<const T> residual,
+                                                                    Weights wt, float eps, const Dropout d, T* y, T* z,
+                                                                    float* mean, float* rstd) {
   __shared__ float scratch[33];
   const float cols = (float)s.cols;
   for (uint64_t r = blockIdx.x; r < s.rows; r += gridDim.x) {
-    const T* in = x.row(r);
+    const T *in = x.row(r), *res = kJoin ? residual.row(r) : nullptr;
     T* out = y + r * s.cols;
     T* zr = kJoin ? z + r * s.cols : nullptr;
+    const RowSplit<T> split(s.cols, in, differ(in, out) | (kJoin ? differ(in, zr) | differ(in, res) : 0));
     float sum = 0.0f;
-    for (uint64_t c = threadIdx.x; c < s.cols; c += blockDim.x) {
-      if (kJoin) {
-        float v = to_f32(in[c]);
-        if (d.threshold) v = dropped(v, keep_at(d, r * s.cols + c), d.scale);
-        const T zc = from_f32<T>(to_f32(residual.row(r)[c]) + v);
-        zr[c] = zc;
-        sum += to_f32(zc);
-      } else {
-        sum += to_f32(in[c]);
+    split.each([&](uint32_t c, auto n) {
+      constexpr uint32_t N = decltype(n)::value;
+      float v[N];
+      row_load<N>(in + c, v);
+      if constexpr (kJoin) {
+        row_drop<N>(d, r * s.cols + c, v);
+        float e[N];
+        row_load<N>(res + c, e);
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) v[j] = to_f32(from_f32<T>(e[j] + v[j]));
+        row_store<N>(zr + c, v);
       }
-    }
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) sum += v[j];
+    });
     const T* src = kJoin ? zr : in;
     const float m = block_sum(sum, scratch) / cols;
     float sq = 0.0f;
-    for (uint64_t c = threadIdx.x; c < s.cols; c += blockDim.x) {
-      const float e = to_f32(src[c]) - m;
-      sq = fmaf(e, e, sq);
-    }
+    split.each([&](uint32_t c, auto n) {
+      constexpr uint32_t N = decltype(n)::value;
+      float v[N];
+      row_load<N>(src + c, v);
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) sq = fmaf(v[j] - m, v[j] - m, sq);
+    });
     const float q = rsqrtf(block_sum(sq, scratch) / cols + eps);
-    for (uint64_t c = threadIdx.x; c < s.cols; c += blockDim.x) {
-      const float w = wt.weight ? load_as(wt.weight, wt.dtype, c) : 1.0f;
-      const float b = wt.bias ? load_as(wt.bias, wt.dtype, c) : 0.0f;
-      out[c] = from_f32<T>(fmaf((to_f32(src[c]) - m) * q, w, b));
-    }
+    split.each([&](uint32_t c, auto n) {
+      constexpr uint32_t N = decltype(n)::value;
+      float v[N], w[N], b[N];
+      row_load<N>(src + c, v);
+      row_weights<N>(wt.weight, wt.dtype, c, 1.0f, w);
+      row_weights<N>(wt.bias, wt.dtype, c, 0.0f, b);
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) v[j] = fmaf((v[j] - m) * q, w[j], b[j]);
+      row_store<N>(out + c, v);
+    });
     if (threadIdx.x == 0) {
       if (mean) mean[r] = m;
       if (rstd) rstd[r] = q;
@@ -62,35 +139,53 @@ __global__ void __launch_bounds__(256) norm_fwd_rows_kernel(Shape s, Mat<const T
 }
 
 template <typename T, bool kJoin>
-__global__ void __launch_bounds__(256) norm_bwd_rows_kernel(Shape s, Mat<const T> dy, Mat<const T> dz, Mat<const T> z,
-                                                            Weights wt, const float* mean, const float* rstd,
-                                                            const Dropout d, T* dx, T* dresidual) {
+__global__ void __launch_bounds__(ROW_THREADS) norm_bwd_rows_kernel(Shape s, Mat<const T> dy, Mat<const T> dz,
+                                                                    Mat<const T> z, Weights wt, const float* mean,
+                                                                    const float* rstd, const Dropout d, T* dx,
+                                                                    T* dresidual) {
   __shared__ float scratch[33];
   const float cols = (float)s.cols;
   for (uint64_t r = blockIdx.x; r < s.rows; r += gridDim.x) {
     const float m = mean[r], q = rstd[r];
-    const T *gy = dy.row(r), *zr = z.row(r);
+    const T *gy = dy.row(r), *zr = z.row(r), *gz = kJoin && dz.p ? dz.row(r) : nullptr;
+    T *out = dx + r * s.cols, *res = kJoin ? dresidual + r * s.cols : nullptr;
+    const RowSplit<T> split(s.cols, gy, differ(gy, zr) | differ(gy, out) | (kJoin ? differ(gy, res) : 0) |
+                                            (gz ? differ(gy, gz) : 0));
     float sg = 0.0f, sgh = 0.0f;
-    for (uint64_t c = threadIdx.x; c < s.cols; c += blockDim.x) {
-      const float g = to_f32(gy[c]) * (wt.weight ? load_as(wt.weight, wt.dtype, c) : 1.0f);
-      sg += g;
-      sgh = fmaf(g, (to_f32(zr[c]) - m) * q, sgh);
-    }
+    split.each([&](uint32_t c, auto n) {
+      constexpr uint32_t N = decltype(n)::value;
+      float g[N], h[N], w[N];
+      row_load<N>(gy + c, g);
+      row_load<N>(zr + c, h);
+      row_weights<N>(wt.weight, wt.dtype, c, 1.0f, w);
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) {
+        const float e = g[j] * w[j];
+        sg += e;
+        sgh = fmaf(e, (h[j] - m) * q, sgh);
+      }
+    });
     sg = block_sum(sg, scratch) / cols;
     sgh = block_sum(sgh, scratch) / cols;
-    for (uint64_t c = threadIdx.x; c < s.cols; c += blockDim.x) {
-      const float g = to_f32(gy[c]) * (wt.weight ? load_as(wt.weight, wt.dtype, c) : 1.0f);
-      float t = q * (g - sg - (to_f32(zr[c]) - m) * q * sgh);
-      if (kJoin) {
-        if (dz.p) t += to_f32(dz.row(r)[c]);
-        float v = t;
-        if (d.threshold) v = dropped(t, keep_at(d, r * s.cols + c), d.scale);
-        dresidual[r * s.cols + c] = from_f32<T>(t);
-        dx[r * s.cols + c] = from_f32<T>(v);
-      } else {
-        dx[r * s.cols + c] = from_f32<T>(t);
+    split.each([&](uint32_t c, auto n) {
+      constexpr uint32_t N = decltype(n)::value;
+      float g[N], h[N], w[N];
+      row_load<N>(gy + c, g);
+      row_load<N>(zr + c, h);
+      row_weights<N>(wt.weight, wt.dtype, c, 1.0f, w);
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) g[j] = q * (g[j] * w[j] - sg - (h[j] - m) * q * sgh);
+      if constexpr (kJoin) {
+        if (gz) {
+          row_load<N>(gz + c, h);
+#pragma unroll
+          for (uint32_t j = 0; j < N; ++j) g[j] += h[j];
+        }
+        row_store<N>(res + c, g);
+        row_drop<N>(d, r * s.cols + c, g);
       }
-    }
+      row_store<N>(out + c, g);
+    });
   }
 }
 
@@ -106,6 +201,7 @@ __global__ void __launch_bounds__(256) norm_cols_kernel(Shape s, Mat<const T> dy
   const uint64_t r1 = r0 + strip < s.rows ? r0 + strip : s.rows;
   float w = 0.0f, b = 0.0f;
   if (c < s.cols) {
+#pragma unroll 4
     for (uint64_t r = r0 + threadIdx.y; r < r1; r += 8) {
       const float g = to_f32(dy.row(r)[c]);
       w = fmaf(g, (to_f32(z.row(r)[c]) - mean[r]) * rstd[r], w);
@@ -236,7 +332,7 @@ vs_status norm_forward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, co
   if (stream && !taken) VS_TRY(norm_row_forward(ctx, dtype, kJoin, f, &taken));
   if (!taken) VS_TRY(norm_direct_forward(ctx, dtype, kJoin, f, &taken));
   if (taken) return VS_OK;
-  norm_fwd_rows_kernel<T, kJoin><<<row_grid(s.rows), 256, 0, ctx->stream>>>(s, mx, mr, wt, eps, d, (T*)y, (T*)z, mean,
+  norm_fwd_rows_kernel<T, kJoin><<<row_grid(s.rows), ROW_THREADS, 0, ctx->stream>>>(s, mx, mr, wt, eps, d, (T*)y, (T*)z, mean,
                                                                             rstd);
   ++ctx->launches;
   return vs_cuda(ctx, cudaGetLastError(), "norm launch");
@@ -296,7 +392,7 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, c
     if (st == VS_OK) st = end;
     VS_TRY(st);
   }
-  norm_bwd_rows_kernel<T, kJoin><<<row_grid(s.rows), 256, 0, ctx->stream>>>(s, mdy, mdz, mz, wt, mean, rstd, d, (T*)dx,
+  norm_bwd_rows_kernel<T, kJoin><<<row_grid(s.rows), ROW_THREADS, 0, ctx->stream>>>(s, mdy, mdz, mz, wt, mean, rstd, d, (T*)dx,
                                                                             (T*)dresidual);
   ++ctx->launches;
   return vs_cuda(ctx, cudaGetLastError(), "norm backward launch");
