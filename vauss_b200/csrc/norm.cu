@@ -17,9 +17,13 @@ using namespace vs;
 
 using Shape = NormShape;
 
-// One CTA per row, three passes over it: any width, stride and alignment.  The
+// One CTA per row, three passes over it: any width, stride and alignment, for rows
+// that the other kernels do not hold.  The later passes read what the first left in
+// L1 and L2; three CTAs an SM (40 registers) hide more of that than two (2000 rows of
+// 30001 f32 134 and 155 us, 55 and 47 % of the copy rate).  The
 // mean is a quotient, not a product with 1 / cols, so that a constant row whose
 // sum is exact has a variance of exactly zero.
+//
 // A row goes in 16-byte vectors where all its buffers begin alike within 16 bytes, its
 // ends and other rows value by value; each pass deals the same values to the same
 // thread, so that a pass may read what the thread wrote or overwrite what it read.
@@ -84,7 +88,7 @@ template <uint32_t N> VSD void row_drop(const Dropout& d, uint64_t i, float* v) 
 }
 
 template <typename T, bool kJoin>
-__global__ void __launch_bounds__(ROW_THREADS) norm_fwd_rows_kernel(Shape s, Mat<const T> x, Mat<const T> residual,
+__global__ void __launch_bounds__(ROW_THREADS, 3) norm_fwd_rows_kernel(Shape s, Mat<const T> x, Mat<const T> residual,
                                                                     Weights wt, float eps, const Dropout d, T* y, T* z,
                                                                     float* mean, float* rstd) {
   __shared__ float scratch[33];
@@ -139,7 +143,7 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_fwd_rows_kernel(Shape s, Mat
 }
 
 template <typename T, bool kJoin>
-__global__ void __launch_bounds__(ROW_THREADS) norm_bwd_rows_kernel(Shape s, Mat<const T> dy, Mat<const T> dz,
+__global__ void __launch_bounds__(ROW_THREADS, 3) norm_bwd_rows_kernel(Shape s, Mat<const T> dy, Mat<const T> dz,
                                                                     Mat<const T> z, Weights wt, const float* mean,
                                                                     const float* rstd, const Dropout d, T* dx,
                                                                     T* dresidual) {
@@ -190,35 +194,49 @@ __global__ void __launch_bounds__(ROW_THREADS) norm_bwd_rows_kernel(Shape s, Mat
 }
 
 // Column sums of a strip of rows: partial[strip][0] = sum dy h, [1] = sum dy.
-// 32 columns x 8 rows of threads; each thread's rows are summed in order, then
-// the eight in order, so the result does not depend on timing.
+// 32 x 8 threads of four columns each (bf16 rows of 16384, the whole backward 308 us,
+// one column each 516); each thread's rows are summed in order, then the eight in
+// order, so the result does not depend on timing.
+constexpr uint32_t COLS_EACH = 4, COLS_WIDE = 32 * COLS_EACH;  // columns of a thread and of a CTA
 template <typename T>
 __global__ void __launch_bounds__(256) norm_cols_kernel(Shape s, Mat<const T> dy, Mat<const T> z, const float* mean,
                                                         const float* rstd, uint64_t strip, float* partial) {
-  __shared__ float sw[8][32], sb[8][32];
-  const uint64_t c = (uint64_t)blockIdx.x * 32 + threadIdx.x;
+  __shared__ float sw[8][COLS_WIDE], sb[8][COLS_WIDE];
+  const uint64_t c0 = (uint64_t)blockIdx.x * COLS_WIDE + threadIdx.x;
   const uint64_t r0 = blockIdx.y * strip;
   const uint64_t r1 = r0 + strip < s.rows ? r0 + strip : s.rows;
-  float w = 0.0f, b = 0.0f;
-  if (c < s.cols) {
-#pragma unroll 4
-    for (uint64_t r = r0 + threadIdx.y; r < r1; r += 8) {
-      const float g = to_f32(dy.row(r)[c]);
-      w = fmaf(g, (to_f32(z.row(r)[c]) - mean[r]) * rstd[r], w);
-      b += g;
+  float w[COLS_EACH], b[COLS_EACH];
+#pragma unroll
+  for (uint32_t j = 0; j < COLS_EACH; ++j) w[j] = b[j] = 0.0f;
+#pragma unroll 2
+  for (uint64_t r = r0 + threadIdx.y; r < r1; r += 8) {
+    const T *g = dy.row(r) + c0, *v = z.row(r) + c0;
+    const float m = mean[r], q = rstd[r];
+#pragma unroll
+    for (uint32_t j = 0; j < COLS_EACH; ++j) {
+      if (c0 + 32 * j >= s.cols) continue;
+      const float e = to_f32(g[32 * j]);
+      w[j] = fmaf(e, (to_f32(v[32 * j]) - m) * q, w[j]);
+      b[j] += e;
     }
   }
-  sw[threadIdx.y][threadIdx.x] = w;
-  sb[threadIdx.y][threadIdx.x] = b;
+#pragma unroll
+  for (uint32_t j = 0; j < COLS_EACH; ++j) {
+    sw[threadIdx.y][threadIdx.x + 32 * j] = w[j];
+    sb[threadIdx.y][threadIdx.x + 32 * j] = b[j];
+  }
   __syncthreads();
-  if (threadIdx.y == 0 && c < s.cols) {
-    for (int k = 1; k < 8; ++k) {
-      w += sw[k][threadIdx.x];
-      b += sb[k][threadIdx.x];
+  const uint32_t k = threadIdx.y * 32 + threadIdx.x;
+  const uint64_t c = (uint64_t)blockIdx.x * COLS_WIDE + k;
+  if (k < COLS_WIDE && c < s.cols) {
+    float tw = 0.0f, tb = 0.0f;
+    for (uint32_t y = 0; y < 8; ++y) {
+      tw += sw[y][k];
+      tb += sb[y][k];
     }
     float* out = partial + (uint64_t)blockIdx.y * 2 * s.cols;
-    out[c] = w;
-    out[s.cols + c] = b;
+    out[c] = tw;
+    out[s.cols + c] = tb;
   }
 }
 
@@ -376,9 +394,9 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, c
   if (taken) return VS_OK;
   // the column sums read dy, which dx may overwrite, so they come first
   if (dweight || dbias) {
-    const uint32_t col_blocks = (s.cols + 31) / 32;
+    const uint32_t col_blocks = (s.cols + COLS_WIDE - 1) / COLS_WIDE;
     const uint64_t want = 1184 / col_blocks + 1;  // CTAs for every SM
-    const uint64_t most = (s.rows + 63) / 64;
+    const uint64_t most = (s.rows + 15) / 16;
     const uint32_t strips = (uint32_t)(want < most ? want : most);
     const uint64_t strip = (s.rows + strips - 1) / strips;
     NormScratch scratch;
