@@ -284,7 +284,7 @@ def test_large_backward(cuda, dtype, rows, cols):
 
 
 # A width for each number of values that a lane holds, in runs of four, two and one.
-WIDTHS = [2, 3, 6, 10, 17, 18, 20, 23, 28, 33, 36, 60, 76, 130, 170, 201, 250, 300, 401, 420, 700]
+WIDTHS = [2, 3, 6, 10, 17, 18, 20, 23, 28, 33, 36, 60, 76, 130, 170, 201, 250, 300, 401, 420, 602, 700, 703, 750, 822, 902]
 
 
 @pytest.mark.parametrize("cols", WIDTHS)

@@ -22,8 +22,11 @@ template <typename T, int VEC, int K> constexpr int warp_ctas() {
   return VEC * sizeof(T) == 16 && sizeof(T) == 4 ? 2 : 3;
 }
 // Bytes of a slot and input: f32 rows 2 KB, 16-bit rows of 128 bytes 2 KB (89 % of
-// the copy rate, 3 KB 82 %), longer ones 3 KB (rows of 256: 93 %, 2 KB 86 %).
+// the copy rate, 3 KB 82 %), longer ones 3 KB (rows of 256: 93 %, 2 KB 86 %).  Rows
+// that are not whole vectors and over 1.5 KB go two to a slot (780 bf16 columns 68 %,
+// one to a slot 47 %; shorter ones lose by slots of 4 KB, 460 columns 59 and 54 %).
 template <typename T, int VEC> constexpr uint32_t warp_slot(uint32_t row_bytes) {
+  if (VEC * sizeof(T) != 16 && row_bytes > 1536) return 4096;
   return VEC * sizeof(T) == 16 && (sizeof(T) == 4 || row_bytes == 128) ? 2048 : 3072;
 }
 
@@ -330,7 +333,8 @@ template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormB
 // Runs of four where they cost less than runs of two (300 bf16 columns 78 %, in runs of
 // two 60 %; 100 columns in runs of two 62 %, of four 52 %).  28 values a lane leave
 // registers for two CTAs only, so they are for rows that nothing else holds (700
-// columns 63 %, a CTA per row 43 %; 28 columns 57 %, 14 values on two lanes 77 %).
+// columns 62 %, a CTA per row 43 %; 28 columns 57 %, 14 values on two lanes 77 %); so are
+// 22 to 30 in runs of two (750 columns 60 and 45 %, 902 columns 66 and 53 %).
 template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   if constexpr (sizeof(T) == 2) {
     const uint32_t cols = f.s.cols;
@@ -347,6 +351,11 @@ template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormBw
         case 5: return run_kernel<T, 2, 5, kJoin>(ctx, f, taken);
         case 7: return run_kernel<T, 2, 7, kJoin>(ctx, f, taken);
         case 9: return run_kernel<T, 2, 9, kJoin>(ctx, f, taken);
+      }
+      switch (norm_fit(f.s.cols / 2, 2, {11, 13, 15}).k) {
+        case 11: return run_kernel<T, 2, 11, kJoin>(ctx, f, taken);
+        case 13: return run_kernel<T, 2, 13, kJoin>(ctx, f, taken);
+        case 15: return run_kernel<T, 2, 15, kJoin>(ctx, f, taken);
       }
       return VS_OK;
     }

@@ -255,7 +255,9 @@ template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormF
 // Blocks of K runs, K odd (bf16 rows of 250: 16 lanes of 18 values 77 % of the copy
 // rate, 32 lanes of 14 values 47 %; of 170: 16 lanes of 14 values 63 %, 32 lanes of 6
 // values 47 %).  Runs as wide as the columns allow: 300 bf16 columns in runs of four
-// 91 %, of two 61 %; 100 columns 76 and 70 %.
+// 91 %, of two 61 %; 100 columns 76 and 70 %.  16-bit rows that more values a lane
+// hold go with those rather than with a CTA each (902 columns 70 and 55 %, 601 columns
+// 47 and 38 %; 31 values a lane for 801 columns 48 and 49 %, so not those).
 template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   if constexpr (sizeof(T) == 2) {
     if (f.s.cols % 4 == 0) {
@@ -273,6 +275,10 @@ template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormFw
         case 7: return run_kernel<T, 2, 7, kJoin>(ctx, f, taken);
         case 9: return run_kernel<T, 2, 9, kJoin>(ctx, f, taken);
       }
+      switch (norm_fit(f.s.cols / 2, 2, {11, 15}).k) {
+        case 11: return run_kernel<T, 2, 11, kJoin>(ctx, f, taken);
+        case 15: return run_kernel<T, 2, 15, kJoin>(ctx, f, taken);
+      }
       return VS_OK;
     }
   }
@@ -281,6 +287,9 @@ template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormFw
     case 9: return run_kernel<T, 1, 9, kJoin>(ctx, f, taken);
     case 11: return run_kernel<T, 1, 11, kJoin>(ctx, f, taken);
     case 15: return run_kernel<T, 1, 15, kJoin>(ctx, f, taken);
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (norm_fit(f.s.cols, 1, {23}).k) return run_kernel<T, 1, 23, kJoin>(ctx, f, taken);
   }
   return VS_OK;
 }
