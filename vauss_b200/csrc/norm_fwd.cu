@@ -27,7 +27,12 @@ template <typename T, int VEC, int K, bool kJoin> constexpr int warp_ctas() {
   if (VEC * sizeof(T) == 16 && sizeof(T) == 4) return kJoin ? 2 : 3;
   return VEC * K > 20 || sizeof(T) == 4 ? 3 : 4;
 }
-template <typename T, int VEC> constexpr uint32_t warp_slot() { return VEC * sizeof(T) == 16 ? 2048 : 4096; }
+// One input's long ones run in slots of 6 KB (750 bf16 columns 71 %, 4 KB 60 %; 450
+// columns 58 and 66 %; joined, 602 columns 47 and 52 %).
+template <typename T, int VEC, bool kJoin> constexpr uint32_t warp_slot(uint32_t row_bytes) {
+  if (VEC * sizeof(T) == 16) return 2048;
+  return !kJoin && row_bytes > 1000 ? 6144 : 4096;
+}
 
 struct FwdArgs {
   uint64_t rows;
@@ -211,7 +216,7 @@ template <typename T, int VEC, int K, bool kJoin> vs_status run_kernel(vs_ctx* c
   while ((1u << a.log_lanes) * K < chunks) ++a.log_lanes;
   // whole passes per slot; fewer where that would leave warps without rows
   const uint32_t per_pass = 32u >> a.log_lanes;
-  uint32_t passes = warp_slot<T, VEC>() / (row_bytes * per_pass);
+  uint32_t passes = warp_slot<T, VEC, kJoin>(row_bytes) / (row_bytes * per_pass);
   const uint64_t share = (uint64_t)B200_SMS * per_sm * NORM_WARPS * per_pass;
   const uint64_t even = (a.rows + share - 1) / share;
   if (passes > even) passes = (uint32_t)even;
@@ -256,8 +261,8 @@ template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormF
 // rate, 32 lanes of 14 values 47 %; of 170: 16 lanes of 14 values 63 %, 32 lanes of 6
 // values 47 %).  Runs as wide as the columns allow: 300 bf16 columns in runs of four
 // 91 %, of two 61 %; 100 columns 76 and 70 %.  16-bit rows that more values a lane
-// hold go with those rather than with a CTA each (902 columns 70 and 55 %, 601 columns
-// 47 and 38 %; 31 values a lane for 801 columns 48 and 49 %, so not those).
+// hold go with those rather than with a CTA each (902 columns 74 and 55 %, 602 columns
+// 65 and 38 %; 31 values a lane for 801 columns 48 and 49 %, so not those).
 template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   if constexpr (sizeof(T) == 2) {
     if (f.s.cols % 4 == 0) {
