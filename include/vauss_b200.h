@@ -460,8 +460,10 @@ VS_API vs_status vs_noise_means(vs_ctx* ctx, uint32_t n, float* transforms, cons
  * Inputs named with a stride hold row r at r * stride elements (a stride of 0
  * stands for cols); everything else is contiguous.  Buffers need the alignment
  * of their element; whole 16-byte vectors are used where base and rows allow.
- * An output may be the same buffer as an input of the same call that is
- * contiguous and of its shape; buffers that overlap otherwise are not allowed.
+ * An output of rows (y, z, dx, dresidual) may be the same buffer as a
+ * contiguous input of rows of the same call, and dweight or dbias the same as
+ * weight; buffers that overlap otherwise are not allowed (mean and rstd in the
+ * weight's or the bias's buffer are refused).
  * rows may be 0 (the weight gradients are then zeros).
  *
  * Dropout's mask is a function of (seed, offset, index), index = row * cols +

@@ -1,0 +1,54 @@
+"""The row operators where calls reach the edges of what the header allows:
+buffers that serve as input and output, sums over very many rows, captured
+graphs, streams and threads.
+
+Helpers and the tolerances of `close` are those of test_gpu_rows.py."""
+import pytest
+import torch
+
+from tests.test_gpu_rows import DTYPES, F32, rows_of, weights_of
+from vauss_b200 import _native, ops
+
+pytestmark = pytest.mark.gpu
+
+# One shape for each backward kernel: rows on warps and on a CTA, direct and streaming, and rows that no kernel holds.
+BACKWARD = [(1, 64), (40, 100), (3, 4096), (900, 64), (50_003, 64), (60_001, 59), (801, 5003), (70, 20_000), (5, 33_333)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", BACKWARD)
+@pytest.mark.parametrize("over", ["dweight", "dbias"])
+def test_weight_gradients_over_the_weight(cuda, dtype, rows, cols, over):
+    """dweight or dbias in the weight's own buffer: the bits of a call with buffers of their own."""
+    z, _ = rows_of(cuda, rows, cols, dtype, 1)
+    dy, _ = rows_of(cuda, rows, cols, dtype, 2)
+    dz, _ = rows_of(cuda, rows, cols, dtype, 3)
+    w, _, _, _ = weights_of(cuda, cols, F32, 4)
+    o = ops.layer_norm(z, w)
+    wide = torch.zeros(rows, cols + 3, dtype=dtype, device=cuda)
+    wide[:, 1:1 + cols] = dy
+    for g in (dy, wide[:, 1:1 + cols]):
+        want = ops.layer_norm_bwd(g, z, w, o.mean, o.rstd)
+        own = w.clone()
+        out = ops.LayerNormGrads(torch.empty_like(z), torch.empty_like(w), torch.empty_like(w))
+        setattr(out, over, own)
+        got = ops.layer_norm_bwd(g, z, own, o.mean, o.rstd, out=out)
+        assert all(torch.equal(getattr(got, k), getattr(want, k)) for k in ("dx", "dweight", "dbias"))
+        want = ops.dropout_add_norm_bwd(g, dz, z, w, o.mean, o.rstd, 0.25, 1, 2)
+        own = w.clone()
+        out = ops.DropoutAddNormGrads(torch.empty_like(z), torch.empty_like(z), torch.empty_like(w), torch.empty_like(w))
+        setattr(out, over, own)
+        got = ops.dropout_add_norm_bwd(g, dz, z, own, o.mean, o.rstd, 0.25, 1, 2, out=out)
+        assert all(torch.equal(getattr(got, k), getattr(want, k)) for k in ("dx", "dresidual", "dweight", "dbias"))
+
+
+def test_statistics_do_not_share_the_weights(cuda):
+    """mean or rstd in the weight's or the bias's buffer (64 rows of 64): rows would read what others wrote."""
+    x, _ = rows_of(cuda, 64, 64, F32, 1)
+    w, b, _, _ = weights_of(cuda, 64, F32, 2)
+    y, s = torch.empty_like(x), torch.empty(64, device=cuda)
+    for mean, rstd in ((w, s), (b, s), (s, w), (s, b)):
+        with pytest.raises(_native.VsError, match="mean and rstd"):
+            ops.layer_norm(x, w, b, out=ops.LayerNormOutput(y, mean, rstd))
+        with pytest.raises(_native.VsError, match="mean and rstd"):
+            ops.dropout_add_norm(x, x, w, b, 0.1, 1, out=ops.DropoutAddNormOutput(y, torch.empty_like(x), mean, rstd))

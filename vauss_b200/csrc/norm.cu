@@ -340,6 +340,10 @@ vs_status norm_forward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, co
   VS_TRY(check_ptr(ctx, what, "rstd", rstd, 4, false));
   VS_TRY(check_ptr(ctx, what, "weight", wt.weight, vs_dtype_size(wt.dtype), false));
   VS_TRY(check_ptr(ctx, what, "bias", wt.bias, vs_dtype_size(wt.dtype), false));
+  // a row's statistics are written while other rows still read the weights
+  for (const float* stat : {mean, rstd})
+    if (stat && (stat == wt.weight || stat == wt.bias))
+      return vs_fail(ctx, VS_ERR_INVALID, "%s: mean and rstd cannot share the weight's or the bias's buffer", what);
   if (!(eps >= 0.0f) || eps > 3e38f) return vs_fail(ctx, VS_ERR_INVALID, "%s: eps = %g", what, (double)eps);
   if (s.rows == 0) return VS_OK;
   VS_CUDA(ctx, cudaSetDevice(ctx->device));
@@ -392,28 +396,34 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, c
   if (!taken) VS_TRY(norm_direct_backward(ctx, dtype, kJoin, f, &taken));
   if (!taken && stream && small) VS_TRY(norm_row_backward(ctx, dtype, kJoin, f, &taken));
   if (taken) return VS_OK;
-  // the column sums read dy, which dx may overwrite, so they come first
-  if (dweight || dbias) {
-    const uint32_t col_blocks = (s.cols + COLS_WIDE - 1) / COLS_WIDE;
-    const uint64_t want = 1184 / col_blocks + 1;  // CTAs for every SM
-    const uint64_t most = (s.rows + 15) / 16;
-    const uint32_t strips = (uint32_t)(want < most ? want : most);
-    const uint64_t strip = (s.rows + strips - 1) / strips;
-    NormScratch scratch;
+  // The column sums read dy, which dx may overwrite, so they come before the rows; dx
+  // reads the weight, which dweight may overwrite, so the sums are joined after them.
+  const bool want = dweight || dbias;
+  const uint32_t col_blocks = (s.cols + COLS_WIDE - 1) / COLS_WIDE;
+  const uint64_t even = 1184 / col_blocks + 1;  // CTAs for every SM
+  const uint64_t most = (s.rows + 15) / 16;
+  const uint32_t strips = (uint32_t)(even < most ? even : most);
+  NormScratch scratch;
+  vs_status st = VS_OK;
+  if (want) {
     VS_TRY(norm_scratch_begin(ctx, (size_t)strips * 2 * s.cols, &scratch));
-    norm_cols_kernel<T><<<dim3(col_blocks, strips), dim3(32, 8), 0, ctx->stream>>>(s, mdy, mz, mean, rstd, strip,
-                                                                                  scratch.p);
+    norm_cols_kernel<T><<<dim3(col_blocks, strips), dim3(32, 8), 0, ctx->stream>>>(
+        s, mdy, mz, mean, rstd, (s.rows + strips - 1) / strips, scratch.p);
     ++ctx->launches;
-    vs_status st = vs_cuda(ctx, cudaGetLastError(), "norm column sums launch");
+    st = vs_cuda(ctx, cudaGetLastError(), "norm column sums launch");
+  }
+  if (st == VS_OK) {
+    norm_bwd_rows_kernel<T, kJoin><<<row_grid(s.rows), ROW_THREADS, 0, ctx->stream>>>(s, mdy, mdz, mz, wt, mean, rstd, d,
+                                                                              (T*)dx, (T*)dresidual);
+    ++ctx->launches;
+    st = vs_cuda(ctx, cudaGetLastError(), "norm backward launch");
+  }
+  if (want) {
     if (st == VS_OK) st = norm_join_partials(ctx, s.cols, strips, scratch.p, wt.dtype, dweight, dbias);
     const vs_status end = norm_scratch_end(ctx, scratch);
     if (st == VS_OK) st = end;
-    VS_TRY(st);
   }
-  norm_bwd_rows_kernel<T, kJoin><<<row_grid(s.rows), ROW_THREADS, 0, ctx->stream>>>(s, mdy, mdz, mz, wt, mean, rstd, d, (T*)dx,
-                                                                            (T*)dresidual);
-  ++ctx->launches;
-  return vs_cuda(ctx, cudaGetLastError(), "norm backward launch");
+  return st;
 }
 
 }  // namespace
