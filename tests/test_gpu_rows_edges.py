@@ -52,3 +52,29 @@ def test_statistics_do_not_share_the_weights(cuda):
             ops.layer_norm(x, w, b, out=ops.LayerNormOutput(y, mean, rstd))
         with pytest.raises(_native.VsError, match="mean and rstd"):
             ops.dropout_add_norm(x, x, w, b, 0.1, 1, out=ops.DropoutAddNormOutput(y, torch.empty_like(x), mean, rstd))
+
+
+def test_destroying_a_context_waits_for_every_stream(cuda):
+    """A ctx whose calls went to one stream and that ends on another: its buffers are freed only after the first
+    stream's work (held back by a long kernel before the calls) has ended."""
+    z, _ = rows_of(cuda, 20_000, 96, F32, 1)
+    dy, _ = rows_of(cuda, 20_000, 96, F32, 2)
+    w, _, _, _ = weights_of(cuda, 96, F32, 3)
+    o = ops.layer_norm(z, w)
+    want = ops.layer_norm_bwd(dy, z, w, o.mean, o.rstd)
+    got = [torch.empty_like(t) for t in (want.dx, want.dweight, want.dbias)]
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    ctx = ops.Context(cuda.index or 0)
+    lib = ctx.lib
+    assert lib.vs_ctx_set_stream(ctx.h, a.cuda_stream) == 0
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(400_000_000)  # about 0.2 s
+    assert lib.vs_layer_norm_backward(ctx.h, 20_000, 96, 0, 0, dy.data_ptr(), 0, z.data_ptr(), 0, w.data_ptr(),
+                                      o.mean.data_ptr(), o.rstd.data_ptr(), *(t.data_ptr() for t in got)) == 0
+    assert not a.query()
+    assert lib.vs_ctx_set_stream(ctx.h, b.cuda_stream) == 0
+    h, ctx.h = ctx.h, None
+    lib.vs_ctx_destroy(h)
+    assert a.query()
+    assert all(torch.equal(t, u) for t, u in zip(got, (want.dx, want.dweight, want.dbias)))

@@ -129,7 +129,9 @@ VS_API vs_status vs_ctx_create(int device, vs_ctx** out) {
 VS_API void vs_ctx_destroy(vs_ctx* ctx) {
   if (!ctx) return;
   cudaSetDevice(ctx->device);
-  cudaStreamSynchronize(ctx->stream);
+  // The ctx may have worked on other streams than its last one (vs_ctx_set_stream),
+  // and what it frees below is ordered by the last one alone.
+  cudaDeviceSynchronize();
   vs_release(ctx, ctx->sort_keys);
   vs_release(ctx, ctx->sort_vals);
   vs_release(ctx, ctx->sort_hist);
@@ -137,7 +139,6 @@ VS_API void vs_ctx_destroy(vs_ctx* ctx) {
   vs_release(ctx, ctx->misc);
   vs_release(ctx, ctx->io_stage);
   vs_release(ctx, ctx->vjp_rows);
-  if (ctx->norm_streams > 1) cudaDeviceSynchronize();  // other streams' buffers
   for (DevBuf& b : ctx->norm_sums) vs_release(ctx, b);
   cudaStreamSynchronize(ctx->stream);
   if (ctx->d_err) cudaFree(ctx->d_err);
