@@ -15,6 +15,9 @@
  *    ctx raises so that this process keeps freed blocks for reuse).  A
  *    vs_frame owns the per-render intermediates (projected splats, the sorted
  *    intersection list, tile ranges) that the backward of that render reads.
+ *  - A ctx and its frames serve one host thread at a time: calls of several
+ *    threads on one ctx race (for its stream and its workspace).  The caller
+ *    serialises them or gives each thread a ctx.
  *  - Calls enqueue work on the ctx stream and return without waiting, except
  *    vs_render_forward, which reads the two projection counts back (the
  *    reference's render-count readback, src/render.rs:590-597) to size the

@@ -3,6 +3,8 @@ buffers that serve as input and output, sums over very many rows, captured
 graphs, streams and threads.
 
 Helpers and the tolerances of `close` are those of test_gpu_rows.py."""
+import threading
+
 import pytest
 import torch
 
@@ -78,3 +80,30 @@ def test_destroying_a_context_waits_for_every_stream(cuda):
     lib.vs_ctx_destroy(h)
     assert a.query()
     assert all(torch.equal(t, u) for t, u in zip(got, (want.dx, want.dweight, want.dbias)))
+
+
+def test_threads_on_streams_of_their_own(cuda):
+    """Calls of several threads at once, each on its stream: the bits of calls one after another."""
+    w, _, _, _ = weights_of(cuda, 96, F32, 1)
+    data = [(rows_of(cuda, 20_000, 96, F32, 10 + k)[0], rows_of(cuda, 20_000, 96, F32, 20 + k)[0]) for k in range(3)]
+    stats = [ops.layer_norm(z, w) for _, z in data]
+    want = [ops.layer_norm_bwd(dy, z, w, o.mean, o.rstd) for (dy, z), o in zip(data, stats)]
+    torch.cuda.synchronize()
+    got, gate = [[] for _ in data], threading.Barrier(len(data))
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            gate.wait(30)
+            for _ in range(50):
+                got[k].append(ops.layer_norm_bwd(*data[k], w, stats[k].mean, stats[k].rstd))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(data))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for per_thread, ref in zip(got, want):
+        assert len(per_thread) == 50
+        for g in per_thread:
+            assert all(torch.equal(getattr(g, k), getattr(ref, k)) for k in ("dx", "dweight", "dbias"))

@@ -8,6 +8,7 @@ libvauss_b200.so.
 from __future__ import annotations
 
 import ctypes
+import threading
 from dataclasses import dataclass
 
 import numpy as np
@@ -408,9 +409,39 @@ _DTYPES = {torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16, torch.bfloat1
 _F32 = torch.float32
 
 
+# ctypes lets other threads run during a call, and a ctx serves one thread at a time (a call's stream and scratch are
+# the ctx's), so each thread has contexts of its own for these operators.  A thread that ends leaves them to the next
+# that needs one: what a ctx keeps is kept by stream.
+_idle_contexts: list[Context] = []
+_idle_lock = threading.Lock()
+
+
+class _ThreadContexts:
+    def __init__(self):
+        self.of: dict[int, Context] = {}  # by device
+        self.idle = _idle_contexts
+
+    def __del__(self):
+        self.idle.extend(self.of.values())
+
+
+class _RowContexts(threading.local):
+    def __init__(self):
+        self.held = _ThreadContexts()
+        self.of = self.held.of
+
+
+_row_contexts = _RowContexts()
+
+
 def _row_context(device: int) -> Context:
-    ctx = _contexts.get(device)
-    return context(device) if ctx is None else ctx.bind()
+    ctx = _row_contexts.of.get(device)
+    if ctx is None:
+        with _idle_lock:
+            at = next((k for k, c in enumerate(_idle_contexts) if c.device == device), None)
+            ctx = Context(device) if at is None else _idle_contexts.pop(at)
+        _row_contexts.of[device] = ctx
+    return ctx.bind()
 
 
 def _row_shape(t: torch.Tensor):
