@@ -469,6 +469,11 @@ VS_API vs_status vs_noise_means(vs_ctx* ctx, uint32_t n, float* transforms, cons
  * weight's or the bias's buffer are refused).
  * rows may be 0 (the weight gradients are then zeros).
  *
+ * The kernels wait for their own copies, a second at most.  A wait that runs
+ * out sets the ctx's device error, which vs_ctx_check reports as
+ * VS_ERR_DEVICE_TIMEOUT; the call's outputs are then undefined, and weight
+ * gradients NaN.
+ *
  * Dropout's mask is a function of (seed, offset, index), index = row * cols +
  * col, and is never stored: with t = round(65536 p) (at most 65535 unless p is
  * 1), the value is kept when its 16-bit number is at least t and multiplied by

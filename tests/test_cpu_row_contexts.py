@@ -17,6 +17,9 @@ class FakeContext:
     def bind(self):
         return self
 
+    def check(self, status):
+        ops.N.check(None, status)
+
 
 @pytest.fixture
 def fake(monkeypatch):
@@ -60,3 +63,21 @@ def test_threads_that_ended_leave_their_contexts(fake):
     assert FakeContext.made == 3 and {id(c) for c in again} == {id(c) for c in first}
     _in_threads(1, lambda: ops._row_context(2))  # no context of another device is taken
     assert FakeContext.made == 4
+
+
+def test_a_wait_that_ran_out_is_reported(fake, monkeypatch):
+    """check_device asks the thread's context of the row operators too, and raises what it reports."""
+    asked = []
+
+    class Lib:
+        def vs_ctx_check(self, h):
+            asked.append(h)
+            return 4 if h == "row" else 0
+
+    row, other = ops._row_context(0), FakeContext(0)
+    monkeypatch.setattr(FakeContext, "lib", Lib(), raising=False)
+    row.h, other.h = "row", "other"
+    ops._contexts[0] = other
+    with pytest.raises(ops.N.VsError, match="TIMEOUT"):
+        ops.check_device(0)
+    assert asked == ["other", "row"]

@@ -3,6 +3,7 @@ buffers that serve as input and output, sums over very many rows, captured
 graphs, streams and threads.
 
 Helpers and the tolerances of `close` are those of test_gpu_rows.py."""
+import ctypes
 import threading
 
 import pytest
@@ -107,3 +108,17 @@ def test_threads_on_streams_of_their_own(cuda):
         assert len(per_thread) == 50
         for g in per_thread:
             assert all(torch.equal(getattr(g, k), getattr(ref, k)) for k in ("dx", "dweight", "dbias"))
+
+
+def test_the_error_word_is_read(cuda):
+    """A wait that runs out on the context of the row operators (a peer barrier that nobody else signals) raises from
+    check_device, once; without one it returns."""
+    ops.layer_norm(torch.ones(4, 8, device=cuda))
+    ops.check_device(cuda)
+    ctx = ops._row_context(cuda.index or 0)
+    mine, other = (torch.zeros(2, dtype=torch.int32, device=cuda) for _ in range(2))
+    ptrs = (ctypes.c_void_p * _native.PEER_MAX)(mine.data_ptr(), other.data_ptr())
+    assert ctx.lib.vs_peer_barrier(ctx.h, ptrs, 2, 0, 1) == 0
+    with pytest.raises(_native.VsError, match="TIMEOUT"):
+        ops.check_device()
+    ops.check_device(0)

@@ -40,7 +40,9 @@ VSD bool mbar_try(uint64_t* b, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Waits for a copy to land; false after a second without it.
+// Waits for a copy to land; false after a second without it.  The caller then sets
+// the device error word and ends, so what it had yet to write is undefined; the column
+// sums of its CTA become NaN.
 constexpr uint64_t COPY_WAIT_NS = 1000000000ull;
 constexpr uint32_t COPY_SPIN_LIMIT = 1u << 26;  // backstop on the iteration count
 VSD uint64_t copy_clock_ns() {
@@ -141,6 +143,8 @@ template <typename U> VSD void span_store(const Span& s, const void* slot, void*
   for (uint64_t i = tail / sizeof(U) + lane; i < s.end / sizeof(U); i += 32)
     static_cast<U*>(base)[i] = reinterpret_cast<const U*>(static_cast<const char*>(slot) + (i * sizeof(U) - s.lo))[0];
 }
+
+VSD float nan_value() { return __uint_as_float(0x7fc00000u); }
 
 // Two f32 operations in one instruction.
 VSD unsigned long long bits2(float2 a) { return reinterpret_cast<unsigned long long&>(a); }

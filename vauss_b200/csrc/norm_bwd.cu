@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
       parity ^= 1;
     }
   }
-  if (!ok && lane == 0) {  // a copy did not land in time: report, and let those in flight end
+  if (!ok && lane == 0) {  // a copy did not land in time: report, and wait for those in flight, as long again each
     atomicOr(a.err, VS_DERR_WAIT);
     for (uint32_t k = 0; k < a.stages && row0 < a.rows; ++k, row0 += step_rows) {
       mbar_wait(&full[slot], parity);
@@ -228,8 +228,12 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
 
   float* out = a.partial + (uint64_t)blockIdx.x * 2 * a.cols;
   // lanes with the same columns (their runs turned differently), then the
-  // warps, each in order, through the rings' memory
-  __syncthreads();
+  // warps, each in order, through the rings' memory; where a warp gave up, whose copies
+  // may still be on their way there, the sums are marked invalid instead
+  if (!__syncthreads_and(ok)) {
+    for (uint32_t c = threadIdx.x; c < 2 * a.cols; c += NORM_WARPS * 32) out[c] = nan_value();
+    return;
+  }
   float* sums = reinterpret_cast<float*>(smem);  // [warp][2][cols]
   float* mine = sums + warp * 2 * a.cols;
   for (uint32_t k = 0; k < per_pass; ++k) {

@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K, kJoin>()
       parity ^= 1;
     }
   }
-  if (!ok && lane == 0) {  // a copy did not land in time: report, and let those in flight end
+  if (!ok && lane == 0) {  // a copy did not land in time: report, and wait for those in flight, as long again each
     atomicOr(a.err, VS_DERR_WAIT);
     for (uint32_t k = 0; k < a.stages && row0 < a.rows; ++k, row0 += step * a.tile_rows) {
       mbar_wait(&full[slot], parity);

@@ -169,7 +169,8 @@ template <typename T> struct RowRing {
     if (at >= (total & ~15ull)) return to_f32(static_cast<const T*>(a.in[input])[at / sizeof(T)]);
     return lds_value<T>(row(slot, input) + c * (uint32_t)sizeof(T));
   }
-  // After a copy that did not land in time: report it and let the others end.
+  // After a copy that did not land in time: report it and wait for those in flight, as
+  // long again for each.
   VSD void give_up(uint32_t slot, uint32_t parity, uint64_t row) const {
     atomicOr(a.err, VS_DERR_WAIT);
     for (uint32_t k = 0; k < a.stages && row < a.rows; ++k, row += gridDim.x) {
@@ -444,6 +445,10 @@ __global__ void __launch_bounds__(row_bwd<T, K>()) norm_row_bwd_kernel(const Row
   }
   if (!ok && tid == 0) ring.give_up(slot, parity, row);
   if (!out) return;
+  if (!ok) {  // the sums are marked invalid, those of the ends' warp too, which has left
+    for (uint32_t c = tid; c < 2 * a.cols; c += part.threads) out[c] = nan_value();
+    return;
+  }
   if (a.cols % 4 == 0 && place.lead % 4 == 0) {  // whole 16-byte pieces: single values would cost the L2 a write each
 #pragma unroll
     for (int i = 0; i < PAIRS; i += 2) {

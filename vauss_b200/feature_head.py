@@ -129,6 +129,7 @@ def fit(steps: int = 60, width: int = 64, hidden: int = 128, blocks: int = 2, p:
             v.grad = head.grads[k]
         opt.step()
         losses.append(loss.loss.clone())
+    ops.check_device(device)
     return torch.stack(losses).tolist()
 
 

@@ -75,6 +75,17 @@ def context(device: int | torch.device | None = None) -> Context:
     return ctx.bind()
 
 
+def check_device(device: int | torch.device | None = None) -> None:
+    """Waits for the current stream and raises if a bounded wait of a kernel gave up in this thread's calls on the device
+    (vs_ctx_check).  The calls return before their kernels run, so none of them can tell by itself."""
+    device = torch.device("cuda" if device is None else device)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    for ctx in (_contexts.get(index), _row_contexts.of.get(index)):
+        if ctx is not None:
+            ctx.bind()
+            ctx.check(ctx.lib.vs_ctx_check(ctx.h))
+
+
 def render_cfg(sh_degree: int, mip: bool = True, sh_half: bool = False, background=(0.0, 0.0, 0.0),
                log_scale_offset: float = 0.0, has_min_scale: bool = False) -> N.RenderCfg:
     c = N.RenderCfg()
