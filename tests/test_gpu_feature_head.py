@@ -76,3 +76,46 @@ def test_refuses_other_types(cuda):
         head.forward(torch.zeros(4, 16, device=cuda))
     with pytest.raises(AssertionError):
         feature_head.FeatureHead(16, 16, 1, 1.5, cuda)
+
+
+@pytest.mark.parametrize("size", [1e-9, 1e-7, 1.0, 1e5])
+def test_f16_gradients_of_any_size(cuda, size):
+    """Gradients of a loss over an image are of the order of 1e-7 and less, f16's smallest value is 6e-8.
+
+    Tolerance, on the whole of each gradient (root of the sum of squares): about 14 values in a row are rounded to f16
+    (14 * 2^-11 = 0.7 %), and the rounding turns the sign of about 3e-4 of the activations that the relu sees, which
+    changes two layers' gradients by the root of that, 1.7 % each: 5 % covers them."""
+    n, width, p = 501, 48, 0.25
+    head = feature_head.FeatureHead(width, 40, 2, p, cuda, torch.float16, seed=5)
+    gen = torch.Generator().manual_seed(n)
+    x = torch.randn(n, width, generator=gen).half()
+    c = torch.randn(n, 3, generator=gen) * size
+    head.forward(x.to(cuda))
+    dx = head.backward(c.to(cuda))
+
+    w = {k: v.detach().cpu().double().requires_grad_() for k, v in head.params.items()}
+    f = x.double().requires_grad_()
+    h, y = f, _norm(f, w["norm0.weight"], w["norm0.bias"])
+    for k in range(2):
+        r = torch.relu(y @ w[f"block{k}.w1"]) @ w[f"block{k}.w2"]
+        keep, scale = keep_mask(r.numel(), p, 5, 1 * 2 + k)
+        h = h + r * keep.view(r.shape) * scale
+        y = _norm(h, w[f"norm{k + 1}.weight"], w[f"norm{k + 1}.bias"])
+    (y @ w["out"]).backward(c.double())
+    for name, got, ref in [("features", dx, f.grad)] + [(k, head.grads[k], w[k].grad) for k in head.params]:
+        err = float((got.detach().cpu().double() - ref).norm() / ref.norm())
+        assert err <= 0.05, f"{name}: {err}"
+
+
+def test_f16_gradients_of_nothing(cuda):
+    head = feature_head.FeatureHead(16, 16, 1, 0.1, cuda, torch.float16)
+    for n, value in ((5, 0.0), (0, 0.0)):
+        head.forward(torch.ones(n, 16, device=cuda, dtype=torch.float16))
+        assert torch.equal(head.backward(torch.full((n, 3), value, device=cuda)), torch.zeros(n, 16, device=cuda))
+        assert all(bool((v == 0).all()) for v in head.grads.values())
+
+
+def test_f16_fit_lowers_the_loss(cuda):
+    losses = feature_head.fit(steps=40, dtype=torch.float16)
+    assert all(np.isfinite(losses))
+    assert np.mean(losses[-4:]) + 0.2 < 0.6 * (np.mean(losses[:4]) + 0.2)

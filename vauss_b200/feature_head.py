@@ -6,7 +6,9 @@ The blocks are the usual ones, h <- h + dropout(relu(norm(h) W1) W2).  Between
 the matrix products (plain library products through torch) stand the row
 operators of ``ops``: ``layer_norm`` at the entry, ``dropout_add_norm`` between
 blocks, which sums, drops and normalises in one pass, and their gradients.
-Weights and the optimizer are f32; rows are f32, f16 or bf16.
+Weights and the optimizer are f32; rows are f32, f16 or bf16.  The gradient of a
+loss over an image is far below f16's range, so an f16 head scales what enters
+its backward by a power of two and takes it out of the results again.
 
 ``python -m vauss_b200.feature_head`` fits the head to a scene whose splats are
 lit differently in the views than in their own colours, and prints the loss.
@@ -64,25 +66,45 @@ class FeatureHead:
         return (y @ self._w("out")).float()
 
     def backward(self, dout: torch.Tensor) -> torch.Tensor:
+        """The features' gradient, in the head's type (f32 for an f16 head, whose range small ones would leave)."""
         features, first, kept, y, p = self._saved
         g, w = self.grads, self.params
-        dout = dout.to(self.dtype)
-        g["out"].copy_(y.t() @ dout)
+        scale = _f16_scale(dout) if self.dtype == torch.float16 else None
+        dout = (dout if scale is None else dout * scale).to(self.dtype)
+
+        def product(a, b):  # over the rows: in f32 where the sum could leave the type's range
+            return a @ b if scale is None else torch.mm(a, b, out_dtype=torch.float32)
+
+        def leave(name, value):
+            g[name].copy_(value if scale is None else value / scale)
+
+        leave("out", product(y.t(), dout))
         dy, dz = dout @ self._w("out").t(), None
         for k in reversed(range(self.blocks)):
             y_in, a, o, offset = kept[k]
             d = ops.dropout_add_norm_bwd(dy, dz, o.z, w[f"norm{k + 1}.weight"], o.mean, o.rstd, p, self.seed, offset)
-            g[f"norm{k + 1}.weight"].copy_(d.dweight)
-            g[f"norm{k + 1}.bias"].copy_(d.dbias)
+            leave(f"norm{k + 1}.weight", d.dweight)
+            leave(f"norm{k + 1}.bias", d.dbias)
             dz = d.dresidual
-            g[f"block{k}.w2"].copy_(a.t() @ d.dx)
+            leave(f"block{k}.w2", product(a.t(), d.dx))
             da = (d.dx @ self._w(f"block{k}.w2").t()).mul_(a > 0)
-            g[f"block{k}.w1"].copy_(y_in.t() @ da)
+            leave(f"block{k}.w1", product(y_in.t(), da))
             dy = da @ self._w(f"block{k}.w1").t()
         d = ops.layer_norm_bwd(dy, features, w["norm0.weight"], first.mean, first.rstd)
-        g["norm0.weight"].copy_(d.dweight)
-        g["norm0.bias"].copy_(d.dbias)
-        return d.dx if dz is None else d.dx + dz
+        leave("norm0.weight", d.dweight)
+        leave("norm0.bias", d.dbias)
+        if scale is None:
+            return d.dx if dz is None else d.dx + dz
+        return (d.dx.float() if dz is None else d.dx.float() + dz.float()) / scale
+
+
+def _f16_scale(dout: torch.Tensor) -> torch.Tensor:
+    """The power of two (on the device) that brings the largest value to 8 to 16: room above for the rows' rstd, of up
+    to 1 / sqrt(eps) = 316, and 17 binary places below for values of f16's full precision."""
+    if dout.numel() == 0:
+        return torch.ones((), device=dout.device)
+    places = torch.floor(4.0 - torch.log2(dout.detach().float().abs().amax())).clamp(-60, 60)  # 60 for zeros
+    return torch.where(places.isfinite(), torch.exp2(places), 1.0)
 
 
 def lit_views(n_views: int = 4, device="cuda:0"):
