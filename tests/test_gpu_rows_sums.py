@@ -1,5 +1,6 @@
 """The row operators' sums on data whose sums are exact, so that a value lost, taken
-twice or put into another row shows at any number of rows.
+twice or put into another row shows at any number of rows, and on random f32 data
+within bounds that follow from the additions.
 
 Exact data: values of 1 and 2, weights of 1/2, 1 and 2, mean 0 and rstd 1.  Every
 product and every sum below 2^24 is then exact in f32 in whatever order it is
@@ -9,7 +10,7 @@ rstd: 2^-24 of each, and 2^-24 of the result once more for dz or the scale."""
 import pytest
 import torch
 
-from tests.test_gpu_rows import DTYPES, F16, F32, LARGE, UNIT, WIDTHS
+from tests.test_gpu_rows import DTYPES, EPS, F16, F32, LARGE, UNIT, WIDTHS, rows_of, weights_of
 from vauss_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -69,3 +70,40 @@ def test_backward_of_exact_sums(cuda, dtype, rows, cols):
             factor = ops.dropout(torch.ones(rows, cols, device=cuda), 0.25, 3, 5).double()
             # the factor's own rounding (4/3 is not f32's) and the product's
             within(j.dx, r * factor, (wide + 2 * E * r.abs()) * 4 / 3, f"joined dx {layout}")
+
+
+@pytest.mark.parametrize("rows,cols", [(r, c) for r, c in SHAPES if c <= 4096 and r <= 70_000])
+def test_f32_rounding(cuda, rows, cols):
+    """f32 results within what their additions cost.  A row's sum of at most 4096 columns is at most 40 additions deep
+    (32 values of a thread as 16 pairs, a warp's 5, its CTA's at most 8 + 2, and the ends), so it is off by at most
+    40 E of the sum of magnitudes; a product or a difference by E of itself; rsqrt by 4 E.  dweight adds chains of at
+    most 1024 rows: with partial sums of random sign the error is about E sqrt(L / 6) of the root of the sum of
+    squares (L the chain), of which six are allowed, and 2 E for each term."""
+    x, _ = rows_of(cuda, rows, cols, F32, rows + cols)
+    w, b, _, _ = weights_of(cuda, cols, F32, cols)
+    x64, w64, b64 = x.double(), w.double(), b.double()
+    m64 = x64.mean(1, keepdim=True)
+    c64 = x64 - m64
+    v64 = (c64 * c64).mean(1, keepdim=True) + EPS
+    q64 = v64.rsqrt()
+    o = ops.layer_norm(x, w, b, EPS)
+    dm = 41 * E * x64.abs().mean(1, keepdim=True)  # of the mean
+    within(o.mean, m64[:, 0], dm[:, 0], "mean")
+    # variance: the squares of x - m (each off by E, the mean's error adds its square and cancels in the sum to first
+    # order), their sum, the quotient and eps; rstd half of that
+    dq = (0.5 * (44 * E + dm * dm / v64) + 4 * E) * q64
+    within(o.rstd, q64[:, 0], dq[:, 0], "rstd")
+    y64 = c64 * q64 * w64 + b64
+    within(o.y, y64, (w64 * q64).abs() * (dm + E * c64.abs()) + (c64 * w64).abs() * (dq + E * q64) + E * y64.abs(), "y")
+    dy, _ = rows_of(cuda, rows, cols, F32, rows + cols + 1)
+    g = ops.layer_norm_bwd(dy, x, w, o.mean, o.rstd)
+    d64, m, q = dy.double(), o.mean.double()[:, None], o.rstd.double()[:, None]
+    h = (x64 - m) * q
+    e = d64 * w64
+    m1, m2 = e.mean(1, keepdim=True), (e * h).mean(1, keepdim=True)
+    t = q * (e - m1 - h * m2)
+    d1, d2 = 42 * E * e.abs().mean(1, keepdim=True), 45 * E * (e * h).abs().mean(1, keepdim=True)
+    within(g.dx, t, q * (d1 + h.abs() * d2 + E * (2 * e.abs() + m1.abs() + 4 * (h * m2).abs())) + 2 * E * t.abs(), "dx")
+    share = E * (2 + 6 * (min(rows, 1024) / 6) ** 0.5)
+    within(g.dweight, (d64 * h).sum(0), share * (d64 * h).square().sum(0).sqrt() + 40 * E * (d64 * h).sum(0).abs() +
+           2 * E * (d64 * h).abs().max(), "dweight")
