@@ -122,3 +122,37 @@ def test_the_error_word_is_read(cuda):
     with pytest.raises(_native.VsError, match="TIMEOUT"):
         ops.check_device()
     ops.check_device(0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", BACKWARD + [(1_000, 64), (40_001, 12), (20_000, 64), (1_001, 4096)])
+def test_every_kernel_in_a_graph(cuda, dtype, rows, cols):
+    """Forward and backward of both norms and of dropout captured and replayed twice, the column sums by one CTA, by the
+    last one and by the joining kernel: the bits of direct calls."""
+    x, _ = rows_of(cuda, rows, cols, dtype, 1)
+    r, _ = rows_of(cuda, rows, cols, dtype, 2)
+    w, b, _, _ = weights_of(cuda, cols, F32, 3)
+
+    def step(o=None, g=None, n=None, gn=None, d=None):
+        o = ops.dropout_add_norm(x, r, w, b, 0.2, 5, 6, out=o)
+        g = ops.dropout_add_norm_bwd(x, r, o.z, w, o.mean, o.rstd, 0.2, 5, 6, out=g)
+        n = ops.layer_norm(x, w, b, out=n)
+        gn = ops.layer_norm_bwd(r, x, w, n.mean, n.rstd, out=gn)
+        return o, g, n, gn, ops.dropout(x, 0.2, 5, 7, out=d)
+
+    outs = step()
+    flat = [t for part in outs[:4] for t in vars(part).values()] + [outs[4]]
+    want = [t.clone() for t in flat]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            step(*outs)
+    for t in flat:
+        t.zero_()
+    torch.cuda.synchronize()
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(want, flat))
