@@ -107,3 +107,49 @@ def test_f32_rounding(cuda, rows, cols):
     share = E * (2 + 6 * (min(rows, 1024) / 6) ** 0.5)
     within(g.dweight, (d64 * h).sum(0), share * (d64 * h).square().sum(0).sqrt() + 40 * E * (d64 * h).sum(0).abs() +
            2 * E * (d64 * h).abs().max(), "dweight")
+
+
+# 16-bit rows that a warp holds with 22 to 30 values a lane where there are many of them
+MANY = [(14_300, c) for c in (487, 601, 703, 644, 700, 892, 706, 750, 822, 902, 958)] + \
+    [(28_500, c) for c in (900, 924, 956)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", SHAPES + MANY)
+def test_forward_of_exact_sums(cuda, dtype, rows, cols):
+    """The mean is the correctly rounded quotient of an exact sum, z of values without a mask exact.  For y and rstd:
+    the squares' sum of like signs is at most 100 additions deep (a thread's share of 140003 columns and the CTA's),
+    rsqrt is within 4 E, and y takes the mean's rounding, a difference, two products and a sum."""
+    gen = torch.Generator(device=cuda).manual_seed(rows + cols)
+    w = torch.exp2(torch.randint(-1, 2, (cols,), device=cuda, generator=gen).float())
+    b = torch.randint(-1, 2, (cols,), device=cuda, generator=gen).float()
+    for layout in ("plain", "strided"):
+        x = small_integers(cuda, rows, cols, dtype, 1, layout)
+        r = small_integers(cuda, rows, cols, dtype, 2, layout)
+        for joined in (False, True):
+            if joined:
+                o = ops.dropout_add_norm(x, r, w, b, 0.0, 1, 2)
+                assert torch.equal(o.z, x + r), layout
+                z = x.double() + r.double()
+            else:
+                o, z = ops.layer_norm(x, w, b), x.double()
+            mean = (z.sum(1) / cols).float()  # in f64: torch divides by a number as a product with its inverse
+            assert torch.equal(o.mean, mean), f"mean {layout}"
+            d = z - mean.double()[:, None]
+            v = (d * d).mean(1, keepdim=True) + EPS
+            q = v.rsqrt()
+            dq = (0.5 * 104 * E + 4 * E) * q
+            within(o.rstd, q[:, 0], dq[:, 0], f"rstd {layout}")
+            y = d * q * w.double() + b.double()
+            within(o.y, y, d.abs() * w.double() * (dq + 3 * E * q) + E * y.abs(), f"y {layout}")
+        o = ops.dropout_add_norm(x, r, w, b, 0.25, 1, 2)
+        factor = ops.dropout(torch.ones(rows, cols, device=cuda), 0.25, 1, 2).double()
+        z = r.double() + x.double() * factor
+        within(o.z, z, 3 * E * z.abs(), f"masked z {layout}")
+        z = o.z.double()
+        mean = z.mean(1, keepdim=True)
+        q = ((z - mean).square().mean(1, keepdim=True) + EPS).rsqrt()
+        dm, dq = 101 * E * mean, (0.5 * 104 * E + 4 * E) * q + 0.5 * q**3 * (101 * E * mean)**2
+        within(o.mean, mean[:, 0], dm[:, 0], f"masked mean {layout}")
+        y = (z - mean) * q * w.double() + b.double()
+        within(o.y, y, w.double() * (q * dm + (z - mean).abs() * (dq + 3 * E * q)) + E * y.abs(), f"masked y {layout}")

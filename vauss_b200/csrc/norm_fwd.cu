@@ -261,17 +261,27 @@ template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormF
 // rate, 32 lanes of 14 values 47 %; of 170: 16 lanes of 14 values 63 %, 32 lanes of 6
 // values 47 %).  Runs as wide as the columns allow: 300 bf16 columns in runs of four
 // 91 %, of two 61 %; 100 columns 76 and 70 %.  16-bit rows that more values a lane
-// hold go with those rather than with a CTA each (902 columns 74 and 55 %, 602 columns
-// 65 and 38 %; 31 values a lane for 801 columns 48 and 49 %, so not those).
+// hold go with those rather than with a CTA each (602 columns 65 and 38 %; 31 values a
+// lane for 801 columns 48 and 49 %, so not those), but 23 values a lane and more, a row
+// to a warp, only where each warp has enough of them to be busy: 750 columns, 4800 rows
+// 8.8 us and 8.9 with a CTA each, 1200 rows 6.0 and 5.2, 38400 rows 32 and 41; joined
+// 4800 rows 16.3 and 13.9, 38400 rows 71 and 77.  Multiples of four that runs of four do
+// not hold go by runs of two from twice as many rows on, where there is one input (924
+// columns, 71k rows 55 and 69 us, 38400 rows 35 and 40, 19200 rows 23.1 and 21.7;
+// joined, 38400 rows 78 and 77).
+constexpr uint64_t NORM_MANY = (uint64_t)B200_SMS * 3 * NORM_WARPS * 8;  // rows: 8 for each warp
 template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormFwd& f, bool* taken) {
+  const bool many = f.s.rows >= NORM_MANY;
   if constexpr (sizeof(T) == 2) {
     if (f.s.cols % 4 == 0) {
       switch (norm_fit(f.s.cols / 4, 4, {3, 5, 7}).k) {
         case 3: return run_kernel<T, 4, 3, kJoin>(ctx, f, taken);
         case 5: return run_kernel<T, 4, 5, kJoin>(ctx, f, taken);
-        case 7: return run_kernel<T, 4, 7, kJoin>(ctx, f, taken);
+        case 7:
+          if (f.s.cols > 640 && !many) return VS_OK;
+          return run_kernel<T, 4, 7, kJoin>(ctx, f, taken);
       }
-      return VS_OK;
+      if (kJoin || f.s.rows < 2 * NORM_MANY) return VS_OK;
     }
     if (f.s.cols % 2 == 0) {
       switch (norm_fit(f.s.cols / 2, 2, {3, 5, 7, 9}).k) {
@@ -282,7 +292,8 @@ template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormFw
       }
       switch (norm_fit(f.s.cols / 2, 2, {11, 15}).k) {
         case 11: return run_kernel<T, 2, 11, kJoin>(ctx, f, taken);
-        case 15: return run_kernel<T, 2, 15, kJoin>(ctx, f, taken);
+        case 15:
+          if (many) return run_kernel<T, 2, 15, kJoin>(ctx, f, taken);
       }
       return VS_OK;
     }
@@ -294,7 +305,7 @@ template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormFw
     case 15: return run_kernel<T, 1, 15, kJoin>(ctx, f, taken);
   }
   if constexpr (sizeof(T) == 2) {
-    if (norm_fit(f.s.cols, 1, {23}).k) return run_kernel<T, 1, 23, kJoin>(ctx, f, taken);
+    if (many && norm_fit(f.s.cols, 1, {23}).k) return run_kernel<T, 1, 23, kJoin>(ctx, f, taken);
   }
   return VS_OK;
 }
