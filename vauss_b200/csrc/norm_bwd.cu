@@ -21,13 +21,16 @@ template <typename T, int VEC, int K> constexpr int warp_ctas() {
   if (VEC * K > 20) return 2;
   return VEC * sizeof(T) == 16 && sizeof(T) == 4 ? 2 : 3;
 }
-// Bytes of a slot and input: f32 rows 2 KB, 16-bit rows of 128 bytes 2 KB (89 % of
-// the copy rate, 3 KB 82 %), longer ones 3 KB (rows of 256: 93 %, 2 KB 86 %).  Rows
-// that are not whole vectors and over 1.5 KB go two to a slot (780 bf16 columns 68 %,
-// one to a slot 47 %; shorter ones lose by slots of 4 KB, 460 columns 59 and 54 %).
-template <typename T, int VEC> constexpr uint32_t warp_slot(uint32_t row_bytes) {
-  if (VEC * sizeof(T) != 16 && row_bytes > 1536) return 4096;
-  return VEC * sizeof(T) == 16 && (sizeof(T) == 4 || row_bytes == 128) ? 2048 : 3072;
+// Bytes of a slot and input; `pass` bytes of rows go through a warp at once.  f32 rows
+// 2 KB, 16-bit rows 3 KB (share of the copy rate at 48 columns 73 %, in 2 KB 63 %, at
+// 128 columns 83 and 81 %, at 256 columns 86 and 79 %), but 2 KB for rows of up to 128
+// bytes whose passes fill that without a rest (8 columns 67 %, in 3 KB 60 %, 32 columns
+// 76 and 72 %, 64 columns 81 and 78 %; 16 columns 64 and 66 %, the rule's one loss).
+// Rows that are not whole vectors and over 1.5 KB go two to a slot (780 bf16 columns
+// 68 %, one to a slot 47 %; shorter ones lose by slots of 4 KB, 460 columns 59 and 54 %).
+template <typename T, int VEC> constexpr uint32_t warp_slot(uint32_t row_bytes, uint32_t pass) {
+  if (VEC * sizeof(T) != 16) return row_bytes > 1536 ? 4096 : 3072;
+  return sizeof(T) == 4 || (row_bytes <= 128 && 2048 % pass == 0) ? 2048 : 3072;
 }
 
 struct BwdArgs {
@@ -277,7 +280,8 @@ template <typename T, int VEC, int K, bool kJoin> vs_status run_kernel(vs_ctx* c
   // As in the forward, and the same for the plain and the joined kernel, so
   // that their weight gradients are the same sums in the same order.
   const uint32_t per_pass = 32u >> a.log_lanes;
-  uint32_t passes = warp_slot<T, VEC>(row_bytes) / (row_bytes * per_pass);
+  const uint32_t pass = row_bytes * per_pass;
+  uint32_t passes = warp_slot<T, VEC>(row_bytes, pass) / pass;
   const uint64_t share = (uint64_t)B200_SMS * per_sm * NORM_WARPS * per_pass;
   const uint64_t even = (a.rows + share - 1) / share;
   if (passes > even) passes = (uint32_t)even;
