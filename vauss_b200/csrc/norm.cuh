@@ -373,7 +373,14 @@ VSD float lanes_sum(float v, uint32_t lanes) {
   return v;
 }
 
-// sum / n with inv = 1 / n, correctly rounded for finite quotients
+// sum / n with inv = 1 / n rounded correctly, for a whole n below 2^16 (the columns of a
+// row): the correction of a quotient by its remainder that P. Markstein describes
+// ("Computation of elementary functions on the IBM RISC System/6000 processor", 1990).
+// q is within two units of its last place, and the remainder is a multiple of one unit,
+// since n is whole, and below 2^18 of them, so the fma gives it exactly; sum / n lies at
+// least 1 / 2n of a unit from the middle between two f32 values, far more than the rounded
+// inverse leaves in the second fma.  So the result is the correctly rounded quotient
+// wherever that is a normal number; an infinite one stays as it is.
 VSD float quotient(float sum, float n, float inv) {
   const float q = sum * inv;
   const float r = fmaf(fmaf(-q, n, sum), inv, q);
