@@ -112,10 +112,12 @@ def test_f32_rounding(cuda, rows, cols):
 # 16-bit rows that a warp holds with 22 to 30 values a lane where there are many of them
 MANY = [(14_300, c) for c in (487, 601, 703, 644, 700, 892, 706, 750, 822, 902, 958)] + \
     [(28_500, c) for c in (900, 924, 956)]
+# rows on a CTA with 16 and 32 values a thread, whole vectors and ragged
+ON_A_CTA = [(700, c) for c in (1536, 1538, 1543, 1544, 1601, 2040, 2047, 2048, 3500, 6001, 8192, 12_288, 16_000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols", SHAPES + MANY)
+@pytest.mark.parametrize("rows,cols", SHAPES + MANY + ON_A_CTA)
 def test_forward_of_exact_sums(cuda, dtype, rows, cols):
     """The mean is the correctly rounded quotient of an exact sum, z of values without a mask exact.  For y and rstd:
     the squares' sum of like signs is at most 100 additions deep (a thread's share of 140003 columns and the CTA's),

@@ -563,17 +563,20 @@ template <typename T, int K, int KG, bool kJoin> vs_status run(vs_ctx* ctx, cons
 }
 
 // Values per thread: 32 make fewer instructions per value, 16 more warps.  Forward,
-// bf16 rows of 4096: 32 values 94 %, 16 values 76 % of the copy rate; f16 rows of
-// 1030, whose ends take a warp, 47 and 61 %; joined f32 rows of 4096 42 and 68 %.
+// bf16 rows of 4096: 32 values 92 %, 16 values 74 % of the copy rate, of 1544 75 and 63 %
+// (from there on 16 values take more than 96 threads), of 1536 75 and 80 %, f16 rows of
+// 1030, whose ends take a warp, 51 and 60 %.  Plain f32 rows of 1536 82 and 89 %, of 4096
+// 90 and 93 %, of 12288 91 and 93 %; joined ones, whose vectors need a generator call
+// each, of 1536 80 and 81 %, of 2049 83 and 72 %, of 4096 94 and 86 %.
 template <typename T, bool kJoin> vs_status pick(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   constexpr int V = 16 / sizeof(T);
-  const uint32_t most = sizeof(T) == 2 ? 2047 : kJoin ? ~0u : 2048;  // columns for 16 values
+  const uint32_t most = sizeof(T) == 2 ? 1543 : kJoin ? 2047 : ~0u;  // columns for 16 values
   if (f.s.cols <= most) VS_TRY((run<T, 16 / V, kJoin>(ctx, f, taken)));
   if (!*taken) VS_TRY((run<T, 32 / V, kJoin>(ctx, f, taken)));
   return VS_OK;
 }
-// Backward: bf16 rows of 4096, joined, 16 values 77 %, 32 values 62 %; the joined
-// f32 kernel, whose vectors need a generator call each, holds 8 where it can.
+// Backward: bf16 rows of 4096, joined, 17k of them, 16 values 83 %, 32 values 51 %; the
+// joined f32 kernel holds 8 where it can (8192 x 4096 93 %, 32 values 42 %).
 template <typename T, bool kJoin> vs_status pick(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   constexpr int V = 16 / sizeof(T), S = 16 / V, L = 32 / V;
   if constexpr (sizeof(T) == 4) VS_TRY((run<T, kJoin ? 2 : S, 2, kJoin>(ctx, f, taken)));
