@@ -155,3 +155,21 @@ def test_forward_of_exact_sums(cuda, dtype, rows, cols):
         within(o.mean, mean[:, 0], dm[:, 0], f"masked mean {layout}")
         y = (z - mean) * q * w.double() + b.double()
         within(o.y, y, w.double() * (q * dm + (z - mean).abs() * (dq + 3 * E * q)) + E * y.abs(), f"masked y {layout}")
+
+
+@pytest.mark.parametrize("rows,cols,layout", [(100_000_000, 1, "plain"), (60_000_000, 2, "plain"), (100_000_000, 1, "strided"),
+                                              (200_000, 1030, "plain"), (30_000, 12_300, "plain")])
+def test_sums_of_many_alike_rows(cuda, rows, cols, layout):
+    """The gradient of a mean: every term of dbias and dweight is the same, so that the roundings of a chain of sums all
+    go one way.  No chain is longer than 256 terms: of a tile's sums (48 terms each) or of rows, then the lanes' (32),
+    the warps' (16) and a share of the CTAs' (100 here); a chain of n alike terms is off by at most (n + 1) / 2 roundings
+    of E: 230 E in all."""
+    dy = torch.full((rows, cols), 0.7123, device=cuda)
+    if layout == "strided":
+        dy = torch.full((rows, cols + 1), 0.7123, device=cuda)[:, 1:]
+    z = torch.ones(rows, cols, device=cuda)
+    mean, rstd = torch.zeros(rows, device=cuda), torch.ones(rows, device=cuda)
+    want = float(dy[0, 0].double()) * rows
+    g = ops.layer_norm_bwd(dy, z, torch.ones(cols, device=cuda), mean, rstd)
+    for got in (g.dweight, g.dbias):
+        assert float((got.double() / want - 1).abs().max()) <= 230 * E

@@ -400,7 +400,8 @@ vs_status norm_backward(vs_ctx* ctx, const char* what, int32_t dtype, Shape s, c
   // reads the weight, which dweight may overwrite, so the sums are joined after them.
   const bool want = dweight || dbias;
   const uint32_t col_blocks = (s.cols + COLS_WIDE - 1) / COLS_WIDE;
-  const uint64_t even = 1184 / col_blocks + 1;  // CTAs for every SM
+  uint64_t even = 1184 / col_blocks + 1;  // CTAs for every SM, and no thread with more than NORM_CHAIN rows
+  if (even < s.rows / (8 * NORM_CHAIN) + 1) even = s.rows / (8 * NORM_CHAIN) + 1;
   const uint64_t most = (s.rows + 15) / 16;
   const uint32_t strips = (uint32_t)(even < most ? even : most);
   NormScratch scratch;

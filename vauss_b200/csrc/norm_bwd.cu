@@ -33,6 +33,11 @@ template <typename T, int VEC> constexpr uint32_t warp_slot(uint32_t row_bytes, 
   return sizeof(T) == 4 || (row_bytes <= 128 && 2048 % pass == 0) ? 2048 : 3072;
 }
 
+// Whether a lane's values are few enough for a second set of sums: those of a tile.
+// Narrow rows need it: at one column a lane has 1055 rows of a call of 100M, and 256 of
+// them to a CTA make so many CTAs that 16M x 3 f32 takes 10 % longer.
+template <int VEC, int K> constexpr bool sums_twice = VEC * K <= 6;
+
 struct BwdArgs {
   uint64_t rows;
   uint32_t cols, tile_rows, log_lanes, slot, stat_slot, bits, stages, inputs;
@@ -101,6 +106,9 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
   part.weights(a.w.weight, a.w.dtype, 1.0f, w);
 #pragma unroll
   for (int i = 0; i < PAIRS; ++i) dw[i] = db[i] = both(0.0f);
+  // where registers allow, a tile's rows are added up and then their sum to the others'
+  constexpr bool kTwice = sums_twice<VEC, K>;
+  float2 tile_w[kTwice ? PAIRS : 1], tile_b[kTwice ? PAIRS : 1];
   const float n = (float)a.cols, inv = 1.0f / n;
   __syncwarp();
 
@@ -135,6 +143,10 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
       fill_bits(d, i0, rows * a.cols, bits, lane, 32);
       __syncwarp();
     }
+    if constexpr (kTwice) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) tile_w[i] = tile_b[i] = both(0.0f);
+    }
     for (uint32_t p = 0; p < rows; p += per_pass) {
       // a lane beyond the tile's rows computes its last row and leaves nothing
       const bool live = p + sub < rows;
@@ -161,8 +173,9 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
       float2 s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {  // g is zero for values that are not the row's
-        dw[i] = fma2(g[i], h[i], dw[i]);
-        db[i] = add2(db[i], g[i]);
+        float2 &sw = kTwice ? tile_w[kTwice ? i : 0] : dw[i], &sb = kTwice ? tile_b[kTwice ? i : 0] : db[i];
+        sw = fma2(g[i], h[i], sw);
+        sb = add2(sb, g[i]);
       }
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
@@ -192,6 +205,13 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) part.set(t, i, g[i]);
         part.store(kDirect ? static_cast<T*>(a.dx) + i0 + r_at : gr, t);
+      }
+    }
+    if constexpr (kTwice) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        dw[i] = add2(dw[i], tile_w[i]);
+        db[i] = add2(db[i], tile_b[i]);
       }
     }
     if (kDirect) {
@@ -307,7 +327,9 @@ template <typename T, int VEC, int K, bool kJoin> vs_status run_kernel(vs_ctx* c
   a.dx = f.dx; a.dresidual = f.dresidual;
   a.err = ctx->d_err;
   const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + NORM_WARPS - 1) / NORM_WARPS;
-  const uint64_t all = (uint64_t)per_sm * B200_SMS;
+  const uint64_t once = (uint64_t)per_sm * B200_SMS;
+  const uint64_t chain = NORM_CHAIN * (sums_twice<VEC, K> ? a.tile_rows : per_pass);  // a warp's rows at most
+  const uint64_t all = once * (a.rows / (once * NORM_WARPS * chain) + 1);
   const uint32_t grid = (uint32_t)(all < most ? all : most);
   const bool want = f.dweight || f.dbias;
   NormScratch scratch;

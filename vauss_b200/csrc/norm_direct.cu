@@ -272,8 +272,10 @@ struct Shape {
   uint32_t grid, threads, log_lanes;
 };
 // `alone`: up to this many rounds of rows stay on one CTA (a second launch costs
-// about 3 us of the host and of the GPU, a round about 1 us).
-template <int VEC, int K, bool kCta> Shape shape_of(const NormShape& s, uint32_t warps, uint32_t alone) {
+// about 3 us of the host and of the GPU, a round about 1 us).  No CTA takes more than
+// `chain` rounds.
+template <int VEC, int K, bool kCta>
+Shape shape_of(const NormShape& s, uint32_t warps, uint32_t alone, uint64_t chain) {
   const uint32_t chunks = (s.cols + VEC - 1) / VEC;
   Shape l{0, warps * 32, 0};
   uint64_t most = s.rows;
@@ -284,19 +286,20 @@ template <int VEC, int K, bool kCta> Shape shape_of(const NormShape& s, uint32_t
     const uint32_t rows = warps * (32u >> l.log_lanes);
     most = (s.rows + rows - 1) / rows;
   }
-  const uint64_t room = (uint64_t)B200_SMS * (l.threads >= 512 ? 1 : 512 / l.threads);
+  uint64_t room = (uint64_t)B200_SMS * (l.threads >= 512 ? 1 : 512 / l.threads);
+  room *= most / (room * chain) + 1;
   l.grid = most <= alone ? 1 : (uint32_t)(room < most ? room : most);
   return l;
 }
 
 template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status launch(vs_ctx* ctx, const NormFwd& f) {
-  const Shape l = shape_of<VEC, K, kCta>(f.s, FWD_WARPS, 1);
+  const Shape l = shape_of<VEC, K, kCta>(f.s, FWD_WARPS, 1, ~0u);
   norm_direct_fwd_kernel<T, VEC, K, kJoin, kCta><<<l.grid, l.threads, 0, ctx->stream>>>(f, l.log_lanes, f.d);
   ++ctx->launches;
   return vs_cuda(ctx, cudaGetLastError(), "norm launch");
 }
 template <typename T, int VEC, int K, bool kJoin, bool kCta> vs_status launch(vs_ctx* ctx, const NormBwd& f) {
-  const Shape l = shape_of<VEC, K, kCta>(f.s, BWD_WARPS, 4);
+  const Shape l = shape_of<VEC, K, kCta>(f.s, BWD_WARPS, 4, NORM_CHAIN);
   const bool want = (f.dweight || f.dbias) && l.grid > 1;
   NormScratch scratch;
   if (want) VS_TRY(norm_scratch_begin(ctx, (size_t)l.grid * (2 * f.s.cols + 3), &scratch));

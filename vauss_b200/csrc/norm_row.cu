@@ -475,12 +475,12 @@ template <typename T, int K> uint32_t row_threads(uint32_t cols) {
   return ((cols / V + K - 1) / K + 31) / 32 * 32 + (cols % V ? 32 : 0);
 }
 
-// Grid and slots of a shape; `held` bytes per thread stand beside the ring, and
-// the grid is that of CTAs of `grid_threads` threads of `sm_threads` with `inputs`
-// inputs.  CTAs beyond what keeps `flight` bytes on their way only queue at the
-// DRAM: one input, f32 rows of 1024, 6 CTAs 95 % of the copy rate, 8 CTAs 85 %; two
-// inputs, bf16 rows of 4096, 3 CTAs 96 %, 4 CTAs 76 %.  False where the slots do not
-// fit.
+// Grid and slots of a shape; `held` bytes per thread stand beside the ring (of the
+// backward, whose threads add up NORM_CHAIN rows each at most), and the grid is that of
+// CTAs of `grid_threads` threads of `sm_threads` with `inputs` inputs.  CTAs beyond what
+// keeps `flight` bytes on their way only queue at the DRAM: one input, f32 rows of 1024,
+// 6 CTAs 95 % of the copy rate, 8 CTAs 85 %; two inputs, bf16 rows of 4096, 3 CTAs 96 %,
+// 4 CTAs 76 %.  False where the slots do not fit.
 template <typename T>
 bool lay_out(RowArgs* a, uint32_t threads, uint32_t grid_threads, uint32_t sm_threads, uint32_t inputs, uint32_t held,
              uint32_t* grid, size_t* smem) {
@@ -497,7 +497,8 @@ bool lay_out(RowArgs* a, uint32_t threads, uint32_t grid_threads, uint32_t sm_th
   if (bytes(inputs, 1) > room()) return false;
   a->stages = bytes(a->inputs, 2) <= room() ? 2 : 1;
   *smem = bytes(a->inputs, a->stages);
-  const uint64_t full = (uint64_t)per_sm * B200_SMS / V * V;
+  const uint64_t once = (uint64_t)per_sm * B200_SMS / V * V;
+  const uint64_t full = held ? once * (a->rows / (once * NORM_CHAIN) + 1) : once;
   *grid = (uint32_t)(a->rows < full ? a->rows : full);
   return true;
 }
