@@ -119,3 +119,39 @@ def test_f16_fit_lowers_the_loss(cuda):
     losses = feature_head.fit(steps=40, dtype=torch.float16)
     assert all(np.isfinite(losses))
     assert np.mean(losses[-4:]) + 0.2 < 0.6 * (np.mean(losses[:4]) + 0.2)
+
+
+@pytest.mark.parametrize("blocks", [0, 2])
+def test_dropped_features(cuda, blocks):
+    """Dropout of the features before the first norm, forward and gradient, against autograd; none outside training."""
+    n, width, p_in = 301, 40, 0.3
+    head = feature_head.FeatureHead(width, 40, blocks, 0.25, cuda, torch.float32, seed=5, p_in=p_in)
+    gen = torch.Generator().manual_seed(n)
+    x, c = torch.randn(n, width, generator=gen), torch.randn(n, 3, generator=gen)
+    # columns of a wider buffer
+    out = head.forward(torch.cat((x, x), 1).to(cuda)[:, :width])
+    dx = head.backward(c.to(cuda))
+    w = {k: v.detach().cpu().double().requires_grad_() for k, v in head.params.items()}
+    f = x.double().requires_grad_()
+    keep, scale = keep_mask(f.numel(), p_in, 5, 2**63 + 1)
+    h = f * keep.view(f.shape) * scale
+    y = _norm(h, w["norm0.weight"], w["norm0.bias"])
+    for k in range(blocks):
+        r = torch.relu(y @ w[f"block{k}.w1"]) @ w[f"block{k}.w2"]
+        keep, scale = keep_mask(r.numel(), 0.25, 5, 1 * 2 + k)
+        h = h + r * keep.view(r.shape) * scale
+        y = _norm(h, w[f"norm{k + 1}.weight"], w[f"norm{k + 1}.bias"])
+    want = y @ w["out"]
+    want.backward(c.double())
+    for what, got, ref in [("out", out, want.detach()), ("features", dx, f.grad)] + \
+            [(k, head.grads[k], w[k].grad) for k in head.params]:
+        err = float((got.detach().cpu().double() - ref).abs().max())
+        assert err <= REL * max(1.0, float(ref.abs().max())), f"{what}: {err}"
+    plain = feature_head.FeatureHead(width, 40, blocks, 0.25, cuda, torch.float32, seed=5)
+    assert torch.equal(head.forward(x.to(cuda), train=False), plain.forward(x.to(cuda), train=False))
+
+
+def test_fit_with_dropped_features(cuda):
+    losses = feature_head.fit(steps=40, p_in=0.02)
+    assert all(np.isfinite(losses))
+    assert np.mean(losses[-4:]) + 0.2 < 0.6 * (np.mean(losses[:4]) + 0.2)

@@ -4,8 +4,9 @@ reference).
 
 The blocks are the usual ones, h <- h + dropout(relu(norm(h) W1) W2).  Between
 the matrix products (plain library products through torch) stand the row
-operators of ``ops``: ``layer_norm`` at the entry, ``dropout_add_norm`` between
-blocks, which sums, drops and normalises in one pass, and their gradients.
+operators of ``ops``: ``dropout`` of the features where it is asked for,
+``layer_norm`` at the entry, ``dropout_add_norm`` between blocks, which sums,
+drops and normalises in one pass, and their gradients.
 Weights and the optimizer are f32; rows are f32, f16 or bf16.  The gradient of a
 loss over an image is far below f16's range, so an f16 head scales what enters
 its backward by a power of two and takes it out of the results again.
@@ -22,12 +23,14 @@ from . import ops
 
 class FeatureHead:
     """forward(features) -> colour offsets [N, 3]; backward(gradient of those) -> gradient of the features, with the
-    parameters' gradients in ``grads``.  One forward is kept for one backward."""
+    parameters' gradients in ``grads``.  One forward is kept for one backward.  ``p`` drops the blocks' branches, ``p_in``
+    the features."""
 
-    def __init__(self, width: int, hidden: int, blocks: int, p: float, device, dtype=torch.bfloat16, seed: int = 0):
-        assert width > 0 and hidden > 0 and blocks >= 0 and 0.0 <= p <= 1.0
+    def __init__(self, width: int, hidden: int, blocks: int, p: float, device, dtype=torch.bfloat16, seed: int = 0,
+                 p_in: float = 0.0):
+        assert width > 0 and hidden > 0 and blocks >= 0 and 0.0 <= p <= 1.0 and 0.0 <= p_in <= 1.0
         gen = torch.Generator(device=device).manual_seed(seed)
-        self.blocks, self.p, self.dtype, self.seed, self.step = blocks, p, dtype, seed, 0
+        self.blocks, self.p, self.p_in, self.dtype, self.seed, self.step = blocks, p, p_in, dtype, seed, 0
         self.params: dict[str, torch.Tensor] = {}
 
         def weight(name, rows, cols, gain):
@@ -49,10 +52,13 @@ class FeatureHead:
     def forward(self, features: torch.Tensor, train: bool = True) -> torch.Tensor:
         """features [N, width] in the head's type.  ``train`` draws a new mask per call and block."""
         assert features.dtype == self.dtype, f"features are {features.dtype}, the head is {self.dtype}"
-        p = self.p if train else 0.0
+        p, p_in = (self.p, self.p_in) if train else (0.0, 0.0)
         if train:
             self.step += 1
         w = self.params
+        offset_in = (1 << 63) + self.step  # apart from the blocks'
+        if p_in:
+            features = ops.dropout(features.contiguous(), p_in, self.seed, offset_in)
         first = ops.layer_norm(features, w["norm0.weight"], w["norm0.bias"])
         h, y, kept = features, first.y, []
         for k in range(self.blocks):
@@ -62,12 +68,12 @@ class FeatureHead:
             o = ops.dropout_add_norm(r, h, w[f"norm{k + 1}.weight"], w[f"norm{k + 1}.bias"], p, self.seed, offset)
             kept.append((y, a, o, offset))
             h, y = o.z, o.y
-        self._saved = (features, first, kept, y, p)
+        self._saved = (features, first, kept, y, p, p_in, offset_in)
         return (y @ self._w("out")).float()
 
     def backward(self, dout: torch.Tensor) -> torch.Tensor:
         """The features' gradient, in the head's type (f32 for an f16 head, whose range small ones would leave)."""
-        features, first, kept, y, p = self._saved
+        features, first, kept, y, p, p_in, offset_in = self._saved
         g, w = self.grads, self.params
         scale = _f16_scale(dout) if self.dtype == torch.float16 else None
         dout = (dout if scale is None else dout * scale).to(self.dtype)
@@ -94,8 +100,10 @@ class FeatureHead:
         leave("norm0.weight", d.dweight)
         leave("norm0.bias", d.dbias)
         if scale is None:
-            return d.dx if dz is None else d.dx + dz
-        return (d.dx.float() if dz is None else d.dx.float() + dz.float()) / scale
+            dx = d.dx if dz is None else d.dx + dz
+        else:
+            dx = (d.dx.float() if dz is None else d.dx.float() + dz.float()) / scale
+        return ops.dropout_bwd(dx, p_in, self.seed, offset_in, out=dx) if p_in else dx
 
 
 def _f16_scale(dout: torch.Tensor) -> torch.Tensor:
@@ -126,14 +134,14 @@ def lit_views(n_views: int = 4, device="cuda:0"):
 
 
 def fit(steps: int = 60, width: int = 64, hidden: int = 128, blocks: int = 2, p: float = 0.1, lr: float = 3e-3,
-        device="cuda:0", dtype=torch.bfloat16) -> list[float]:
+        device="cuda:0", dtype=torch.bfloat16, p_in: float = 0.0) -> list[float]:
     """Trains a head (and nothing else) on ``lit_views``; returns the loss of every step."""
     splats, views = lit_views(device=device)
     cfg = ops.render_cfg(0, mip=True)
     gen = torch.Generator(device=device).manual_seed(1)
     mix = torch.randn(3, width, device=device, generator=gen)
     features = torch.sin(3.0 * splats.transforms[:, :3] @ mix).to(dtype)  # what a splat's place tells
-    head = FeatureHead(width, hidden, blocks, p, device, dtype)
+    head = FeatureHead(width, hidden, blocks, p, device, dtype, p_in=p_in)
     opt = torch.optim.Adam(head.params.values(), lr=lr)
     n = splats.num_splats
     base, frame, losses = splats.sh_coeffs[:, 0, :], ops.Frame(ops.context(splats.transforms.device)), []
