@@ -15,6 +15,7 @@ class FakeContext:
         FakeContext.made += 1
 
     def bind(self):
+        self.stream = ops._raw_stream(self.device)
         return self
 
     def check(self, status):
@@ -27,6 +28,7 @@ def fake(monkeypatch):
     monkeypatch.setattr(ops, "_contexts", {})
     monkeypatch.setattr(ops, "_idle_contexts", [], raising=False)
     monkeypatch.setattr(FakeContext, "made", 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 0)
     if hasattr(ops, "_RowContexts"):
         monkeypatch.setattr(ops, "_row_contexts", ops._RowContexts())
 

@@ -43,6 +43,7 @@ class Context:
     def bind(self) -> "Context":
         s = _raw_stream(self.device)  # the current stream's handle, without a Stream object around it
         N.check(self.h, self.lib.vs_ctx_set_stream(self.h, s))
+        self.stream = s
         return self
 
     def check(self, status: int):
@@ -452,7 +453,9 @@ def _row_context(device: int) -> Context:
             at = next((k for k, c in enumerate(_idle_contexts) if c.device == device), None)
             ctx = Context(device) if at is None else _idle_contexts.pop(at)
         _row_contexts.of[device] = ctx
-    return ctx.bind()
+        return ctx.bind()
+    # nobody else sets this context's stream, so it is set where it changes only
+    return ctx if ctx.stream == _raw_stream(device) else ctx.bind()
 
 
 def _row_shape(t: torch.Tensor):
