@@ -113,7 +113,7 @@ def test_f32_rounding(cuda, rows, cols):
 MANY = [(14_300, c) for c in (487, 601, 703, 644, 700, 892, 706, 750, 822, 902, 958)] + \
     [(28_500, c) for c in (900, 924, 956)]
 # rows on a CTA with 16 and 32 values a thread, whole vectors and ragged
-ON_A_CTA = [(700, c) for c in (1536, 1538, 1543, 1544, 1601, 2040, 2047, 2048, 3500, 6001, 8192, 12_288, 16_000)]
+ON_A_CTA = [(700, c) for c in (1536, 1538, 1543, 1544, 1601, 2040, 2047, 2048, 3500, 6001, 8192, 11_501, 12_288, 16_000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

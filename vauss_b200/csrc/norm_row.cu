@@ -574,6 +574,8 @@ template <typename T, bool kJoin> vs_status pick(vs_ctx* ctx, const NormFwd& f, 
   const uint32_t most = sizeof(T) == 2 ? 1543 : kJoin ? 2047 : ~0u;  // columns for 16 values
   if (f.s.cols <= most) VS_TRY((run<T, 16 / V, kJoin>(ctx, f, taken)));
   if (!*taken) VS_TRY((run<T, 32 / V, kJoin>(ctx, f, taken)));
+  // beside their ends' warp, 16 values a thread hold 512 columns more of joined rows
+  if (kJoin && !*taken && f.s.cols > most) VS_TRY((run<T, 16 / V, kJoin>(ctx, f, taken)));
   return VS_OK;
 }
 // Backward: bf16 rows of 4096, joined, 17k of them, 16 values 83 %, 32 values 51 %; the
