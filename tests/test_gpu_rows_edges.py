@@ -156,3 +156,43 @@ def test_every_kernel_in_a_graph(cuda, dtype, rows, cols):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, c) for a, c in zip(want, flat))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", BACKWARD + [(1_000, 3), (15_000, 750), (300, 703), (9, 1), (1_000, 1030)])
+def test_nan_and_infinity_stay_in_their_rows(cuda, dtype, rows, cols):
+    """Rows that hold a NaN or an infinity leave the other rows' results as they are, bit for bit, wherever the kernels
+    keep rows side by side; their own are NaN (of one column: NaN too, from inf - inf)."""
+    clean = [rows_of(cuda, rows, cols, dtype, k)[0] for k in range(3)]
+    w, b, _, _ = weights_of(cuda, cols, F32, 4)
+    bad = torch.arange(rows, device=cuda) % 7 == 3
+    bad[0] = bad[-1] = True
+    if rows == 1:
+        bad[:] = True
+    value = torch.where(torch.arange(rows, device=cuda) % 2 == 0, float("nan"), float("inf")).to(dtype)
+    at = torch.arange(rows, device=cuda) % cols
+    x = clean[0].clone()
+    x[bad, at[bad]] = value[bad]
+    for strided in (False, True):
+        def lay(t):
+            if not strided:
+                return t
+            wide = torch.full((rows, cols + 3), float("nan"), dtype=dtype, device=cuda)
+            wide[:, 1:1 + cols] = t
+            return wide[:, 1:1 + cols]
+        want, got = ops.layer_norm(lay(clean[0]), w, b), ops.layer_norm(lay(x), w, b)
+        for k in ("y", "mean", "rstd"):
+            assert torch.equal(getattr(got, k)[~bad], getattr(want, k)[~bad]), f"{k} strided {strided}"
+        assert bool(got.y[bad].isnan().all())
+        want = ops.dropout_add_norm(lay(clean[1]), lay(clean[0]), w, b, 0.25, 1, 2)
+        got = ops.dropout_add_norm(lay(clean[1]), lay(x), w, b, 0.25, 1, 2)
+        for k in ("y", "z", "mean", "rstd"):
+            assert torch.equal(getattr(got, k)[~bad], getattr(want, k)[~bad]), f"joined {k} strided {strided}"
+        o = ops.layer_norm(clean[0], w, b)
+        for args, ref in (((clean[1], x), (clean[1], clean[0])), ((x, clean[1]), (clean[0], clean[1]))):  # in z, in dy
+            args, ref = [lay(t) for t in args], [lay(t) for t in ref]
+            g, r = ops.layer_norm_bwd(*args, w, o.mean, o.rstd), ops.layer_norm_bwd(*ref, w, o.mean, o.rstd)
+            assert torch.equal(g.dx[~bad], r.dx[~bad]), f"dx strided {strided}"
+            j = ops.dropout_add_norm_bwd(args[0], lay(clean[2]), args[1], w, o.mean, o.rstd, 0.25, 1, 2)
+            q = ops.dropout_add_norm_bwd(ref[0], lay(clean[2]), ref[1], w, o.mean, o.rstd, 0.25, 1, 2)
+            assert torch.equal(j.dx[~bad], q.dx[~bad]) and torch.equal(j.dresidual[~bad], q.dresidual[~bad])
