@@ -360,14 +360,15 @@ template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormB
   return VS_OK;
 }
 
-// Runs of four where they cost less than runs of two (300 bf16 columns 78 %, in runs of
-// two 60 %; 100 columns in runs of two 62 %, of four 52 %), but on one lane up to 16
-// values only (12 columns 63 %, in runs of two 53 %; 20 columns, 3.2M rows 59 and 69 %,
-// 200k rows 41 and 23 us, since the lanes' column sums are added one lane after another).
-// 28 values a lane leave registers for two CTAs only, so they are for rows that nothing
-// else holds (700 columns 62 %, a CTA per row 43 %; 28 columns 57 %, 14 values on two
-// lanes 77 %); so are 22 to 30 in runs of two (750 columns 60 and 45 %, 902 columns 66
-// and 53 %; joined 902 columns 47 and 50 %, which the plain rows' choice decides).
+// Runs of four where they cost less than runs of two (64M bf16 values in 300 columns
+// 71 %, in runs of two 57 %; 100 columns in runs of two 62 %, of four 52 %), but on one
+// lane up to 16 values only (12 columns 63 %, in runs of two 53 %; 20 columns, 3.2M rows
+// 59 and 69 %, 200k rows 41 and 23 us, since the lanes' column sums are added one lane
+// after another).  28 values a lane leave registers for two CTAs only, so they are for
+// rows that nothing else holds (700 columns 62 %, a CTA per row 43 %; 28 columns 57 %,
+// 14 values on two lanes 70 %); so are 22 to 30 in runs of two (750 columns 60 and 45 %,
+// 902 columns 66 and 53 %; joined 902 columns 47 and 50 %, which the plain rows' choice
+// decides).
 template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormBwd& f, bool* taken) {
   if constexpr (sizeof(T) == 2) {
     const uint32_t cols = f.s.cols;

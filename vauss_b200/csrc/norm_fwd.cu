@@ -259,18 +259,18 @@ template <typename T, bool kJoin> vs_status run_vectors(vs_ctx* ctx, const NormF
 
 // Blocks of K runs, K odd (bf16 rows of 250: 16 lanes of 18 values 77 % of the copy
 // rate, 32 lanes of 14 values 47 %; of 170: 16 lanes of 14 values 63 %, 32 lanes of 6
-// values 47 %).  Runs as wide as the columns allow: 300 bf16 columns in runs of four
-// 91 %, of two 61 %; 100 columns 76 and 70 %; where a lane holds a row on its own it
-// depends on their number (20 columns, 3.2M rows 53 us, in runs of two 49, 200k rows 6.4
-// and 7.3; joined, 3.2M rows 112 and 130).  16-bit rows that more values a lane hold go
-// with those rather than with a CTA each (602 columns 65 and 38 %; 31 values a lane for
-// 801 columns 48 and 49 %, so not those), but 23 values a lane and more, a row to a warp,
-// only where each warp has enough of them to be busy: 750 columns, 4800 rows 8.8 us and
-// 8.9 with a CTA each, 1200 rows 6.0 and 5.2, 38400 rows 32 and 41; joined 4800 rows 16.3
-// and 13.9, 38400 rows 71 and 77.  Multiples of four that runs of four do not hold go by
-// runs of two from twice as many rows on, where there is one input (924 columns, 71k rows
-// 55 and 69 us, 38400 rows 35 and 40, 19200 rows 23.1 and 21.7; joined, 38400 rows 78 and
-// 77).
+// values 47 %).  Runs as wide as the columns allow: 64M bf16 values in 300 columns in
+// runs of four 82 %, of two 57 %, in 100 columns 70 and 65 %; where a lane holds a row
+// on its own it depends on their number (20 columns, 3.2M rows 53 us, in runs of two 49,
+// 200k rows 6.4 and 7.3; joined, 3.2M rows 112 and 130).  16-bit rows that more values a
+// lane hold go with those rather than with a CTA each (602 columns 65 and 38 %; 31 values
+// a lane for 801 columns 48 and 49 %, so not those), but 23 values a lane and more, a row
+// to a warp, only where each warp has enough of them to be busy: 750 columns, 4800 rows
+// 8.8 us and 8.9 with a CTA each, 1200 rows 6.0 and 5.2, 38400 rows 32 and 41; joined
+// 4800 rows 16.3 and 13.9, 38400 rows 71 and 77.  Multiples of four that runs of four do
+// not hold go by runs of two from twice as many rows on, where there is one input (924
+// columns, 69k rows 55 and 69 us, 38400 rows 35 and 40, 19200 rows 23.1 and 21.7; joined,
+// 38400 rows 78 and 77).
 constexpr uint64_t NORM_MANY = (uint64_t)B200_SMS * 3 * NORM_WARPS * 8;  // rows: 8 for each warp
 template <typename T, bool kJoin> vs_status run_blocks(vs_ctx* ctx, const NormFwd& f, bool* taken) {
   const bool many = f.s.rows >= NORM_MANY;
