@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 3) norm_bwd_rows_kernel(Shape s, 
                                                                     T* dresidual) {
   __shared__ float scratch[33];
   const float cols = (float)s.cols;
+  launch_next();
   for (uint64_t r = blockIdx.x; r < s.rows; r += gridDim.x) {
     const float m = mean[r], q = rstd[r];
     const T *gy = dy.row(r), *zr = z.row(r), *gz = kJoin && dz.p ? dz.row(r) : nullptr;

@@ -544,10 +544,11 @@ inline NormFit norm_fit(uint32_t runs, int width, std::initializer_list<int> cho
   return best;
 }
 
-// Rows that a thread of the backward adds up one by one, at most: the error of a chain
-// grows with its length, by half a unit a row where the terms are alike (of a mean's
-// gradient, 1055 rows 1.6e-5 of the sum, 256 rows 3.8e-6).  Beyond it there are more CTAs
-// than an SM holds at once, which add up fewer rows each.
+// Rows that a thread of the backward adds up one by one, at most (four times as many for
+// a tile kernel's lane of more than six values): the error of a chain grows with its
+// length, by half a unit a row where the terms are alike (of a mean's gradient, 1055 rows
+// 1.6e-5 of the sum, 256 rows 3.8e-6).  Beyond it there are more CTAs than an SM holds at
+// once, which add up fewer rows each.
 constexpr uint64_t NORM_CHAIN = 256;
 
 // The streaming kernels take contiguous rows on 16-byte aligned buffers: tiles of

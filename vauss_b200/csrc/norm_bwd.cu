@@ -23,14 +23,16 @@ template <typename T, int VEC, int K> constexpr int warp_ctas() {
 }
 // Bytes of a slot and input; `pass` bytes of rows go through a warp at once.  f32 rows
 // 2 KB, 16-bit rows 3 KB (share of the copy rate at 48 columns 73 %, in 2 KB 63 %, at
-// 128 columns 83 and 81 %, at 256 columns 86 and 79 %), but 2 KB for rows of up to 128
-// bytes whose passes fill that without a rest (8 columns 67 %, in 3 KB 60 %, 32 columns
-// 76 and 72 %, 64 columns 81 and 78 %; 16 columns 64 and 66 %, the rule's one loss).
-// Rows that are not whole vectors and over 1.5 KB go two to a slot (780 bf16 columns
-// 68 %, one to a slot 47 %; shorter ones lose by slots of 4 KB, 460 columns 59 and 54 %).
+// 128 columns 83 and 81 %, at 256 columns 86 and 79 %), but 2 KB for rows of 64 to 128
+// bytes whose passes fill that without a rest (32 columns 76 %, in 3 KB 72 %, joined 81
+// and 75 %, joined without a mask 73 and 73 %; 64 columns 81 and 78 %).  Shorter rows, a
+// lane each: 16 columns 66 %, in 2 KB 64 %; 8 columns 60 and 67 %, joined 63 and 70 %, but
+// without a mask 79 and 67 %.  Rows that are not whole vectors and over 1.5 KB go two to a
+// slot (780 bf16 columns 68 %, one to a slot 47 %; shorter ones lose by slots of 4 KB, 460
+// columns 59 and 54 %).
 template <typename T, int VEC> constexpr uint32_t warp_slot(uint32_t row_bytes, uint32_t pass) {
   if (VEC * sizeof(T) != 16) return row_bytes > 1536 ? 4096 : 3072;
-  return sizeof(T) == 4 || (row_bytes <= 128 && 2048 % pass == 0) ? 2048 : 3072;
+  return sizeof(T) == 4 || (row_bytes >= 64 && row_bytes <= 128 && 2048 % pass == 0) ? 2048 : 3072;
 }
 
 // Whether a lane's values are few enough for a second set of sums: those of a tile.
@@ -61,6 +63,7 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
   constexpr bool kBits = kJoin && VEC != 8;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[NORM_WARPS][NORM_STAGES];
+  __shared__ uint32_t gave_up[NORM_WARPS];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const uint32_t lanes = 1u << a.log_lanes, sub = lane >> a.log_lanes, per_pass = 32u >> a.log_lanes;
   const P part(lane & (lanes - 1), lanes, sub, a.cols);
@@ -173,9 +176,13 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
       float2 s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {  // g is zero for values that are not the row's
-        float2 &sw = kTwice ? tile_w[kTwice ? i : 0] : dw[i], &sb = kTwice ? tile_b[kTwice ? i : 0] : db[i];
-        sw = fma2(g[i], h[i], sw);
-        sb = add2(sb, g[i]);
+        if constexpr (kTwice) {
+          tile_w[i] = fma2(g[i], h[i], tile_w[i]);
+          tile_b[i] = add2(tile_b[i], g[i]);
+        } else {
+          dw[i] = fma2(g[i], h[i], dw[i]);
+          db[i] = add2(db[i], g[i]);
+        }
       }
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
@@ -252,11 +259,9 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
   float* out = a.partial + (uint64_t)blockIdx.x * 2 * a.cols;
   // lanes with the same columns (their runs turned differently), then the
   // warps, each in order, through the rings' memory; where a warp gave up, whose copies
-  // may still be on their way there, the sums are marked invalid instead
-  if (!__syncthreads_and(ok)) {
-    for (uint32_t c = threadIdx.x; c < 2 * a.cols; c += NORM_WARPS * 32) out[c] = nan_value();
-    return;
-  }
+  // may still be on their way there, the sums are marked invalid
+  if (lane == 0) gave_up[warp] = ok ? 0u : 1u;
+  __syncthreads();
   float* sums = reinterpret_cast<float*>(smem);  // [warp][2][cols]
   float* mine = sums + warp * 2 * a.cols;
   for (uint32_t k = 0; k < per_pass; ++k) {
@@ -276,8 +281,12 @@ __global__ void __launch_bounds__(NORM_WARPS * 32, warp_ctas<T, VEC, K>())
   __syncthreads();
   for (uint32_t c = threadIdx.x; c < 2 * a.cols; c += NORM_WARPS * 32) {
     float v = sums[c];
-    for (uint32_t k = 1; k < NORM_WARPS; ++k) v += sums[k * 2 * a.cols + c];
-    out[c] = v;
+    uint32_t late = gave_up[0];
+    for (uint32_t k = 1; k < NORM_WARPS; ++k) {
+      v += sums[k * 2 * a.cols + c];
+      late |= gave_up[k];
+    }
+    out[c] = late ? nan_value() : v;
   }
 }
 
@@ -328,7 +337,9 @@ template <typename T, int VEC, int K, bool kJoin> vs_status run_kernel(vs_ctx* c
   a.err = ctx->d_err;
   const uint64_t most = ((a.rows + a.tile_rows - 1) / a.tile_rows + NORM_WARPS - 1) / NORM_WARPS;
   const uint64_t once = (uint64_t)per_sm * B200_SMS;
-  const uint64_t chain = NORM_CHAIN * (sums_twice<VEC, K> ? a.tile_rows : per_pass);  // a warp's rows at most
+  // A warp's rows at most.  Another wave of warps costs about 20 us (12.5M x 8 bf16 139 us,
+  // in two waves 162), so lanes of many values take four times the chain.
+  const uint64_t chain = NORM_CHAIN * (sums_twice<VEC, K> ? a.tile_rows : 4 * per_pass);
   const uint64_t all = once * (a.rows / (once * NORM_WARPS * chain) + 1);
   const uint32_t grid = (uint32_t)(all < most ? all : most);
   const bool want = f.dweight || f.dbias;
